@@ -21,6 +21,18 @@ RSFA_DTYPE_BF16 = 1
 RSFA_PATH_GENERIC = 0
 RSFA_PATH_TCGEN05 = 1
 
+RSFA_ROTARY = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+class Cache4(ctypes.Structure):
+    """rsfa_cache4 of include/rsfa.h."""
+    _fields_ = [("kv", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("position", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("kv_stride", ctypes.c_int64 * 2), ("weight_stride", ctypes.c_int64 * 2),
+                ("position_stride", ctypes.c_int64 * 2), ("table_stride", ctypes.c_int64)] + [
+                    (n, ctypes.c_int) for n in ("batch", "heads", "head_dim", "page_size", "pages", "max_pages", "dtype")]
+
+
 # name -> (restype, argtypes); mirrors include/rsfa.h one to one
 _c = ctypes
 SIGNATURES = {
@@ -33,6 +45,22 @@ SIGNATURES = {
     "rsfa_fwd_noalloc": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                     _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_int64),
                                     _c.c_int, _c.c_float, _c.c_int, _c.c_void_p]),
+    "rsfa_rotary_table": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int, _c.c_double, _c.c_int, _c.c_double, _c.c_int,
+                                     _c.c_double, _c.c_double, _c.c_double, _c.c_void_p]),
+    "rsfa_rotary": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 5 + [_c.POINTER(_c.c_int64), _c.c_void_p, _c.c_int,
+                               _c.c_int, _c.c_void_p, _c.c_int, _c.POINTER(_c.c_int64), _c.c_int, _c.c_int, _c.c_int,
+                               _c.c_void_p]),
+    "rsfa_cache4_append": (_c.c_int, [_c.POINTER(Cache4), _c.c_void_p, _c.c_void_p, _c.c_int, _c.POINTER(_c.c_int64),
+                                      _c.c_void_p, _c.c_void_p, _c.POINTER(_c.c_int64), _c.c_void_p]),
+    "rsfa_cache4_read": (_c.c_int, [_c.POINTER(Cache4), _c.c_void_p, _c.c_void_p, _c.c_int, _c.POINTER(_c.c_int64),
+                                    _c.c_void_p, _c.c_void_p]),
+    "rsfa_cache4_attention_workspace": (_c.c_longlong, [_c.c_int] * 4),
+    "rsfa_cache4_attention": (_c.c_int, [_c.POINTER(Cache4), _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int,
+                                         _c.POINTER(_c.c_int64), _c.c_void_p, _c.c_float, _c.c_void_p, _c.c_longlong,
+                                         _c.c_void_p]),
+    "rsfa_cache4_evict_workspace": (_c.c_longlong, [_c.c_int] * 3),
+    "rsfa_cache4_evict": (_c.c_int, [_c.POINTER(Cache4), _c.c_int, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_longlong,
+                                     _c.c_void_p]),
     "rsfa_get_tiling": (_c.c_int, [_c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int,
                                    _c.POINTER(_c.c_int), _c.POINTER(_c.c_int)]),
     "rsfa_select_path": (_c.c_int, [_c.c_int, _c.c_int, _c.c_int, _c.c_float, _c.c_int, _c.c_int,

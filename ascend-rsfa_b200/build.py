@@ -32,8 +32,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "ascend_rsfa", "librsfa_b200.so")
 OUT_TRACE = os.path.join(HERE, "ascend_rsfa", "librsfa_b200_trace.so")
-SOURCES = ["rsfa_api.cu", "fwd_generic.cu", "fwd_tcgen05.cu", "fwd_tcgen05_db.cu", "fwd_tcgen05_sp.cu", "fwd_short.cu"]
-HEADERS = ["common.cuh", "ptx_sm100.cuh", "tcgen05_common.cuh", "tile_table.inc", os.path.join("..", "..", "include", "rsfa.h")]
+SOURCES = ["rsfa_api.cu", "fwd_generic.cu", "fwd_tcgen05.cu", "fwd_tcgen05_db.cu", "fwd_tcgen05_sp.cu", "fwd_short.cu",
+           "ops_api.cu", "rotary.cu", "cache4_rows.cu", "cache4_attention.cu", "cache4_evict.cu"]
+HEADERS = ["common.cuh", "ptx_sm100.cuh", "tcgen05_common.cuh", "ops_common.cuh", "tile_table.inc", os.path.join("..", "..", "include", "rsfa.h")]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-cudart", "static",

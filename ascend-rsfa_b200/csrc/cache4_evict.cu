@@ -1,0 +1,228 @@
+// Eviction from a paged cache of 4-bit records by accumulated attention weight.
+//
+// Of the n tokens of a sequence, every K/V head keeps `budget`: those whose position is among the newest `recent`
+// ones (position > newest - recent), then those with the largest weight, the lowest slot first among equals.  The
+// kept tokens beyond slot `budget` move into the slots below it that are given up, both in rising order, so nothing
+// else moves and the order of the others stays; attention does not depend on the order.
+//
+// Two launches.  select: one CTA per (sequence, head) finds the budget-th largest key with three histograms of 11,
+// 11 and 10 bits (a weight is not negative, so its bits order as an integer; a protected token has the largest key) and
+// lists the moves by prefix sums over the slots.  move: the listed records, spread over the whole device.
+// What bounds it: the latency of the passes over n keys of one CTA; the traffic, 8 bytes per token and 2 * 5 D / 4 per
+// move, is small next to a step's attention.
+#include "../../include/rsfa.h"
+#include "ops_common.cuh"
+
+namespace rsfa {
+namespace {
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSlotsEach = 4;              // neighbouring slots of a thread in the listing pass
+constexpr int kBins = 2048;
+constexpr int kKeysInShared = 40 * 1024;   // keys kept in shared memory; longer sequences read them again
+constexpr int kMoveThreads = 256;
+constexpr uint32_t kProtected = 0xffffffffu;
+
+__device__ __forceinline__ int64_t moves_at(const Cache4Evict& e, int bh) { return static_cast<int64_t>(bh) * (2ll * e.budget + 2); }
+
+// Exclusive prefix sum over the block and the block's total.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t sum = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += u;
+  }
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  uint32_t w = warp_sums[lane];                 // 32 warps
+  uint32_t ws = w;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, ws, d);
+    if (lane >= d) ws += u;
+  }
+  *total = __shfl_sync(0xffffffffu, ws, 31);
+  const uint32_t before = __shfl_sync(0xffffffffu, ws - w, warp);
+  __syncthreads();                              // warp_sums may be written again
+  return before + sum - v;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) cache4_select_kernel(const Cache4 c, const Cache4Evict e) {
+  extern __shared__ uint32_t keys[];            // min(n, kKeysInShared)
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t warp_sums[32];
+  __shared__ int newest_word;
+  __shared__ uint32_t found_bin, found_above;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int bh = blockIdx.x, b = bh / c.H, h = bh - b * c.H;
+  const int tid = threadIdx.x;
+  const int n = tokens_of(c, b);
+  int* count = e.moves + moves_at(e, bh);
+  int2* moves = reinterpret_cast<int2*>(count + 2);
+  if (tid == 0 && h == 0) e.new_lengths[b] = min(n, e.budget);
+  if (n <= e.budget) {
+    if (tid == 0) *count = 0;
+    return;
+  }
+  const int mask = (1 << c.page_shift) - 1;
+  auto position_of = [&](int slot) {
+    int64_t page;
+    if (!find_page(c, b, slot, &page)) return INT_MIN;
+    return c.position[page * c.position_stride[0] + h * c.position_stride[1] + (slot & mask)];
+  };
+  if (tid == 0) newest_word = INT_MIN;
+  __syncthreads();
+  int newest = INT_MIN;
+  for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, position_of(i));
+  newest = __reduce_max_sync(0xffffffffu, newest);
+  if ((tid & 31) == 0) atomicMax(&newest_word, newest);
+  __syncthreads();
+  const long long oldest_kept = static_cast<long long>(newest_word) - e.recent;
+  auto key_of = [&](int slot) -> uint32_t {
+    int64_t page;
+    if (!find_page(c, b, slot, &page)) return 0u;
+    const int pos = c.position[page * c.position_stride[0] + h * c.position_stride[1] + (slot & mask)];
+    const float w = c.weight[page * c.weight_stride[0] + h * c.weight_stride[1] + (slot & mask)];
+    if (static_cast<long long>(pos) > oldest_kept) return kProtected;
+    return w > 0.f ? __float_as_uint(w) : 0u;   // NaN, negative: as no weight
+  };
+  for (int i = tid; i < min(n, kKeysInShared); i += kSelectThreads) keys[i] = key_of(i);
+  auto key_at = [&](int slot) { return slot < kKeysInShared ? keys[slot] : key_of(slot); };
+
+  // ---- the budget-th largest key, by digits from the top
+  uint32_t prefix = 0, want = e.budget;         // `want` keys are to come from those that share the prefix
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t digit_mask = pass == 2 ? 1023u : 2047u;
+    const uint32_t above = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;
+    for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelectThreads) {
+      const uint32_t key = key_at(i);
+      if (((key ^ prefix) & above) == 0) atomicAdd(&hist[(key >> shift) & digit_mask], 1u);
+    }
+    __syncthreads();
+    // two bins per thread, from the highest down
+    const int hi = kBins - 1 - 2 * tid;
+    const uint32_t a = hist[hi], d = hist[hi - 1];
+    uint32_t total;
+    const uint32_t before = block_scan(a + d, warp_sums, &total);
+    if (before < want && want <= before + a) {
+      found_bin = hi;
+      found_above = before;
+    } else if (before + a < want && want <= before + a + d) {
+      found_bin = hi - 1;
+      found_above = before + a;
+    }
+    __syncthreads();
+    prefix |= found_bin << shift;
+    want -= found_above;
+  }
+
+  // ---- kept: larger keys, and the first `want` slots of equal ones; the moves in rising order
+  uint32_t equals = 0, holes = 0, movers = 0;
+  for (int base = 0; base < n; base += kSelectThreads * kSlotsEach) {
+    const int first = base + tid * kSlotsEach;
+    uint32_t key[kSlotsEach], eq = 0;
+#pragma unroll
+    for (int j = 0; j < kSlotsEach; ++j) {
+      key[j] = first + j < n ? key_at(first + j) : 0u;
+      eq += first + j < n && key[j] == prefix;
+    }
+    uint32_t total;
+    uint32_t rank = equals + block_scan(eq, warp_sums, &total);
+    equals += total;
+    uint32_t is_hole = 0, is_mover = 0;
+#pragma unroll
+    for (int j = 0; j < kSlotsEach; ++j) {
+      const int slot = first + j;
+      if (slot < n) {
+        const bool same = key[j] == prefix;
+        const bool kept = key[j] > prefix || (same && rank < want);
+        rank += same;
+        if (slot < e.budget && !kept) is_hole |= 1u << j;
+        if (slot >= e.budget && kept) is_mover |= 1u << j;
+      }
+    }
+    // both counts of a block's 4096 slots in one word
+    const uint32_t at = block_scan(__popc(is_hole) | (__popc(is_mover) << 16), warp_sums, &total);
+    uint32_t hole_at = holes + (at & 0xffffu), mover_at = movers + (at >> 16);
+#pragma unroll
+    for (int j = 0; j < kSlotsEach; ++j) {
+      if (is_hole >> j & 1) moves[hole_at++].x = first + j;
+      if (is_mover >> j & 1) moves[mover_at++].y = first + j;
+    }
+    holes += total & 0xffffu;
+    movers += total >> 16;
+  }
+  if (tid == 0) *count = static_cast<int>(holes);   // as many as movers: budget slots are kept
+}
+
+// Pieces of 16 bytes, and one more per record for its weight and position.
+__global__ void __launch_bounds__(kMoveThreads) cache4_move_kernel(const Cache4 c, const Cache4Evict e, const int pieces) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int bh = blockIdx.x, b = bh / c.H, h = bh - b * c.H;
+  const int* count = e.moves + moves_at(e, bh);
+  const int2* moves = reinterpret_cast<const int2*>(count + 2);
+  const long long total = static_cast<long long>(*count) * pieces;
+  const int mask = (1 << c.page_shift) - 1;
+  for (long long i = static_cast<long long>(blockIdx.y) * kMoveThreads + threadIdx.x; i < total; i += static_cast<long long>(gridDim.y) * kMoveThreads) {
+    const int m = static_cast<int>(i / pieces), piece = static_cast<int>(i - static_cast<long long>(m) * pieces);
+    const int2 move = moves[m];                 // to, from
+    int64_t to, from;
+    if (!find_page(c, b, move.x, &to) || !find_page(c, b, move.y, &from)) continue;
+    if (piece < pieces - 1) {
+      const int64_t rec = 16ll * (pieces - 1);
+      const uint8_t* src = c.kv + from * c.kv_stride[0] + h * c.kv_stride[1] + (move.y & mask) * rec + 16 * piece;
+      uint8_t* dst = c.kv + to * c.kv_stride[0] + h * c.kv_stride[1] + (move.x & mask) * rec + 16 * piece;
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+    } else {
+      c.weight[to * c.weight_stride[0] + h * c.weight_stride[1] + (move.x & mask)] =
+          c.weight[from * c.weight_stride[0] + h * c.weight_stride[1] + (move.y & mask)];
+      c.position[to * c.position_stride[0] + h * c.position_stride[1] + (move.x & mask)] =
+          c.position[from * c.position_stride[0] + h * c.position_stride[1] + (move.y & mask)];
+    }
+  }
+}
+
+}  // namespace
+
+size_t cache4_evict_workspace(int B, int H, int budget) {
+  return static_cast<size_t>(B) * H * (2ull * budget + 2) * sizeof(int);
+}
+
+cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& ev, int sm_count, cudaStream_t stream, long long* launches) {
+  const long long room = static_cast<long long>(c.max_pages) << c.page_shift;
+  const int smem = static_cast<int>(room < kKeysInShared ? room : kKeysInShared) * 4;
+  static std::atomic<unsigned long long> smem_done{0};
+  cudaError_t e = set_dynamic_smem_once(smem_done, reinterpret_cast<const void*>(cache4_select_kernel), kKeysInShared * 4);
+  if (e != cudaSuccess) return e;
+  const int heads = c.B * c.H;
+  e = launch_persistent(cache4_select_kernel, heads, kSelectThreads, smem, stream, option_pdl() != 0, c, ev);
+  if (e != cudaSuccess) return e;
+  *launches += 1;
+  const int pieces = c.D * 5 / 4 / 16 + 1;
+  // enough CTAs for a large cut, and no more than its moves could keep busy
+  long long each = (8ll * sm_count + heads - 1) / heads;
+  const long long most = (static_cast<long long>(ev.budget) * pieces + kMoveThreads - 1) / kMoveThreads;
+  if (each > most) each = most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(heads), static_cast<unsigned>(each < 1 ? 1 : each));
+  cfg.blockDim = dim3(kMoveThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = option_pdl() ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, cache4_move_kernel, c, ev, pieces);
+  if (e == cudaSuccess) *launches += 1;
+  return e;
+}
+
+}  // namespace rsfa

@@ -41,6 +41,77 @@ struct FwdParams {
 #endif
 };
 
+// A paged cache of 4-bit records (see rsfa_cache4 in rsfa.h) as the kernels see it.
+struct Cache4 {
+  uint8_t* kv;
+  float* weight;        // may be null
+  int* position;        // may be null
+  const int* table;     // [B][max_pages] page of every page_size slots
+  const int* lengths;   // [B]
+  int64_t kv_stride[2];        // bytes: page, head
+  int64_t weight_stride[2];    // elements: page, head
+  int64_t position_stride[2];
+  int64_t table_stride;        // elements: sequence
+  int B, H, D, pages, max_pages;
+  int page_shift;              // page_size = 1 << page_shift
+  int bf16;
+  int* status;                 // device status word, never null
+};
+
+struct RotaryParams {
+  const void* x[2];        // q and k; k may be absent (heads[1] = 0)
+  void* y[2];
+  int64_t x_stride[2][3];  // batch, head, row
+  int64_t y_stride[2][3];
+  int heads[2];
+  const float* table;      // [table_length][R / 2][2]: cosine and sine
+  const void* positions;   // may be null: 0 .. S - 1
+  int positions_64;        // int64 instead of int32
+  int64_t pos_stride[2];   // batch, row
+  int B, S, D, R, table_length;
+  int interleaved, inverse, bf16;
+  int* status;
+};
+
+struct Cache4Rows {        // dense K and V rows that go into or come out of a cache
+  void* k;
+  void* v;
+  int64_t k_stride[3];     // batch, head, row
+  int64_t v_stride[3];
+  int S;
+  const int* counts;       // append: rows of each sequence that count; may be null: all
+  const int* starts;       // read: first slot of each sequence; may be null: 0
+  const int* positions;    // append: may be null
+  int64_t positions_stride[2];
+};
+
+struct Cache4Attention {
+  const void* q;
+  void* o;
+  float* lse;              // may be null
+  int64_t q_stride[3], o_stride[3];
+  int Hq, S;
+  const int* counts;       // may be null
+  float sm_scale;
+  float* pieces;           // workspace
+};
+
+struct Cache4Evict {
+  int budget, recent;
+  int* new_lengths;
+  int* moves;              // workspace
+};
+
+// What a call needs of the current device: multiprocessors and the status word.  begin_call refuses under the
+// "check_status" option as rsfa_fwd does; end_call turns a launch's outcome into a return code.
+struct CallScratch {
+  int sm_count;
+  int* status;
+  int* status_mirror;
+};
+int begin_call(CallScratch* out);
+int end_call(const CallScratch& d, cudaStream_t stream, cudaError_t e, long long launches);
+
 // Raises a kernel's dynamic shared-memory limit once per device instead of on every call (the
 // attribute stays with the function in that device's context).  `done` is a bit mask by device
 // ordinal, one per kernel instantiation (a static of the launcher that owns the kernel).
@@ -79,6 +150,16 @@ bool tcgen05_sp_fits(const FwdParams& p);
 // request / table decide, 0 forces 128-key tiles with single-buffered S, 1 forces 64-key tiles (D <= 128
 // only), 2 forces 128-key tiles with the separate-P kernel where it exists (D = 64).
 void tcgen05_resolve_tile(int S, int D, int causal, int req_bm, int req_bn, int variant, int* bm, int* bn);
+// The operators around attention (rotary.cu, cache4_rows.cu, cache4_attention.cu, cache4_evict.cu).
+cudaError_t launch_rotary(const RotaryParams& p, int sm_count, cudaStream_t stream, long long* launches);
+cudaError_t launch_rotary_table(float* table, int length, int dim, const double* freq_args, int scaling, cudaStream_t stream,
+                                long long* launches);
+cudaError_t launch_cache4_append(const Cache4& c, const Cache4Rows& r, cudaStream_t stream, long long* launches);
+cudaError_t launch_cache4_read(const Cache4& c, const Cache4Rows& r, cudaStream_t stream, long long* launches);
+cudaError_t launch_cache4_attention(const Cache4& c, const Cache4Attention& a, int sm_count, cudaStream_t stream, long long* launches);
+size_t cache4_attention_workspace(int D, int Hq, int H, int S, int sm_count);
+cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& e, int sm_count, cudaStream_t stream, long long* launches);
+size_t cache4_evict_workspace(int B, int H, int budget);
 // Adds to the process-wide kernel-launch counter behind rsfa_launch_count().
 void count_launches(long long n);
 // Current values of the "wait_limit_ms" (in ns), "pdl" and "test_drop_load" options.

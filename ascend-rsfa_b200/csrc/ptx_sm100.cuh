@@ -56,6 +56,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 enum : int {
   kStatusOk = 0,
   kStatusWaitExpired = 1,  // a bounded wait ran out; low bits say which role
+  kStatusBadIndex = 2,     // an index in device memory was out of range; low bits say which
+};
+enum : int {
+  kTagRotaryPosition = 1,  // a position outside the rotary table
+  kTagCachePage = 2,       // a page number outside the cache
+  kTagCacheLength = 3,     // a length that is negative or more than the sequence's pages hold
 };
 
 // try_wait with an explicit suspend-time hint: the hardware may park the thread for up to

@@ -126,6 +126,33 @@ unsigned long long option_wait_limit_ns() {
 }
 int option_pdl() { return static_cast<int>(g_pdl.load()); }
 int option_test_drop_load() { return static_cast<int>(g_test_drop_load.load()); }
+
+int begin_call(CallScratch* out) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) {
+    cudaGetLastError();
+    return RSFA_ERR_NO_DEVICE;
+  }
+  DeviceState* d = nullptr;
+  const int rc = ensure_device(device, &d);
+  if (rc != RSFA_OK) return rc;
+  if (g_check_status.load() != 0 && *static_cast<volatile int*>(d->status_mirror) != 0) return RSFA_ERR_DEVICE_STATUS;
+  out->sm_count = d->sm_count;
+  out->status = d->status;
+  out->status_mirror = d->status_mirror;
+  return RSFA_OK;
+}
+
+int end_call(const CallScratch& d, cudaStream_t stream, cudaError_t e, long long launches) {
+  g_launches.fetch_add(launches);
+  if (e == cudaSuccess && g_check_status.load() != 0)
+    e = cudaMemcpyAsync(d.status_mirror, d.status, sizeof(int), cudaMemcpyDeviceToHost, stream);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return RSFA_ERR_CUDA;
+  }
+  return RSFA_OK;
+}
 }  // namespace rsfa
 
 extern "C" {
@@ -138,7 +165,7 @@ const char* rsfa_strerror(int code) {
     case RSFA_ERR_INVALID_ARGUMENT: return "invalid argument (shape, stride, alignment, tile or dtype)";
     case RSFA_ERR_UNSUPPORTED: return "unsupported configuration";
     case RSFA_ERR_CUDA: return "CUDA call failed";
-    case RSFA_ERR_DEVICE_STATUS: return "a kernel reported a non-zero device status (bounded wait expired)";
+    case RSFA_ERR_DEVICE_STATUS: return "a kernel reported a non-zero device status (bounded wait expired, or an index out of range)";
     case RSFA_ERR_NO_DEVICE: return "no usable sm_100 CUDA device";
     case RSFA_ERR_TOO_LARGE: return "problem too large: beyond the fixed scratch of the allocation-free entry point, or more CTAs than a grid holds";
     default: return "unknown error code";

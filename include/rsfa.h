@@ -128,6 +128,113 @@ RSFA_API int rsfa_fwd_noalloc(const void* q, const void* k, const void* v, void*
                               int causal, float sm_scale, int dtype, void* stream);
 
 /*
+ * ---------------------------------------------------------------------------------------------
+ * Around attention: rotary positions, and a paged cache that holds K and V in 4 bits for decoding.
+ * The reference has no counterpart.  All calls are asynchronous on `stream`, run on the current
+ * device, allocate nothing (but the library's workspace on a device's first call, which therefore
+ * is made outside stream capture) and keep nothing from one call for the next; scratch is the
+ * caller's, and a scratch buffer belongs to one call at a time.  What lies in device memory cannot
+ * be checked when a call is made: a position, page number or length that is out of range is skipped by
+ * the kernel that finds it and leaves (2 << 16) | tag in the status word (rsfa_device_status): tag
+ * 1 a position outside the rotary table, 2 a page outside the cache, 3 a length below zero or beyond the
+ * sequence's pages.
+ */
+
+/* How the angles of rotary positions are scaled for contexts longer than those of training. */
+#define RSFA_ROTARY_NONE 0
+#define RSFA_ROTARY_LINEAR 1 /* every angle divided by factor                                        */
+#define RSFA_ROTARY_NTK 2    /* base times factor^(dim / (dim - 2)); dim = 2: as LINEAR               */
+#define RSFA_ROTARY_YARN 3   /* a ramp over the pairs, from unscaled to divided by factor, between    */
+                             /* those with high_turns and low_turns turns over original_length        */
+#define RSFA_ROTARY_BANDS 4  /* the same between the two numbers of turns, linear in the turns        */
+
+/*
+ * The table of a rotation: table[p][i] = multiplier * (cos, sin)(p * f_i) for positions p < length and
+ * pairs i < dim / 2, fp32, from angles in 64 bits; f_i = base^(-2 i / dim), scaled as asked for.
+ * table: device, 16-byte aligned, length * dim floats; dim even, 2 ... 256; base > 1.  factor counts
+ * unless scaling is NONE, original_length and the turns (0 < low_turns < high_turns) for YARN and BANDS.
+ */
+RSFA_API int rsfa_rotary_table(float* table, int length, int dim, double base, int scaling, double factor,
+                               int original_length, double low_turns, double high_turns, double multiplier,
+                               void* stream);
+
+/*
+ * Rotary positions on q [B,Hq,S,D] and k [B,Hk,S,D] in one launch (k and k_out NULL with Hk = 0: q alone).
+ * The pair (a, b) of frequency i becomes (a c - b s, b c + a s), (c, s) = table[position][i]; pairs are
+ * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved; dims from rotary_dim on are copied.  inverse: the
+ * transposed rotation, which is the gradient.  strides: 16 element strides, q[4], k[4], q_out[4], k_out[4], as
+ * rsfa_fwd asks for them; outputs do not overlap inputs.  rotary_dim: even, 2 ... D; multiples of 16 (8 if
+ * interleaved) are fast.  positions: int32 (int64 if positions_64) with element strides (batch, row), 0 for
+ * a row that all sequences share; NULL: 0 ... S - 1.  A row whose position is outside the table comes out as NaN.
+ */
+RSFA_API int rsfa_rotary(const void* q, const void* k, void* q_out, void* k_out, int B, int Hq, int Hk, int S, int D,
+                         const int64_t* strides, const float* table, int table_length, int rotary_dim,
+                         const void* positions, int positions_64, const int64_t* position_strides, int interleaved,
+                         int inverse, int dtype, void* stream);
+
+/*
+ * A paged cache of 4-bit records.  Slot s of sequence b lies in page table[b * table_stride + s / page_size], row
+ * s % page_size; lengths[b] slots are in use.  A record (one token of one K/V head) is 5 head_dim / 4 bytes:
+ * head_dim / 2 of K codes, as many of V codes, then for K and for V a (scale, minimum) pair of `dtype` per group of
+ * 32 dims; a value is scale * code + minimum.  The order of the codes is the kernels' own (csrc/ops_common.cuh).
+ * head_dim 64, 128 or 256; page_size a power of two, 16 ... 1024; kv 16-byte aligned, its strides (bytes: page, head)
+ * multiples of 16, a head's rows of a page contiguous.  weight (fp32) and position (int32), one per record with element
+ * strides (page, head), are NULL where a call does not use them.  Sequences may share pages that are only read.
+ */
+typedef struct rsfa_cache4 {
+  void* kv;
+  float* weight;
+  int* position;
+  const int* table;
+  const int* lengths;
+  int64_t kv_stride[2];
+  int64_t weight_stride[2];
+  int64_t position_stride[2];
+  int64_t table_stride;
+  int batch, heads, head_dim, page_size, pages, max_pages, dtype;
+} rsfa_cache4;
+
+/*
+ * K and V rows [B,heads,S,D] into the last slots of each sequence: row j < counts[b] (NULL: S) goes to slot
+ * lengths[b] - counts[b] + j, so lengths is what they are WITH the new rows; slots below zero are left out.  Per group the
+ * minimum, the scale 16-bit((max - min) / 15) and the nearest codes; a group that holds an infinity or NaN reads back
+ * as NaN.  weight is set to 0 and position to positions[b][j] (element strides; given if position is).
+ * strides: 8 element strides, k[4], v[4], as rsfa_fwd asks for them.
+ */
+RSFA_API int rsfa_cache4_append(const rsfa_cache4* cache, const void* k, const void* v, int S, const int64_t* strides,
+                                const int* counts, const int* positions, const int64_t* position_strides, void* stream);
+
+/* Slots starts[b] (NULL: 0) ... + N - 1 back to dense K and V rows [B,heads,N,D]; slots not in use are zero. */
+RSFA_API int rsfa_cache4_read(const rsfa_cache4* cache, void* k, void* v, int N, const int64_t* strides,
+                              const int* starts, void* stream);
+
+/*
+ * Attention of the last counts[b] (NULL: S) tokens of each sequence over its cache: query i of q [B,q_heads,S,D] sees the
+ * slots up to lengths[b] - counts[b] + i, its own among them (append comes first).  q_heads is a multiple of heads;
+ * K/V head h serves the query heads h * q_heads / heads ... .  o like q, both of cache->dtype; a row that sees nothing
+ * (a sequence of length zero, a row of padding) is zero, its lse -infinity.  lse: [B,q_heads,S] fp32, natural log, may
+ * be NULL unless cache->weight is given: weight[slot] then grows by the softmax weights that the token gets from all
+ * query rows of its K/V head.  Results do not depend on timing.  strides: 8 element strides, q[4], o[4].
+ * workspace: rsfa_cache4_attention_workspace bytes (or a negative error), 16-byte aligned, no content asked for.
+ */
+RSFA_API long long rsfa_cache4_attention_workspace(int head_dim, int q_heads, int heads, int S);
+RSFA_API int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, float* lse, int q_heads, int S,
+                                   const int64_t* strides, const int* counts, float sm_scale, void* workspace,
+                                   long long workspace_bytes, void* stream);
+
+/*
+ * Cuts every sequence back to `budget` slots, for each K/V head on its own: kept are the tokens at the newest `recent`
+ * positions (position > largest - recent), then those of the largest weight, the lowest slot first among equals; a
+ * weight that is negative or NaN counts as none.  Kept records beyond slot `budget` move, with weight and position, into
+ * the slots below that are given up, both in rising order; nothing else is written.  new_lengths[b] =
+ * min(lengths[b], budget), which is not lengths itself: other layers' caches may still need that.  0 <= recent <= budget.
+ * No page may belong to two sequences.  workspace as above.
+ */
+RSFA_API long long rsfa_cache4_evict_workspace(int batch, int heads, int budget);
+RSFA_API int rsfa_cache4_evict(const rsfa_cache4* cache, int budget, int recent, int* new_lengths, void* workspace,
+                               long long workspace_bytes, void* stream);
+
+/*
  * Tile lookup.  Replaces get_tiling (:624-665): the reference keys a 32-entry dict by the full
  * (Z, H, N_CTX, HEAD_DIM, causal) tuple and raises KeyError otherwise; here the table is keyed by
  * (S, D, causal) only, any B and H are accepted, and only tiles that are instantiated are returned.
@@ -163,7 +270,7 @@ RSFA_API int rsfa_sm_count(int device);
  * Synchronise `device` and return the status word its kernels share (this call allocates nothing
  * and reads only the scratch that rsfa_fwd or rsfa_fwd_noalloc has already set up on the device): RSFA_OK, or
  * RSFA_ERR_DEVICE_STATUS with the raw word in *raw (if not NULL): (1 << 16) | tag, where tag names
- * the wait that ran out.  Reading clears the word.  rsfa_fwd itself returns RSFA_OK for a call
+ * the wait that ran out, or (2 << 16) | tag, see above, for an index out of range.  Reading clears the word.  rsfa_fwd itself returns RSFA_OK for a call
  * whose kernel later gives up (the launch is asynchronous) and the output of that call is then
  * incomplete: callers that care call this function at their synchronisation points, or set the
  * "check_status" option, under which every rsfa_fwd copies the word to the host behind its kernels
