@@ -23,10 +23,22 @@ namespace rsfa {
 namespace {
 
 constexpr int kTile = 32;            // tokens per tile
-constexpr int kWarps = 8;            // per CTA
+constexpr int kWarps = 4;            // per CTA
 constexpr int kThreads = 32 * kWarps;
-constexpr int kCtasPerSm = 1;
 constexpr int kJoinThreads = 128;
+#ifndef C4_CTAS128
+#define C4_CTAS128 4
+#define C4_STAGES128 2
+#endif
+// CTAs per multiprocessor by the registers of their accumulators, and slots of a warp's ring by its shared memory.
+template <int D, int NT>
+struct Shape {
+  static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : C4_CTAS128;
+  static constexpr int kStages = D == 64 ? 4 : D == 256 ? 2 : NT == 2 ? 4 : C4_STAGES128;
+  static constexpr int kSlotBytes = kTile * Record<D>::kBytes;
+  static constexpr int kRingBytes = kWarps * kStages * kSlotBytes;
+};
+constexpr int kTagCache4Load = 40;   // of a bounded wait, in the status word
 constexpr float kRaise = 8.f;        // log2 units above the reference at which it is raised
 constexpr float kRaiseScale = 64.f;  // and the scales' one
 
@@ -44,6 +56,12 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+
+// Global to this CTA's shared memory, both 16-byte aligned, counted in bytes on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bar, uint32_t bytes) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 // ------------------------------------------------------------------ the list of tiles
@@ -454,47 +472,138 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
   }
 }
 
+// A place in the list of tiles: item `item` of sequence b, tile t of `tiles`.
+struct Cursor {
+  int b, n, tiles, item, t;
+  long long left;          // tiles of the share from here on
+};
+__device__ __forceinline__ Cursor cursor_at(const Cache4& c, const int* counts, int per_sequence, long long at, long long end) {
+  Cursor k;
+  long long first;
+  k.b = sequence_of(c, counts, per_sequence, at, &first, &k.tiles);
+  k.n = tokens_of(c, k.b);
+  k.item = static_cast<int>((at - first) / k.tiles);
+  k.t = static_cast<int>(at - first - static_cast<long long>(k.item) * k.tiles);
+  k.left = end - at;
+  return k;
+}
+__device__ __forceinline__ void advance(Cursor& k, const Cache4& c, const int* counts, int per_sequence) {
+  --k.left;
+  if (++k.t < k.tiles || k.left == 0) return;
+  k.t = 0;
+  if (++k.item < per_sequence) return;
+  k.item = 0;
+  do {                     // the next sequence that has tokens: there is one, tiles are left
+    k.tiles = tiles_of(c, counts, ++k.b);
+  } while (k.tiles == 0);
+  k.n = tokens_of(c, k.b);
+}
+
+// Every warp works for itself: a ring of tiles in shared memory, which its first lane fills with bulk copies as soon
+// as the warp is done with a slot, across the items of its share.
 template <int D, int NT, bool kBf16>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) cache4_attention_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks) {
+__global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attention_kernel(const Cache4 c, const Cache4Attention a, const Rows rows,
+                                                                                        const int row_blocks, const unsigned long long wait_limit_ns) {
   using R = Record<D>;
+  using Sh = Shape<D, NT>;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t full_bar[kWarps * Sh::kStages];
+  __shared__ int abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < kWarps * Sh::kStages) mbar_init(smem_u32(&full_bar[threadIdx.x]), 1);
+  if (threadIdx.x == 0) abort_word = 0;
+  fence_barrier_init();
+  fence_proxy_async();
+  __syncthreads();
   griddep_launch_dependents();
   griddep_wait();
   const int per_sequence = c.H * row_blocks;
   const long long total = tiles_before(c, a.counts, c.B) * per_sequence;
   const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
   if (worker >= workers) return;
-  long long at = share_begin(total, worker, workers);
-  const long long end = share_begin(total, worker + 1, workers);
-  long long first;
-  int tiles;
-  int b = sequence_of(c, a.counts, per_sequence, at, &first, &tiles);
-  while (at < end) {
-    if (at >= first + static_cast<long long>(tiles) * per_sequence) b = sequence_of(c, a.counts, per_sequence, at, &first, &tiles);
-    const int item = static_cast<int>((at - first) / tiles);
-    const int t0 = static_cast<int>(at - first - static_cast<long long>(item) * tiles);
-    const int t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + end - at));
-    const int h = item / row_blocks, row0 = (item - h * row_blocks) * 8 * NT;
-    const int n = tokens_of(c, b);
+  Cursor use = cursor_at(c, a.counts, per_sequence, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  Cursor load = use;
+  const uint8_t* const my_ring = ring + warp * Sh::kStages * Sh::kSlotBytes;
+  const uint32_t my_bar = smem_u32(&full_bar[warp * Sh::kStages]);
+  const int mask = (1 << c.page_shift) - 1;
+  const bool split = c.page_shift == 4;    // a tile is two pages
+
+  // Pages of tiles window .. window + 31 of sequence window_b, one per lane (two where a tile is two pages).
+  int window_b = -1, window = 0, page_lo = 0, page_hi = 0;
+  uint32_t have = 0;                       // two bits per slot: which halves of its tile are there
+  auto issue = [&](int stage) {
+    if (load.b != window_b || load.t < window || load.t >= window + 32) {
+      window_b = load.b;
+      window = load.t;
+      const int slot = (window + lane) * kTile;
+      const int* row = c.table + static_cast<int64_t>(load.b) * c.table_stride;
+      page_lo = slot < load.n ? row[slot >> c.page_shift] : 0;
+      page_hi = split && slot + 16 < load.n ? row[(slot + 16) >> 4] : 0;
+    }
+    const int lo = __shfl_sync(0xffffffffu, page_lo, load.t - window), hi = __shfl_sync(0xffffffffu, page_hi, load.t - window);
+    const int slot = load.t * kTile, left = load.n - slot;
+    const bool lo_ok = static_cast<unsigned>(lo) < static_cast<unsigned>(c.pages);
+    const bool hi_there = left > 16, hi_ok = split ? static_cast<unsigned>(hi) < static_cast<unsigned>(c.pages) : lo_ok;
+    if (!(lo_ok && (hi_ok || !hi_there))) report_bad_index(c.status, kTagCachePage);
+    have = (have & ~(3u << (2 * stage))) | ((lo_ok ? 1u : 0u) | (hi_there && hi_ok ? 2u : 0u)) << (2 * stage);
+    if (lane == 0) {
+      constexpr uint32_t kHalf = 16 * R::kBytes;
+      const uint32_t bar = my_bar + 8 * stage, dst = smem_u32(my_ring + stage * Sh::kSlotBytes);
+      const int h = load.item / row_blocks;
+      const uint8_t* head = c.kv + h * c.kv_stride[1] + static_cast<int64_t>(slot & mask) * R::kBytes;
+      if (split) {
+        mbar_arrive_expect_tx(bar, (lo_ok ? kHalf : 0u) + (hi_there && hi_ok ? kHalf : 0u));
+        if (lo_ok) bulk_load(dst, head + lo * c.kv_stride[0], bar, kHalf);
+        if (hi_there && hi_ok) bulk_load(dst + kHalf, head + hi * c.kv_stride[0], bar, kHalf);
+      } else {
+        const uint32_t bytes = !lo_ok ? 0u : hi_there ? 2 * kHalf : kHalf;
+        mbar_arrive_expect_tx(bar, bytes);
+        if (lo_ok) bulk_load(dst, head + lo * c.kv_stride[0], bar, bytes);
+      }
+    }
+    advance(load, c, a.counts, per_sequence);
+  };
+#pragma unroll 1
+  for (int i = 0; i < Sh::kStages && load.left > 0; ++i) issue(i);
+
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  while (use.left > 0) {
+    // one piece: the tiles of one item that belong to this share
+    const int b = use.b, t0 = use.t, tiles = use.tiles, h = use.item / row_blocks, row0 = (use.item - h * row_blocks) * 8 * NT, n = use.n;
+    const int t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + use.left));
     Query<D, NT> f;
     load_query<D, NT, kBf16>(f, c, a, rows, b, h, row0, n);
     Sums<D, NT> x;
     clear(x);
-    const int mask = (1 << c.page_shift) - 1;
+#pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-      const uint8_t* rec[2] = {nullptr, nullptr};
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int slot = t * kTile + 16 * k;
-        int64_t page;
-        if (slot < n && find_page(c, b, slot, &page))
-          rec[k] = c.kv + page * c.kv_stride[0] + h * c.kv_stride[1] + static_cast<int64_t>(slot & mask) * R::kBytes;
-      }
+      ok = ok && mbar_wait_warp(my_bar + 8 * stage, phase, &abort_word, wait_limit_ns, kTagCache4Load);
+      if (!ok) break;
+      const uint8_t* slot = my_ring + stage * Sh::kSlotBytes;
+      const uint8_t* rec[2] = {(have >> (2 * stage)) & 1 ? slot : nullptr, (have >> (2 * stage)) & 2 ? slot + 16 * R::kBytes : nullptr};
       one_tile<D, NT, kBf16>(x, f, rec, t * kTile, n - t * kTile);
+      __syncwarp();
+      if (load.left > 0) issue(stage);
+      if (++stage == Sh::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      advance(use, c, a.counts, per_sequence);
     }
+    if (!ok) break;
     float* piece = nullptr;
     if (t0 > 0 || t1 < tiles) piece = a.pieces + (worker * 2 + (t0 == 0)) * piece_floats<D, NT>();
     store_sums<D, NT, kBf16>(x, a, rows, b, h, row0, piece);
-    at += t1 - t0;
+  }
+  if (!ok) {
+    // a copy did not arrive in time: said in the status word; no copy is left behind without a second wait
+    if (lane == 0) atomicCAS(c.status, 0, abort_word);
+    for (int i = 0; i < Sh::kStages; ++i) {
+      int again = 0;
+      mbar_wait(my_bar + 8 * i, i < stage ? phase ^ 1 : phase, &again, wait_limit_ns, kTagCache4Load);
+    }
   }
 }
 
@@ -631,9 +740,13 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   rows.group = a.Hq / c.H;
   rows.count = rows.group * a.S;
   const int row_blocks = (rows.count + 8 * NT - 1) / (8 * NT);
-  const int grid = sm_count * kCtasPerSm;
+  using Sh = Shape<D, NT>;
+  const int grid = sm_count * Sh::kCtas;
   const bool pdl = option_pdl() != 0;
-  cudaError_t e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, kThreads, 0, stream, pdl, c, a, rows, row_blocks);
+  static std::atomic<unsigned long long> smem_done{0};   // per kernel instantiation, bit per device
+  cudaError_t e = set_dynamic_smem_once(smem_done, reinterpret_cast<const void*>(cache4_attention_kernel<D, NT, kBf16>), Sh::kRingBytes);
+  if (e != cudaSuccess) return e;
+  e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, kThreads, Sh::kRingBytes, stream, pdl, c, a, rows, row_blocks, option_wait_limit_ns());
   if (e != cudaSuccess) return e;
   *launches += 1;
   e = launch_persistent(cache4_join_kernel<D, NT, kBf16>, c.B * c.H * rows.count, kJoinThreads, 0, stream, pdl, c, a, rows, row_blocks,
@@ -662,9 +775,15 @@ cudaError_t launch_dim(const Cache4& c, const Cache4Attention& a, int sm_count, 
 
 }  // namespace
 
+template <int D, int NT>
+size_t pieces_bytes(int sm_count) {
+  return static_cast<size_t>(sm_count) * Shape<D, NT>::kCtas * kWarps * 2 * piece_floats<D, NT>() * sizeof(float);
+}
 size_t cache4_attention_workspace(int D, int Hq, int H, int S, int sm_count) {
-  const size_t rows = sixteen_rows(D, Hq / H * S) ? 16 : 8;
-  return static_cast<size_t>(sm_count) * kCtasPerSm * kWarps * 2 * rows * (D + 2) * sizeof(float);
+  const bool wide = sixteen_rows(D, Hq / H * S);
+  if (D == 64) return wide ? pieces_bytes<64, 2>(sm_count) : pieces_bytes<64, 1>(sm_count);
+  if (D == 128) return wide ? pieces_bytes<128, 2>(sm_count) : pieces_bytes<128, 1>(sm_count);
+  return pieces_bytes<256, 1>(sm_count);
 }
 
 cudaError_t launch_cache4_attention(const Cache4& c, const Cache4Attention& a, int sm_count, cudaStream_t stream, long long* launches) {
