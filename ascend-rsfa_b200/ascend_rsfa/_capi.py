@@ -54,7 +54,7 @@ SIGNATURES = {
                                       _c.c_void_p, _c.c_void_p, _c.POINTER(_c.c_int64), _c.c_void_p]),
     "rsfa_cache4_read": (_c.c_int, [_c.POINTER(Cache4), _c.c_void_p, _c.c_void_p, _c.c_int, _c.POINTER(_c.c_int64),
                                     _c.c_void_p, _c.c_void_p]),
-    "rsfa_cache4_attention_workspace": (_c.c_longlong, [_c.c_int] * 4),
+    "rsfa_cache4_attention_workspace": (_c.c_longlong, [_c.POINTER(Cache4), _c.c_int, _c.c_int]),
     "rsfa_cache4_attention": (_c.c_int, [_c.POINTER(Cache4), _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int,
                                          _c.POINTER(_c.c_int64), _c.c_void_p, _c.c_float, _c.c_void_p, _c.c_longlong,
                                          _c.c_void_p]),

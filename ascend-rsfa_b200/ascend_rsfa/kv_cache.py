@@ -12,7 +12,7 @@ the host, so a decoding step can be captured in a CUDA graph.  Rows are quantise
 scale and minimum each, 1.25 bytes per pair of a K and a V element; K goes in as attention is to see it, with its rotary
 positions applied (rotary.py).  Head dims 64, 128 and 256, fp16 and bf16; the dtype of q, k and v is the cache's.
 
-Lengths or page numbers out of range are skipped by the kernels, and device_status() tells.  The reference has no cache
+Lengths and page numbers out of range make the kernels touch nothing outside; device_status() tells.  The reference has no cache
 and no decoding; the kernels are in csrc/cache4_*.cu, without a CPU path.
 """
 import ctypes
@@ -159,11 +159,11 @@ def cache4_attention(q, kv, table, lengths, sm_scale, counts=None, weight=None, 
     qd = _readable(q)
     o = _rows(qd)
     lse = torch.empty((B, Hq, S), dtype=torch.float32, device=q.device) if want_lse or weight is not None else None
-    key = (D, Hq // c.heads * S, kv.device.index)
+    key = (D, Hq // c.heads * S, kv.device.index, 0 if weight is None else B * c.heads * c.page_size * c.max_pages)
     nbytes = _workspace_bytes.get(key)
     if nbytes is None:
         with torch.cuda.device(kv.device):
-            nbytes = _lib.rsfa_cache4_attention_workspace(D, Hq, c.heads, S)
+            nbytes = _lib.rsfa_cache4_attention_workspace(ctypes.byref(c), Hq, S)
         if nbytes < 0:
             _capi.check(nbytes, "rsfa_cache4_attention_workspace")
         if len(_workspace_bytes) > 256:

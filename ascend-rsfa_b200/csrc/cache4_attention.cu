@@ -25,10 +25,10 @@ namespace {
 constexpr int kTile = 32;            // tokens per tile
 constexpr int kWarps = 4;            // per CTA
 constexpr int kThreads = 32 * kWarps;
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 128, kJoinMost = 512;
 #ifndef C4_CTAS128
-#define C4_CTAS128 4
-#define C4_STAGES128 2
+#define C4_CTAS128 3
+#define C4_STAGES128 3
 #endif
 // CTAs per multiprocessor by the registers of their accumulators, and slots of a warp's ring by its shared memory.
 template <int D, int NT>
@@ -66,22 +66,26 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 // ------------------------------------------------------------------ the list of tiles
 // Items are (sequence, K/V head, block of query rows) in this order, an item's tiles follow one another.
-struct Items {
-  int per_sequence;    // K/V heads * blocks of rows
-  long long total;     // tiles
-};
 __device__ __forceinline__ int visible_tokens(const Cache4& c, const int* counts, int b) {
   return counts != nullptr && counts[b] <= 0 ? 0 : tokens_of(c, b);
 }
 __device__ __forceinline__ int tiles_of(const Cache4& c, const int* counts, int b) {
   return (visible_tokens(c, counts, b) + kTile - 1) / kTile;
 }
-// One warp: tiles of the sequences below `end`, per item.
-__device__ __forceinline__ long long tiles_before(const Cache4& c, const int* counts, int end) {
-  long long n = 0;
-  for (int b = threadIdx.x & 31; b < end; b += 32) n += tiles_of(c, counts, b);
+// One warp: tiles of all sequences and of those before b, per K/V head and block of rows.
+__device__ __forceinline__ long long all_tiles(const Cache4& c, const int* counts, int b, long long* before) {
+  long long n = 0, m = 0;
+  for (int i = threadIdx.x & 31; i < c.B; i += 32) {
+    const int tiles = tiles_of(c, counts, i);
+    n += tiles;
+    m += i < b ? tiles : 0;
+  }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+  for (int d = 16; d; d >>= 1) {
+    n += __shfl_xor_sync(0xffffffffu, n, d);
+    m += __shfl_xor_sync(0xffffffffu, m, d);
+  }
+  *before = m;
   return n;
 }
 // One warp: the sequence that tile `at` belongs to and the first tile of that sequence.
@@ -118,6 +122,33 @@ __device__ __forceinline__ long long worker_of(long long total, long long tile, 
   return ((tile + 1) * workers - 1) / total;
 }
 
+// A place in the list: item `item` of sequence b, tile t of `tiles`, and the tiles of the share from here on.
+struct Cursor {
+  int b, n, tiles, item, t, left;
+  long long at;
+};
+__device__ __forceinline__ Cursor cursor_at(const Cache4& c, const int* counts, int per_sequence, long long at, long long end) {
+  Cursor k;
+  long long first;
+  k.b = sequence_of(c, counts, per_sequence, at, &first, &k.tiles);
+  k.n = tokens_of(c, k.b);
+  k.item = static_cast<int>((at - first) / k.tiles);
+  k.t = static_cast<int>(at - first - static_cast<long long>(k.item) * k.tiles);
+  k.left = static_cast<int>(end - at);
+  k.at = at;
+  return k;
+}
+// To the next item, for which tiles are left.
+__device__ __forceinline__ void next_item(Cursor& k, const Cache4& c, const int* counts, int per_sequence) {
+  k.t = 0;
+  if (++k.item < per_sequence) return;
+  k.item = 0;
+  do {                     // a sequence that has tokens: there is one
+    k.tiles = tiles_of(c, counts, ++k.b);
+  } while (k.tiles == 0);
+  k.n = tokens_of(c, k.b);
+}
+
 // ------------------------------------------------------------------ query rows
 // Row r of an item is query token r / group of head (r % group) of the K/V head's query heads.
 struct Rows {
@@ -125,14 +156,15 @@ struct Rows {
 };
 
 // The B fragments of 8 NT query rows, each row divided by a power of two so that its largest element is about 2^10
-// (fp16 then holds bf16's numbers as well), the sums of its groups and its factor.
+// (fp16 then holds bf16's numbers as well), the sums of its groups and the factor that its sums are scores by.
 template <int D, int NT>
 struct Query {
   static constexpr int G = D / 32;
   uint32_t frag[NT][G][4];
   float sums[NT][G][2];     // of rows 2 c, 2 c + 1 (c = lane % 4), times 2^-24
-  float factor[NT][2];
+  float factor[NT][2];      // > 0, log2 units
   int last[NT][2];          // last visible slot
+  int last_all;             // slots up to here are visible to every row
 };
 
 template <int D, int NT, bool kBf16>
@@ -170,7 +202,7 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     int e = static_cast<int>(__float_as_uint(top) >> 23) - 127 - 10;
     e = max(min(e, 100), -100);
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);   // 2^-e
+    const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), a.sm_scale);   // 2^-e, and the scale's sign
     const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
     for (int w = 0; w < G; ++w) {
@@ -191,19 +223,24 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
       f.sums[nt][w][0] = __shfl_sync(0xffffffffu, sum, 8 * q4);
       f.sums[nt][w][1] = __shfl_sync(0xffffffffu, sum, 8 * q4 + 4);
     }
-    const float factor = up * 16777216.f * (a.sm_scale * kLog2e);
+    const float factor = fmaxf(up * 16777216.f * (fabsf(a.sm_scale) * kLog2e), 1e-37f);   // -inf times it stays -inf
     f.factor[nt][0] = __shfl_sync(0xffffffffu, factor, 8 * q4);
     f.factor[nt][1] = __shfl_sync(0xffffffffu, factor, 8 * q4 + 4);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int r = row0 + 8 * nt + 2 * q4 + j, i = r / rows.group;
-      f.last[nt][j] = r < rows.count && i < count ? n - count + i : -1;
+      f.last[nt][j] = r >= rows.count ? INT_MAX : i < count ? n - count + i : -1;   // rows that do not exist: whatever is cheap
     }
   }
+  int all = INT_MAX;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) all = min(all, min(f.last[nt][0], f.last[nt][1]));
+  f.last_all = __reduce_min_sync(0xffffffffu, all);
 }
 
 // ------------------------------------------------------------------ one block of 16 tokens
-// Scores of tokens (g, g + 8) (g = lane / 4) and query rows (2 c, 2 c + 1) from the records at `rec`, in log2 units.
+// Scores of tokens (g, g + 8) (g = lane / 4) and query rows (2 c, 2 c + 1) from the records at `rec`, but for the
+// rows' factors.
 template <int D, int NT, bool kBf16>
 __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* rec, const Query<D, NT>& f) {
   using R = Record<D>;
@@ -247,26 +284,30 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
       s[nt][3] = fmaf(sh.x, acc[3], fmaf(sh.y, f.sums[nt][w][1], s[nt][3]));
     }
   }
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[nt][j] *= f.factor[nt][j & 1];
 }
 
-// The sums of one piece of an item.
+// The sums of one piece of an item.  A code u enters the second product as it is, but the rounding of p * s would then
+// show times u: sum p s u + sum p m is taken as sum P u - 8 sum P + sum p (m + 8 s), P = fp16(p s), which leaves it
+// times u - 8, half as much on average.  The sum of P comes out of an MMA of its own (`eights`), whose row w is group w.
 template <int D, int NT>
 struct Sums {
   static constexpr int G = D / 32;
   float o[2 * G][NT][4];       // tile 2 w + t: dims 32 w + 4 g + 2 t (times 2^-24) and + 1 (times 2^-20), both over `unit`
-  float minima[G][NT][2];      // this lane's share of sum p m, rows 2 c, 2 c + 1
+  float eights[NT][4];         // 8 sum P of group g = lane / 4, rows 2 c, 2 c + 1, times 2^-24 over `unit`
+  float mids[G][NT][2];        // this lane's share of sum p (m + 8 s), rows 2 c, 2 c + 1
   float l[NT][2], ref[NT][2];
   float unit;                  // power of two that p * s is divided by
+  uint32_t unit_limit;         // 16-bit pattern of the scale from which on it is raised
 };
+constexpr float kLeastUnit = 7.888609052210118e-31f;   // 2^-100
+constexpr float kNoScore = -3.4028234663852886e38f;    // reference of a row that has seen nothing
 
 template <int D, int NT>
 __device__ __forceinline__ void clear(Sums<D, NT>& x) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.eights[nt][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < 2 * (D / 32); ++j)
 #pragma unroll
@@ -274,23 +315,23 @@ __device__ __forceinline__ void clear(Sums<D, NT>& x) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) x.minima[w][nt][i] = 0.f;
+      for (int w = 0; w < D / 32; ++w) x.mids[w][nt][i] = 0.f;
       x.l[nt][i] = 0.f;
-      x.ref[nt][i] = -INFINITY;
+      x.ref[nt][i] = kNoScore;
     }
   }
-  x.unit = 1.17549435e-38f;
+  x.unit = kLeastUnit;
+  x.unit_limit = 0;
 }
 
-// The second product of 16 tokens: p of tokens (g, g + 8), zero where hidden; `left`: tokens of the block that exist.
-template <int D, int NT, bool kBf16>
-__device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT][4], const uint8_t* rec, const float2 (&lo_pair)[D / 32],
-                                             const float2 (&hi_pair)[D / 32], float per_unit) {
+// The second product of 16 tokens: p of tokens (g, g + 8).  kCareful: some scale is NaN, and hidden tokens must not show.
+template <int D, int NT, bool kBf16, bool kCareful>
+__device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT][4], const uint8_t* rec, float per_unit) {
   using R = Record<D>;
   constexpr int G = D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   constexpr int kWords = G / 2;                  // 32-bit words of one token's V codes in a lane
-  uint32_t v[4][kWords];
+  uint32_t v[4][kWords], pl[G], ph[G];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint8_t* at = rec + (2 * q4 + (j & 1) + 8 * (j >> 1)) * R::kBytes + R::kVCodes + g * (D / 16);
@@ -304,118 +345,147 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
       v[j][0] = u.x, v[j][1] = u.y, v[j][2] = u.z, v[j][3] = u.w;
     }
   }
+  const uint8_t* lo = rec + g * R::kBytes + R::kVPairs;
+  const uint8_t* hi = lo + 8 * R::kBytes;
+#pragma unroll
+  for (int w = 0; w < G; w += 2) {
+    const uint2 y = *reinterpret_cast<const uint2*>(lo + 4 * w), z = *reinterpret_cast<const uint2*>(hi + 4 * w);
+    pl[w] = y.x, pl[w + 1] = y.y, ph[w] = z.x, ph[w + 1] = z.y;
+  }
+  float pu[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pu[nt][j] = p[nt][j] * per_unit;
 #pragma unroll
   for (int w = 0; w < G; ++w) {
     // the half words of group w: low half token 2 c (2 c + 8), high half the token behind it
     const uint32_t pick = (w & 1) ? 0x7632u : 0x5410u;
     const uint32_t y = __byte_perm(v[0][w / 2], v[1][w / 2], pick), z = __byte_perm(v[2][w / 2], v[3][w / 2], pick);
     const uint32_t y8 = y >> 8, z8 = z >> 8;
-    const float sl = lo_pair[w].x * per_unit, sh = hi_pair[w].x * per_unit;
+    const float2 sl = to_f32x2<kBf16>(pl[w]), sh = to_f32x2<kBf16>(ph[w]);
+    const float ml = fmaf(8.f, sl.x, sl.y), mh = fmaf(8.f, sh.x, sh.y);
+    const uint32_t eight = g == w ? 0x00080008u : 0u;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t b0 = transpose_8x8(from_f32x2<false>(p[nt][0] * sl, p[nt][1] * sl));
-      const uint32_t b1 = transpose_8x8(from_f32x2<false>(p[nt][2] * sh, p[nt][3] * sh));
+      auto part = [&](int j, float by) { return kCareful && p[nt][j] == 0.f ? 0.f : pu[nt][j] * by; };
+      auto mid = [&](int j, float by, float sum) { return kCareful && p[nt][j] == 0.f ? sum : fmaf(p[nt][j], by, sum); };
+      const uint32_t b0 = transpose_8x8(from_f32x2<false>(part(0, sl.x), part(1, sl.x)));
+      const uint32_t b1 = transpose_8x8(from_f32x2<false>(part(2, sh.x), part(3, sh.x)));
       mma_f16(x.o[2 * w][nt], y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, b0, b1);
       mma_f16(x.o[2 * w + 1][nt], y8 & 0x000f000fu, y8 & 0x00f000f0u, z8 & 0x000f000fu, z8 & 0x00f000f0u, b0, b1);
-      x.minima[w][nt][0] = fmaf(p[nt][0], lo_pair[w].y, fmaf(p[nt][2], hi_pair[w].y, x.minima[w][nt][0]));
-      x.minima[w][nt][1] = fmaf(p[nt][1], lo_pair[w].y, fmaf(p[nt][3], hi_pair[w].y, x.minima[w][nt][1]));
+      mma_f16(x.eights[nt], eight, 0u, eight, 0u, b0, b1);
+      x.mids[w][nt][0] = mid(0, ml, mid(2, mh, x.mids[w][nt][0]));
+      x.mids[w][nt][1] = mid(1, ml, mid(3, mh, x.mids[w][nt][1]));
     }
   }
 }
 
-// Scales and minima of V of tokens (g, g + 8); zero for tokens that do not exist (what the page holds there may be NaN).
-template <int D, bool kBf16>
-__device__ __forceinline__ void value_pairs(float2 (&lo)[D / 32], float2 (&hi)[D / 32], const uint8_t* rec, int left) {
-  using R = Record<D>;
-  const int g = (threadIdx.x & 31) >> 2;
+// Raises the references of the rows.
+template <int D, int NT>
+__device__ __forceinline__ void raise_references(Sums<D, NT>& x, const float (&top)[NT][2]) {
 #pragma unroll
-  for (int w = 0; w < D / 32; ++w) {
-    const uint32_t a = g < left ? *reinterpret_cast<const uint32_t*>(rec + g * R::kBytes + R::kVPairs + 4 * w) : 0u;
-    const uint32_t b = g + 8 < left ? *reinterpret_cast<const uint32_t*>(rec + (g + 8) * R::kBytes + R::kVPairs + 4 * w) : 0u;
-    lo[w] = to_f32x2<kBf16>(a);
-    hi[w] = to_f32x2<kBf16>(b);
-  }
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float m = top[nt][i];
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const float ref = fmaxf(m, x.ref[nt][i]);
+      const float by = ex2(x.ref[nt][i] - ref);
+      x.ref[nt][i] = ref;
+      x.l[nt][i] *= by;
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) x.mids[w][nt][i] *= by;
+#pragma unroll
+      for (int j = 0; j < 2 * (D / 32); ++j) {
+        x.o[j][nt][i] *= by;
+        x.o[j][nt][i + 2] *= by;
+      }
+      x.eights[nt][i] *= by;
+      x.eights[nt][i + 2] *= by;
+    }
 }
 
-// One tile of 32 tokens: `rec` the records of its two blocks (null: the page is not there), `left` its tokens.
+// One tile of 32 tokens at `rec`, whose first slot is `slot`.  scores: where the tile's scores are kept, null: nowhere.
 template <int D, int NT, bool kBf16>
-__device__ __forceinline__ void one_tile(Sums<D, NT>& x, const Query<D, NT>& f, const uint8_t* const (&rec)[2], int slot, int left) {
+__device__ __forceinline__ void one_tile(Sums<D, NT>& x, const Query<D, NT>& f, const uint8_t* rec, int slot, float* scores, int score_rows) {
+  using R = Record<D>;
   constexpr int G = D / 32;
-  const int g = (threadIdx.x & 31) >> 2;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   float s[2][NT][4];
-  float top[NT][2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+  for (int k = 0; k < 2; ++k) block_scores<D, NT, kBf16>(s[k], rec + 16 * k * R::kBytes, f);
+  if (slot + kTile - 1 > f.last_all) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (16 * k < left && rec[k] != nullptr) {
-      block_scores<D, NT, kBf16>(s[k], rec[k], f);
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j)
           if (slot + 16 * k + g + 8 * (j >> 1) > f.last[nt][j & 1]) s[k][nt][j] = -INFINITY;
-          top[nt][j & 1] = fmaxf(top[nt][j & 1], s[k][nt][j]);
-        }
-    }
   }
   bool raise = false;
+  float top[NT][2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) raise |= top[nt][0] > x.ref[nt][0] + kRaise || top[nt][1] > x.ref[nt][1] + kRaise;
-  if (__any_sync(0xffffffffu, raise)) {
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[nt][i] = fmaxf(fmaxf(s[0][nt][i], s[0][nt][i + 2]), fmaxf(s[1][nt][i], s[1][nt][i + 2])) * f.factor[nt][i];
+      raise |= top[nt][i] > x.ref[nt][i] + kRaise;
+    }
+  if (__any_sync(0xffffffffu, raise)) raise_references<D, NT>(x, top);
+  // a scale much above all before: each lane looks at its share of the tile's
+  uint32_t widest = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int w = 0; w < (G + 3) / 4; ++w)
+      widest = max(widest, *reinterpret_cast<const uint16_t*>(rec + (g + 8 * i) * R::kBytes + R::kVPairs + 4 * ((q4 + 4 * w) % G)) + 0u);
+  bool odd = false;
+  if (__any_sync(0xffffffffu, widest > x.unit_limit)) {
+    odd = __any_sync(0xffffffffu, widest > (kBf16 ? 0x7f80u : 0x7c00u));
+    float top_scale = to_f32<kBf16>(static_cast<uint16_t>(widest));
+    top_scale = top_scale < INFINITY ? top_scale : 0.f;             // NaN is left to the products
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) top_scale = fmaxf(top_scale, __shfl_xor_sync(0xffffffffu, top_scale, d));
+    const float unit = fmaxf(__uint_as_float(__float_as_uint(top_scale) & 0x7f800000u), x.unit);   // the power of two below it
+    const float by = x.unit / unit;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float m = top[nt][i];
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const float ref = fmaxf(m, x.ref[nt][i]);
-        const float by = ref == -INFINITY ? 1.f : ex2(x.ref[nt][i] - ref);
-        x.ref[nt][i] = ref;
-        x.l[nt][i] *= by;
-#pragma unroll
-        for (int w = 0; w < G; ++w) x.minima[w][nt][i] *= by;
-#pragma unroll
-        for (int j = 0; j < 2 * G; ++j) {
-          x.o[j][nt][i] *= by;
-          x.o[j][nt][i + 2] *= by;
-        }
+        for (int j = 0; j < 2 * G; ++j) x.o[j][nt][i] *= by;
+        x.eights[nt][i] *= by;
       }
+    x.unit = unit;
+    x.unit_limit = from_f32<kBf16>(unit * kRaiseScale);
   }
+  const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(x.unit));   // 1 / a power of two
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    if (16 * k < left && rec[k] != nullptr) {
-      float2 lo[G], hi[G];
-      value_pairs<D, kBf16>(lo, hi, rec[k], left - 16 * k);
-      float widest = 0.f;
+    float p[NT][4];
 #pragma unroll
-      for (int w = 0; w < G; ++w) widest = fmaxf(widest, fmaxf(lo[w].x, hi[w].x));
-      if (__any_sync(0xffffffffu, widest > x.unit * kRaiseScale)) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) widest = fmaxf(widest, __shfl_xor_sync(0xffffffffu, widest, d));
-        // the power of two below it, and no less than can be divided by
-        const float unit = fmaxf(__uint_as_float(__float_as_uint(widest) & 0x7f800000u), 1.17549435e-38f);
-        const float by = x.unit / unit;
-#pragma unroll
-        for (int j = 0; j < 2 * G; ++j)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.o[j][nt][i] *= by;
-        x.unit = unit;
+      for (int j = 0; j < 4; ++j) {
+        p[nt][j] = ex2(fmaf(s[k][nt][j], f.factor[nt][j & 1], -x.ref[nt][j & 1]));
+        x.l[nt][j & 1] += p[nt][j];
       }
-      float p[NT][4];
+    if (scores != nullptr) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          // a row that sees nothing yet has no reference to subtract
-          p[nt][j] = s[k][nt][j] == -INFINITY ? 0.f : ex2(s[k][nt][j] - x.ref[nt][j & 1]);
-          x.l[nt][j & 1] += p[nt][j];
+          const int r = 8 * nt + 2 * q4 + (j & 1);
+          if (r < score_rows) scores[r * kTile + 16 * k + g + 8 * (j >> 1)] = s[k][nt][j] * f.factor[nt][j & 1];
         }
-      block_output<D, NT, kBf16>(x, p, rec[k], lo, hi, 1.f / x.unit);
     }
+    if (!odd)
+      block_output<D, NT, kBf16, false>(x, p, rec + 16 * k * R::kBytes, per_unit);
+    else
+      block_output<D, NT, kBf16, true>(x, p, rec + 16 * k * R::kBytes, per_unit);
   }
 }
 
@@ -436,67 +506,43 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      // sum p m: what is left of sum p (m + 8 s) without the eights of the group, which lane 4 w + q4 has
+      float l = x.l[nt][i], m[G];
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        x.l[nt][i] += __shfl_xor_sync(0xffffffffu, x.l[nt][i], d);
+      for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
 #pragma unroll
-        for (int w = 0; w < G; ++w) x.minima[w][nt][i] += __shfl_xor_sync(0xffffffffu, x.minima[w][nt][i], d);
+      for (int w = 0; w < G; ++w) {
+        m[w] = x.mids[w][nt][i];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) m[w] += __shfl_xor_sync(0xffffffffu, m[w], d);
+        m[w] -= low(__shfl_sync(0xffffffffu, x.eights[nt][i], 4 * w + q4));
       }
       const int r = 8 * nt + 2 * q4 + i, row = row0 + r;
-      if (row >= rows.count) continue;
-      const float l = x.l[nt][i];
-      if (piece != nullptr) {
-        float* dst = piece + r * (D + 2);
+      if (row < rows.count) {
+        if (piece != nullptr) {
+          float* dst = piece + r * (D + 2);
 #pragma unroll
-        for (int w = 0; w < G; ++w) {
-          const float m = x.minima[w][nt][i];
-          *reinterpret_cast<float2*>(dst + 32 * w + 4 * g) = make_float2(low(x.o[2 * w][nt][i]) + m, high(x.o[2 * w][nt][i + 2]) + m);
-          *reinterpret_cast<float2*>(dst + 32 * w + 4 * g + 2) = make_float2(low(x.o[2 * w + 1][nt][i]) + m, high(x.o[2 * w + 1][nt][i + 2]) + m);
-        }
-        if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(x.ref[nt][i], l);
-      } else {
-        const int t = row / rows.group, hq = h * rows.group + row - t * rows.group;
-        const float inv = l == 0.f ? 0.f : 1.f / l;      // a row that sees nothing is zero
-        uint16_t* dst = static_cast<uint16_t*>(a.o) + b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2];
+          for (int w = 0; w < G; ++w) {
+            *reinterpret_cast<float2*>(dst + 32 * w + 4 * g) = make_float2(low(x.o[2 * w][nt][i]) + m[w], high(x.o[2 * w][nt][i + 2]) + m[w]);
+            *reinterpret_cast<float2*>(dst + 32 * w + 4 * g + 2) =
+                make_float2(low(x.o[2 * w + 1][nt][i]) + m[w], high(x.o[2 * w + 1][nt][i + 2]) + m[w]);
+          }
+          if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(x.ref[nt][i], l);
+        } else {
+          const int t = row / rows.group, hq = h * rows.group + row - t * rows.group;
+          const float inv = l == 0.f ? 0.f : 1.f / l;      // a row that sees nothing is zero
+          uint16_t* dst = static_cast<uint16_t*>(a.o) + b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2];
 #pragma unroll
-        for (int w = 0; w < G; ++w) {
-          const float m = x.minima[w][nt][i];
-          const uint2 v = make_uint2(from_f32x2<kBf16>((low(x.o[2 * w][nt][i]) + m) * inv, (high(x.o[2 * w][nt][i + 2]) + m) * inv),
-                                     from_f32x2<kBf16>((low(x.o[2 * w + 1][nt][i]) + m) * inv, (high(x.o[2 * w + 1][nt][i + 2]) + m) * inv));
-          *reinterpret_cast<uint2*>(dst + 32 * w + 4 * g) = v;
+          for (int w = 0; w < G; ++w)
+            *reinterpret_cast<uint2*>(dst + 32 * w + 4 * g) =
+                make_uint2(from_f32x2<kBf16>((low(x.o[2 * w][nt][i]) + m[w]) * inv, (high(x.o[2 * w][nt][i + 2]) + m[w]) * inv),
+                           from_f32x2<kBf16>((low(x.o[2 * w + 1][nt][i]) + m[w]) * inv, (high(x.o[2 * w + 1][nt][i + 2]) + m[w]) * inv));
+          if (g == 0 && a.lse != nullptr)
+            a.lse[(static_cast<int64_t>(b) * a.Hq + hq) * a.S + t] = l == 0.f ? -INFINITY : (x.ref[nt][i] + __log2f(l)) * kLn2;
         }
-        if (g == 0 && a.lse != nullptr)
-          a.lse[(static_cast<int64_t>(b) * a.Hq + hq) * a.S + t] = l == 0.f ? -INFINITY : (x.ref[nt][i] + __log2f(l)) * kLn2;
       }
     }
   }
-}
-
-// A place in the list of tiles: item `item` of sequence b, tile t of `tiles`.
-struct Cursor {
-  int b, n, tiles, item, t;
-  long long left;          // tiles of the share from here on
-};
-__device__ __forceinline__ Cursor cursor_at(const Cache4& c, const int* counts, int per_sequence, long long at, long long end) {
-  Cursor k;
-  long long first;
-  k.b = sequence_of(c, counts, per_sequence, at, &first, &k.tiles);
-  k.n = tokens_of(c, k.b);
-  k.item = static_cast<int>((at - first) / k.tiles);
-  k.t = static_cast<int>(at - first - static_cast<long long>(k.item) * k.tiles);
-  k.left = end - at;
-  return k;
-}
-__device__ __forceinline__ void advance(Cursor& k, const Cache4& c, const int* counts, int per_sequence) {
-  --k.left;
-  if (++k.t < k.tiles || k.left == 0) return;
-  k.t = 0;
-  if (++k.item < per_sequence) return;
-  k.item = 0;
-  do {                     // the next sequence that has tokens: there is one, tiles are left
-    k.tiles = tiles_of(c, counts, ++k.b);
-  } while (k.tiles == 0);
-  k.n = tokens_of(c, k.b);
 }
 
 // Every warp works for itself: a ring of tiles in shared memory, which its first lane fills with bulk copies as soon
@@ -518,19 +564,20 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   griddep_launch_dependents();
   griddep_wait();
   const int per_sequence = c.H * row_blocks;
-  const long long total = tiles_before(c, a.counts, c.B) * per_sequence;
+  long long none;
+  const long long total = all_tiles(c, a.counts, 0, &none) * per_sequence;
   const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
   if (worker >= workers) return;
   Cursor use = cursor_at(c, a.counts, per_sequence, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
   Cursor load = use;
-  const uint8_t* const my_ring = ring + warp * Sh::kStages * Sh::kSlotBytes;
+  uint8_t* const my_ring = ring + warp * Sh::kStages * Sh::kSlotBytes;
   const uint32_t my_bar = smem_u32(&full_bar[warp * Sh::kStages]);
   const int mask = (1 << c.page_shift) - 1;
   const bool split = c.page_shift == 4;    // a tile is two pages
 
   // Pages of tiles window .. window + 31 of sequence window_b, one per lane (two where a tile is two pages).
   int window_b = -1, window = 0, page_lo = 0, page_hi = 0;
-  uint32_t have = 0;                       // two bits per slot: which halves of its tile are there
+  uint32_t have = 0;                       // two bits per slot: which halves of its tile have a page
   auto issue = [&](int stage) {
     if (load.b != window_b || load.t < window || load.t >= window + 32) {
       window_b = load.b;
@@ -544,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
     const int slot = load.t * kTile, left = load.n - slot;
     const bool lo_ok = static_cast<unsigned>(lo) < static_cast<unsigned>(c.pages);
     const bool hi_there = left > 16, hi_ok = split ? static_cast<unsigned>(hi) < static_cast<unsigned>(c.pages) : lo_ok;
-    if (!(lo_ok && (hi_ok || !hi_there))) report_bad_index(c.status, kTagCachePage);
+    if (!lo_ok || (hi_there && !hi_ok)) report_bad_index(c.status, kTagCachePage);
     have = (have & ~(3u << (2 * stage))) | ((lo_ok ? 1u : 0u) | (hi_there && hi_ok ? 2u : 0u)) << (2 * stage);
     if (lane == 0) {
       constexpr uint32_t kHalf = 16 * R::kBytes;
@@ -561,41 +608,58 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
         if (lo_ok) bulk_load(dst, head + lo * c.kv_stride[0], bar, bytes);
       }
     }
-    advance(load, c, a.counts, per_sequence);
+    --load.left;
+    if (++load.t == load.tiles && load.left > 0) next_item(load, c, a.counts, per_sequence);
   };
 #pragma unroll 1
   for (int i = 0; i < Sh::kStages && load.left > 0; ++i) issue(i);
 
+  const int score_rows = min(8 * NT, rows.count);     // of a tile; as many as an item has
+  float* const kept = c.weight != nullptr && row_blocks == 1 ? a.scores : nullptr;
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
   while (use.left > 0) {
     // one piece: the tiles of one item that belong to this share
     const int b = use.b, t0 = use.t, tiles = use.tiles, h = use.item / row_blocks, row0 = (use.item - h * row_blocks) * 8 * NT, n = use.n;
-    const int t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + use.left));
+    const int t1 = min(tiles, t0 + use.left);
     Query<D, NT> f;
     load_query<D, NT, kBf16>(f, c, a, rows, b, h, row0, n);
     Sums<D, NT> x;
     clear(x);
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-      ok = ok && mbar_wait_warp(my_bar + 8 * stage, phase, &abort_word, wait_limit_ns, kTagCache4Load);
+      ok = mbar_wait_warp(my_bar + 8 * stage, phase, &abort_word, wait_limit_ns, kTagCache4Load);
       if (!ok) break;
-      const uint8_t* slot = my_ring + stage * Sh::kSlotBytes;
-      const uint8_t* rec[2] = {(have >> (2 * stage)) & 1 ? slot : nullptr, (have >> (2 * stage)) & 2 ? slot + 16 * R::kBytes : nullptr};
-      one_tile<D, NT, kBf16>(x, f, rec, t * kTile, n - t * kTile);
+      uint8_t* const slot = my_ring + stage * Sh::kSlotBytes;
+      // what is not there, tokens behind the last one and pages that do not exist, is made zeros
+      const int left = min(n - t * kTile, kTile);
+      const uint32_t there = (have >> (2 * stage)) & 3u;
+      const bool patch = left < kTile || there != 3u;
+      if (patch) {
+        for (int i = lane; i < kTile * (R::kBytes / 16); i += 32) {
+          const int token = i / (R::kBytes / 16);
+          if (token >= left || !((there >> (token >> 4)) & 1)) *reinterpret_cast<uint4*>(slot + 16 * i) = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+      }
+      float* scores = kept != nullptr ? kept + (use.at + t - t0) * score_rows * kTile : nullptr;
+      one_tile<D, NT, kBf16>(x, f, slot, t * kTile, scores, score_rows);
+      if (patch) fence_proxy_async();      // before a copy writes where this warp has written
       __syncwarp();
       if (load.left > 0) issue(stage);
       if (++stage == Sh::kStages) {
         stage = 0;
         phase ^= 1;
       }
-      advance(use, c, a.counts, per_sequence);
     }
     if (!ok) break;
     float* piece = nullptr;
     if (t0 > 0 || t1 < tiles) piece = a.pieces + (worker * 2 + (t0 == 0)) * piece_floats<D, NT>();
     store_sums<D, NT, kBf16>(x, a, rows, b, h, row0, piece);
+    use.left -= t1 - t0;
+    use.at += t1 - t0;
+    if (use.left > 0) next_item(use, c, a.counts, per_sequence);
   }
   if (!ok) {
     // a copy did not arrive in time: said in the status word; no copy is left behind without a second wait
@@ -607,130 +671,182 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   }
 }
 
-// One CTA per query row of an item: joins the item's pieces where there are several, and answers for items without
-// tokens.  The order of the pieces is that of the tokens, so results do not depend on timing.
+// A CTA has an item's rows from blockIdx.y * rows_each on: it joins the item's pieces where there are several, and
+// answers for items without tokens.  The pieces are taken in an order that does not depend on timing.
 template <int D, int NT, bool kBf16>
-__global__ void __launch_bounds__(kJoinThreads) cache4_join_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks,
-                                                                   const long long all_workers) {
-  constexpr int kJoinWarps = kJoinThreads / 32;
+__global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks,
+                                                                const long long all_workers, const int rows_each) {
   constexpr int kEach = D / 32;
-  __shared__ float part[kJoinWarps][D];
+  __shared__ float part[kJoinMost / 32][D];
+  __shared__ float sums[kJoinMost / 32];
   griddep_launch_dependents();
   griddep_wait();
-  const int row = blockIdx.x % rows.count;
-  const int bh = blockIdx.x / rows.count, b = bh / c.H, h = bh - b * c.H;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int item = blockIdx.x % (c.H * row_blocks), b = blockIdx.x / (c.H * row_blocks), h = item / row_blocks;
+  const int from = blockIdx.y * rows_each, row0 = (item - h * row_blocks) * 8 * NT + from;
+  const int count = min(min(rows_each, 8 * NT - from), rows.count - row0);   // rows of this CTA
+  if (count <= 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int tiles = tiles_of(c, a.counts, b);
-  const int t = row / rows.group, hq = h * rows.group + row - t * rows.group;
-  uint16_t* dst = static_cast<uint16_t*>(a.o) + b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2];
-  float* lse = a.lse != nullptr ? a.lse + (static_cast<int64_t>(b) * a.Hq + hq) * a.S + t : nullptr;
+  auto answer = [&](int row, int64_t* at_lse) {
+    const int t = row / rows.group, hq = h * rows.group + row - t * rows.group;
+    *at_lse = (static_cast<int64_t>(b) * a.Hq + hq) * a.S + t;
+    return static_cast<uint16_t*>(a.o) + b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2];
+  };
   if (tiles == 0) {
-    for (int d = threadIdx.x; d < D; d += kJoinThreads) dst[d] = 0;
-    if (threadIdx.x == 0 && lse != nullptr) *lse = -INFINITY;
+    for (int r = warp; r < count; r += warps) {
+      int64_t at_lse;
+      uint16_t* dst = answer(row0 + r, &at_lse);
+      for (int d = lane; d < D; d += 32) dst[d] = 0;
+      if (lane == 0 && a.lse != nullptr) a.lse[at_lse] = -INFINITY;
+    }
     return;
   }
   const int per_sequence = c.H * row_blocks;
-  const long long total = tiles_before(c, a.counts, c.B) * per_sequence;
+  long long before;
+  const long long total = all_tiles(c, a.counts, b, &before) * per_sequence;
   const long long workers = workers_used(total, all_workers);
-  const int block = row / (8 * NT), r = row - block * 8 * NT;
-  const long long first = tiles_before(c, a.counts, b) * per_sequence + static_cast<long long>(h * row_blocks + block) * tiles;
+  const long long first = before * per_sequence + static_cast<long long>(item) * tiles;
   const long long w0 = worker_of(total, first, workers), w1 = worker_of(total, first + tiles - 1, workers);
   if (w0 == w1) return;                       // in one piece: answered already
   const int pieces = static_cast<int>(w1 - w0) + 1;
-  auto piece_of = [&](int i) {                // the first one is its worker's last item, the others their workers' first
-    return a.pieces + ((w0 + i) * 2 + (i == 0)) * piece_floats<D, NT>() + r * (D + 2);
-  };
-  float ref = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) ref = fmaxf(ref, piece_of(i)[D]);
+  // the warps in teams, one per row, as far as they go
+  const int teams = min(count, warps), members = warps / teams, team = warp % teams, member = warp / teams;
+  for (int r0 = 0; r0 < count; r0 += teams) {
+    const int r = r0 + team;
+    const bool busy = r < count && member < members;
+    float ref = kNoScore;
+    if (busy) {
+      auto piece_of = [&](int i) {            // the first one is its worker's last item, the others their workers' first
+        return a.pieces + ((w0 + i) * 2 + (i == 0)) * piece_floats<D, NT>() + (from + r) * (D + 2);
+      };
+      for (int i = lane; i < pieces; i += 32) ref = fmaxf(ref, piece_of(i)[D]);
 #pragma unroll
-  for (int d = 16; d; d >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, d));
-  float l = 0.f;
-  for (int i = lane; i < pieces; i += 32) {
-    const float* p = piece_of(i);
-    // what a piece that saw nothing holds: no reference and a sum of zero
-    l += p[D] == -INFINITY ? p[D + 1] : ex2(p[D] - ref) * p[D + 1];
-  }
+      for (int d = 16; d; d >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, d));
+      float sum[kEach], l = 0.f;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  float sum[kEach];
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) sum[j] = 0.f;
+      for (int j = 0; j < kEach; ++j) sum[j] = 0.f;
 #pragma unroll 4
-  for (int i = warp; i < pieces; i += kJoinWarps) {
-    const float* p = piece_of(i);
-    const float by = p[D] == -INFINITY ? 1.f : ex2(p[D] - ref);
+      for (int i = member; i < pieces; i += members) {
+        const float* p = piece_of(i);
+        const float by = ex2(p[D] - ref);
+        l += by * p[D + 1];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) sum[j] += by * p[lane + 32 * j];
+        for (int j = 0; j < kEach; ++j) sum[j] += by * p[lane + 32 * j];
+      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) part[warp][lane + 32 * j] = sum[j];
+      if (lane == 0) sums[warp] = l;
+    }
+    __syncthreads();
+    if (busy && member == 0) {
+      float o[kEach], l = 0.f;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) o[j] = 0.f;
+      for (int m = 0; m < members; ++m) {
+        l += sums[team + m * teams];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) o[j] += part[team + m * teams][lane + 32 * j];
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      int64_t at_lse;
+      uint16_t* dst = answer(row0 + r, &at_lse);
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) dst[lane + 32 * j] = from_f32<kBf16>(o[j] * inv);
+      if (lane == 0 && a.lse != nullptr) a.lse[at_lse] = l == 0.f ? -INFINITY : (ref + __log2f(l)) * kLn2;
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) part[warp][lane + 32 * j] = sum[j];
-  __syncthreads();
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int d = threadIdx.x; d < D; d += kJoinThreads) {
-    float o = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) o += part[w][d];
-    dst[d] = from_f32<kBf16>(o * inv);
-  }
-  if (threadIdx.x == 0 && lse != nullptr) *lse = l == 0.f ? -INFINITY : (ref + __log2f(l)) * kLn2;
 }
 
-// The weights: every token's softmax weights over all query rows of its K/V head, added to weight[].  The scores are
-// computed again from K, against the rows' log-sum-exp; a token belongs to one warp, so nothing is added twice at once.
+// The weights: every token's softmax weights over all query rows of its K/V head, added to weight[].  A token belongs to
+// one warp, so nothing is added twice at once and the order is fixed.  This one reads the scores that the attention
+// kernel has kept, 4 bytes per row and token: one tile of 32 tokens per warp at a time, one token per lane.
+template <int NT>
+__global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c, const Cache4Attention a, const Rows rows) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  long long none;
+  const long long total = all_tiles(c, a.counts, 0, &none) * c.H;
+  const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
+  if (worker >= workers) return;
+  Cursor k = cursor_at(c, a.counts, c.H, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  const int mask = (1 << c.page_shift) - 1;
+  while (k.left > 0) {
+    // log-sum-exps of the item's rows, one per lane (there are no more than 16)
+    float lse = 0.f;
+    if (lane < rows.count) {
+      const int t = lane / rows.group, hq = k.item * rows.group + lane - t * rows.group;
+      lse = a.lse[(static_cast<int64_t>(k.b) * a.Hq + hq) * a.S + t] * kLog2e;
+      if (lse == -INFINITY) lse = 0.f;                         // a row that sees nothing: its scores are -inf
+    }
+    const int run = min(k.tiles - k.t, k.left);
+    for (int i = 0; i < run; ++i) {
+      const float* scores = a.scores + (k.at + i) * rows.count * kTile + lane;
+      float sum = 0.f;
+#pragma unroll 8
+      for (int r = 0; r < rows.count; ++r) sum += ex2(scores[r * kTile] - __shfl_sync(0xffffffffu, lse, r));
+      const int slot = (k.t + i) * kTile + lane;
+      int64_t page;
+      if (slot < k.n && find_page(c, k.b, slot, &page))
+        c.weight[page * c.weight_stride[0] + k.item * c.weight_stride[1] + (slot & mask)] += sum;
+    }
+    k.left -= run;
+    k.at += run;
+    if (k.left > 0) next_item(k, c, a.counts, c.H);
+  }
+}
+
+// The same with more rows than one block: the scores are computed again from K, against the rows' log-sum-exp.
 template <int D, int NT, bool kBf16>
-__global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks) {
+__global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks) {
   using R = Record<D>;
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-  const long long total = tiles_before(c, a.counts, c.B) * c.H;
+  long long none;
+  const long long total = all_tiles(c, a.counts, 0, &none) * c.H;
   const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
   if (worker >= workers) return;
-  long long at = share_begin(total, worker, workers);
-  const long long end = share_begin(total, worker + 1, workers);
-  long long first;
-  int tiles;
-  int b = sequence_of(c, a.counts, c.H, at, &first, &tiles);
+  Cursor k = cursor_at(c, a.counts, c.H, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
   const int mask = (1 << c.page_shift) - 1;
-  while (at < end) {
-    if (at >= first + static_cast<long long>(tiles) * c.H) b = sequence_of(c, a.counts, c.H, at, &first, &tiles);
-    const int h = static_cast<int>((at - first) / tiles);
-    const int t0 = static_cast<int>(at - first - static_cast<long long>(h) * tiles);
-    const int t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + end - at));
-    const int n = tokens_of(c, b);
+  while (k.left > 0) {
+    const int run = min(k.tiles - k.t, k.left);
     for (int block = 0; block < row_blocks; ++block) {
       Query<D, NT> f;
-      load_query<D, NT, kBf16>(f, c, a, rows, b, h, 8 * NT * block, n);
+      load_query<D, NT, kBf16>(f, c, a, rows, k.b, k.item, 8 * NT * block, k.n);
       float lse[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int row = 8 * (NT * block + nt) + 2 * q4 + i, t = row / rows.group, hq = h * rows.group + row - t * rows.group;
-          lse[nt][i] = f.last[nt][i] >= 0 ? a.lse[(static_cast<int64_t>(b) * a.Hq + hq) * a.S + t] * kLog2e : 0.f;
+          const int row = 8 * (NT * block + nt) + 2 * q4 + i, t = row / rows.group, hq = k.item * rows.group + row - t * rows.group;
+          if (row >= rows.count) f.last[nt][i] = -1;
+          lse[nt][i] = f.last[nt][i] >= 0 ? a.lse[(static_cast<int64_t>(k.b) * a.Hq + hq) * a.S + t] * kLog2e : 0.f;
         }
-      for (int t = 2 * t0; t < 2 * t1; ++t) {
+      for (int t = 2 * k.t; t < 2 * (k.t + run); ++t) {
         const int slot = 16 * t;
         int64_t page;
-        if (slot >= n || !find_page(c, b, slot, &page)) continue;
+        if (slot >= k.n || !find_page(c, k.b, slot, &page)) continue;
         float s[NT][4];
-        block_scores<D, NT, kBf16>(s, c.kv + page * c.kv_stride[0] + h * c.kv_stride[1] + static_cast<int64_t>(slot & mask) * R::kBytes, f);
+        block_scores<D, NT, kBf16>(s, c.kv + page * c.kv_stride[0] + k.item * c.kv_stride[1] + static_cast<int64_t>(slot & mask) * R::kBytes, f);
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (slot + g + 8 * (j >> 1) <= f.last[nt][j & 1]) sum[j >> 1] += ex2(s[nt][j] - lse[nt][j & 1]);
+            if (slot + g + 8 * (j >> 1) <= f.last[nt][j & 1]) sum[j >> 1] += ex2(fmaf(s[nt][j], f.factor[nt][j & 1], -lse[nt][j & 1]));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
           sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-          if (q4 == 0 && slot + g + 8 * i < n)
-            c.weight[page * c.weight_stride[0] + h * c.weight_stride[1] + (slot & mask) + g + 8 * i] += sum[i];
+          if (q4 == 0 && slot + g + 8 * i < k.n)
+            c.weight[page * c.weight_stride[0] + k.item * c.weight_stride[1] + (slot & mask) + g + 8 * i] += sum[i];
         }
       }
     }
-    at += t1 - t0;
+    k.left -= run;
+    if (k.left > 0) next_item(k, c, a.counts, c.H);
   }
 }
 
@@ -749,12 +865,27 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, kThreads, Sh::kRingBytes, stream, pdl, c, a, rows, row_blocks, option_wait_limit_ns());
   if (e != cudaSuccess) return e;
   *launches += 1;
-  e = launch_persistent(cache4_join_kernel<D, NT, kBf16>, c.B * c.H * rows.count, kJoinThreads, 0, stream, pdl, c, a, rows, row_blocks,
-                        static_cast<long long>(grid) * kWarps);
+  // Few items are cut into many pieces each: then every row gets a large CTA of its own.
+  const int items = c.B * c.H * row_blocks;
+  const bool many_pieces = static_cast<long long>(grid) * kWarps > 8ll * items;
+  const int rows_each = many_pieces ? 1 : 8 * NT;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items), static_cast<unsigned>(many_pieces ? (rows.count < 8 * NT ? rows.count : 8 * NT) : 1));
+  cfg.blockDim = dim3(many_pieces ? kJoinMost : kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, cache4_join_kernel<D, NT, kBf16>, c, a, rows, row_blocks, static_cast<long long>(grid) * kWarps, rows_each);
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (c.weight != nullptr) {
-    e = launch_persistent(cache4_weight_kernel<D, NT, kBf16>, 2 * sm_count, kThreads, 0, stream, pdl, c, a, rows, row_blocks);
+    if (row_blocks == 1)
+      e = launch_persistent(cache4_weight_kernel<NT>, 8 * sm_count, kThreads, 0, stream, pdl, c, a, rows);
+    else
+      e = launch_persistent(cache4_weight_again_kernel<D, NT, kBf16>, 4 * sm_count, kThreads, 0, stream, pdl, c, a, rows, row_blocks);
     if (e == cudaSuccess) *launches += 1;
   }
   return e;
@@ -779,11 +910,18 @@ template <int D, int NT>
 size_t pieces_bytes(int sm_count) {
   return static_cast<size_t>(sm_count) * Shape<D, NT>::kCtas * kWarps * 2 * piece_floats<D, NT>() * sizeof(float);
 }
-size_t cache4_attention_workspace(int D, int Hq, int H, int S, int sm_count) {
-  const bool wide = sixteen_rows(D, Hq / H * S);
-  if (D == 64) return wide ? pieces_bytes<64, 2>(sm_count) : pieces_bytes<64, 1>(sm_count);
-  if (D == 128) return wide ? pieces_bytes<128, 2>(sm_count) : pieces_bytes<128, 1>(sm_count);
-  return pieces_bytes<256, 1>(sm_count);
+// The pieces, then the kept scores of the longest sequences that the table allows.
+Cache4Workspace cache4_attention_workspace(const Cache4& c, int Hq, int S, int sm_count) {
+  const int rows = Hq / c.H * S;
+  const bool wide = sixteen_rows(c.D, rows);
+  Cache4Workspace w;
+  w.pieces = c.D == 64    ? (wide ? pieces_bytes<64, 2>(sm_count) : pieces_bytes<64, 1>(sm_count))
+             : c.D == 128 ? (wide ? pieces_bytes<128, 2>(sm_count) : pieces_bytes<128, 1>(sm_count))
+                          : pieces_bytes<256, 1>(sm_count);
+  const bool one_block = rows <= (wide ? 16 : 8);
+  const size_t tiles = static_cast<size_t>(c.B) * c.H * (((static_cast<size_t>(c.max_pages) << c.page_shift) + kTile - 1) / kTile);
+  w.total = w.pieces + (c.weight != nullptr && one_block ? tiles * rows * kTile * sizeof(float) : 0);
+  return w;
 }
 
 cudaError_t launch_cache4_attention(const Cache4& c, const Cache4Attention& a, int sm_count, cudaStream_t stream, long long* launches) {

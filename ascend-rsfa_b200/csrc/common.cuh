@@ -93,7 +93,8 @@ struct Cache4Attention {
   int Hq, S;
   const int* counts;       // may be null
   float sm_scale;
-  float* pieces;           // workspace
+  float* pieces;           // workspace: partial sums
+  float* scores;           // workspace: scores kept for the weights
 };
 
 struct Cache4Evict {
@@ -157,7 +158,10 @@ cudaError_t launch_rotary_table(float* table, int length, int dim, const double*
 cudaError_t launch_cache4_append(const Cache4& c, const Cache4Rows& r, cudaStream_t stream, long long* launches);
 cudaError_t launch_cache4_read(const Cache4& c, const Cache4Rows& r, cudaStream_t stream, long long* launches);
 cudaError_t launch_cache4_attention(const Cache4& c, const Cache4Attention& a, int sm_count, cudaStream_t stream, long long* launches);
-size_t cache4_attention_workspace(int D, int Hq, int H, int S, int sm_count);
+struct Cache4Workspace {
+  size_t pieces, total;   // bytes
+};
+Cache4Workspace cache4_attention_workspace(const Cache4& c, int Hq, int S, int sm_count);
 cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& e, int sm_count, cudaStream_t stream, long long* launches);
 size_t cache4_evict_workspace(int B, int H, int budget);
 // Adds to the process-wide kernel-launch counter behind rsfa_launch_count().

@@ -194,9 +194,11 @@ int rsfa_cache4_read(const rsfa_cache4* cache, void* k, void* v, int N, const in
   return rsfa::end_call(d, static_cast<cudaStream_t>(stream), e, launches);
 }
 
-long long rsfa_cache4_attention_workspace(int head_dim, int q_heads, int heads, int S) {
-  if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || heads < 1 || q_heads < heads || q_heads % heads != 0 || S < 1)
-    return RSFA_ERR_INVALID_ARGUMENT;
+long long rsfa_cache4_attention_workspace(const rsfa_cache4* cache, int q_heads, int S) {
+  rsfa::Cache4 c;
+  const int rc = take_cache(cache, &c);
+  if (rc != RSFA_OK) return rc;
+  if (q_heads < c.H || q_heads % c.H != 0 || S < 1) return RSFA_ERR_INVALID_ARGUMENT;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) {
     cudaGetLastError();
@@ -204,7 +206,7 @@ long long rsfa_cache4_attention_workspace(int head_dim, int q_heads, int heads, 
   }
   const int sms = rsfa_sm_count(device);
   if (sms <= 0) return sms;
-  return static_cast<long long>(rsfa::cache4_attention_workspace(head_dim, q_heads, heads, S, sms));
+  return static_cast<long long>(rsfa::cache4_attention_workspace(c, q_heads, S, sms).total);
 }
 
 int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, float* lse, int q_heads, int S, const int64_t* strides,
@@ -219,9 +221,8 @@ int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, floa
   rsfa::CallScratch d;
   rc = rsfa::begin_call(&d);
   if (rc != RSFA_OK) return rc;
-  if (workspace == nullptr || !aligned(workspace, 16) ||
-      workspace_bytes < static_cast<long long>(rsfa::cache4_attention_workspace(c.D, q_heads, c.H, S, d.sm_count)))
-    return RSFA_ERR_INVALID_ARGUMENT;
+  const rsfa::Cache4Workspace need = rsfa::cache4_attention_workspace(c, q_heads, S, d.sm_count);
+  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < static_cast<long long>(need.total)) return RSFA_ERR_INVALID_ARGUMENT;
   c.status = d.status;
   rsfa::Cache4Attention a;
   std::memset(&a, 0, sizeof(a));
@@ -237,6 +238,7 @@ int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, floa
   a.counts = counts;
   a.sm_scale = sm_scale;
   a.pieces = static_cast<float*>(workspace);
+  a.scores = a.pieces + need.pieces / sizeof(float);
   long long launches = 0;
   const cudaError_t e = rsfa::launch_cache4_attention(c, a, d.sm_count, static_cast<cudaStream_t>(stream), &launches);
   return rsfa::end_call(d, static_cast<cudaStream_t>(stream), e, launches);

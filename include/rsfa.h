@@ -134,8 +134,8 @@ RSFA_API int rsfa_fwd_noalloc(const void* q, const void* k, const void* v, void*
  * device, allocate nothing (but the library's workspace on a device's first call, which therefore
  * is made outside stream capture) and keep nothing from one call for the next; scratch is the
  * caller's, and a scratch buffer belongs to one call at a time.  What lies in device memory cannot
- * be checked when a call is made: a position, page number or length that is out of range is skipped by
- * the kernel that finds it and leaves (2 << 16) | tag in the status word (rsfa_device_status): tag
+ * be checked when a call is made: a kernel that finds a position, page number or length out of range
+ * touches nothing outside, goes on (the results of that sequence have no meaning) and leaves (2 << 16) | tag in the status word (rsfa_device_status): tag
  * 1 a position outside the rotary table, 2 a page outside the cache, 3 a length below zero or beyond the
  * sequence's pages.
  */
@@ -217,7 +217,7 @@ RSFA_API int rsfa_cache4_read(const rsfa_cache4* cache, void* k, void* v, int N,
  * query rows of its K/V head.  Results do not depend on timing.  strides: 8 element strides, q[4], o[4].
  * workspace: rsfa_cache4_attention_workspace bytes (or a negative error), 16-byte aligned, no content asked for.
  */
-RSFA_API long long rsfa_cache4_attention_workspace(int head_dim, int q_heads, int heads, int S);
+RSFA_API long long rsfa_cache4_attention_workspace(const rsfa_cache4* cache, int q_heads, int S);
 RSFA_API int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, float* lse, int q_heads, int S,
                                    const int64_t* strides, const int* counts, float sm_scale, void* workspace,
                                    long long workspace_bytes, void* stream);

@@ -125,7 +125,7 @@ def test_c_refusals_need_no_device():
     assert lib.rsfa_cache4_evict(c, 8, 2, p, p, 1 << 40, None) == bad                           # new_lengths are lengths
     assert lib.rsfa_cache4_evict(c_cache(weight=None), 8, 2, ctypes.c_void_p(8192), p, 1 << 40, None) == bad
     assert lib.rsfa_cache4_evict_workspace(2, 2, 8) > 0 and lib.rsfa_cache4_evict_workspace(0, 2, 8) == bad
-    assert lib.rsfa_cache4_attention_workspace(48, 2, 2, 1) == bad and lib.rsfa_cache4_attention_workspace(64, 3, 2, 1) == bad
+    assert lib.rsfa_cache4_attention_workspace(c_cache(head_dim=48), 2, 1) == bad and lib.rsfa_cache4_attention_workspace(c, 3, 1) == bad
 
 
 def test_oracle_record_round_trip():
