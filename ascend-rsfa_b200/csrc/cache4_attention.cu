@@ -47,6 +47,27 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The 16-bit numbers of the cache's own type.
+template <bool kBf16>
+__device__ __forceinline__ void mma_own(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    mma_f16(c, a0, a1, a2, a3, b0, b1);
+}
+// 8 s + m of two neighbouring tokens' pairs (low half scale, high half minimum).
+template <bool kBf16>
+__device__ __forceinline__ uint32_t middles(uint32_t first, uint32_t second) {
+  const uint32_t s = __byte_perm(first, second, 0x5410), m = __byte_perm(first, second, 0x7632);
+  uint32_t r;
+  if constexpr (kBf16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(s), "r"(0x41004100u), "r"(m));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(s), "r"(0x48004800u), "r"(m));
+  return r;
+}
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -161,7 +182,10 @@ template <int D, int NT>
 struct Query {
   static constexpr int G = D / 32;
   uint32_t frag[NT][G][4];
-  float sums[NT][G][2];     // of rows 2 c, 2 c + 1 (c = lane % 4), times 2^-24
+  // Sums of the groups times 2^-6, as three numbers of the cache's type each: B fragments of the product with the
+  // minima, whose k index runs over (part, group).
+  static constexpr int kSumMmas = G == 8 ? 2 : 1;
+  uint32_t sums[NT][kSumMmas][2];
   float factor[NT][2];      // > 0, log2 units
   int last[NT][2];          // last visible slot
   int last_all;             // slots up to here are visible to every row
@@ -204,9 +228,10 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
     e = max(min(e, 100), -100);
     const float down = copysignf(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), a.sm_scale);   // 2^-e, and the scale's sign
     const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    float rest[G];
 #pragma unroll
     for (int w = 0; w < G; ++w) {
-      float sum = 0.f;
+      float sum = 0.f;   // of the group
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[w][j] *= down;
@@ -219,9 +244,22 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
       f.frag[nt][w][3] = from_f32x2<false>(x[w][3] * 0.0625f, x[w][7] * 0.0625f);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= 5.9604644775390625e-8f;   // 2^-24
-      f.sums[nt][w][0] = __shfl_sync(0xffffffffu, sum, 8 * q4);
-      f.sums[nt][w][1] = __shfl_sync(0xffffffffu, sum, 8 * q4 + 4);
+      rest[w] = sum * 0.015625f;
+    }
+    // parts of (2 c, 2 c + 1) of 16 or 32 numbers (part, group)
+#pragma unroll
+    for (int k = 0; k < 2 * Query<D, NT>::kSumMmas; ++k) f.sums[nt][k >> 1][k & 1] = 0u;
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+#pragma unroll
+      for (int w = 0; w < G; w += 2) {
+        const uint32_t pair = from_f32x2<kBf16>(rest[w], rest[w + 1]);
+        const float2 taken = to_f32x2<kBf16>(pair);
+        rest[w] -= taken.x;
+        rest[w + 1] -= taken.y;
+        const int at = part * G + w;                   // k index of the pair
+        if (2 * q4 == (at & 7)) f.sums[nt][at >> 4][(at >> 3) & 1] = pair;
+      }
     }
     const float factor = fmaxf(up * 16777216.f * (fabsf(a.sm_scale) * kLog2e), 1e-37f);   // -inf times it stays -inf
     f.factor[nt][0] = __shfl_sync(0xffffffffu, factor, 8 * q4);
@@ -265,36 +303,47 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
       ph[4 * q] = y.x, ph[4 * q + 1] = y.y, ph[4 * q + 2] = y.z, ph[4 * q + 3] = y.w;
     }
   }
+  // the minima's part: groups (2 c, 2 c + 1) of either token, in every place of the k index that stands for them
+  const int w2 = (2 * q4) % G;
+  const uint2 ml = *reinterpret_cast<const uint2*>(lo + R::kKPairs + 4 * w2), mh = *reinterpret_cast<const uint2*>(hi + R::kKPairs + 4 * w2);
+  const uint32_t m_lo = __byte_perm(ml.x, ml.y, 0x7632), m_hi = __byte_perm(mh.x, mh.y, 0x7632);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[nt][j] = 0.f;
 #pragma unroll
+    for (int k = 0; k < Query<D, NT>::kSumMmas; ++k) mma_own<kBf16>(s[nt], m_lo, m_hi, m_lo, m_hi, f.sums[nt][k][0], f.sums[nt][k][1]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[nt][j] *= 3.814697265625e-6f;   // 2^6 and 2^-24
+  }
+#pragma unroll
   for (int w = 0; w < G; ++w) {
     const uint32_t a8 = kl[w] >> 8, b8 = kh[w] >> 8;
-    const float2 sl = to_f32x2<kBf16>(pl[w]), sh = to_f32x2<kBf16>(ph[w]);
+    const float sl = to_f32<kBf16>(static_cast<uint16_t>(pl[w])), sh = to_f32<kBf16>(static_cast<uint16_t>(ph[w]));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float acc[4];
       mma_f16_first(acc, kl[w] & 0x000f000fu, kh[w] & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu, f.frag[nt][w][0], f.frag[nt][w][1]);
       mma_f16(acc, kl[w] & 0x00f000f0u, kh[w] & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u, f.frag[nt][w][2], f.frag[nt][w][3]);
-      s[nt][0] = fmaf(sl.x, acc[0], fmaf(sl.y, f.sums[nt][w][0], s[nt][0]));
-      s[nt][1] = fmaf(sl.x, acc[1], fmaf(sl.y, f.sums[nt][w][1], s[nt][1]));
-      s[nt][2] = fmaf(sh.x, acc[2], fmaf(sh.y, f.sums[nt][w][0], s[nt][2]));
-      s[nt][3] = fmaf(sh.x, acc[3], fmaf(sh.y, f.sums[nt][w][1], s[nt][3]));
+      s[nt][0] = fmaf(sl, acc[0], s[nt][0]);
+      s[nt][1] = fmaf(sl, acc[1], s[nt][1]);
+      s[nt][2] = fmaf(sh, acc[2], s[nt][2]);
+      s[nt][3] = fmaf(sh, acc[3], s[nt][3]);
     }
   }
 }
 
 // The sums of one piece of an item.  A code u enters the second product as it is, but the rounding of p * s would then
 // show times u: sum p s u + sum p m is taken as sum P u - 8 sum P + sum p (m + 8 s), P = fp16(p s), which leaves it
-// times u - 8, half as much on average.  The sum of P comes out of an MMA of its own (`eights`), whose row w is group w.
+// times u - 8, half as much on average.  The sum of P comes out of an MMA of its own (`eights`), whose row w is group w, and
+// so does the last sum (`mids`), with p and m + 8 s rounded to the cache's type like the weights and values of any
+// 16-bit attention.
 template <int D, int NT>
 struct Sums {
   static constexpr int G = D / 32;
   float o[2 * G][NT][4];       // tile 2 w + t: dims 32 w + 4 g + 2 t (times 2^-24) and + 1 (times 2^-20), both over `unit`
   float eights[NT][4];         // 8 sum P of group g = lane / 4, rows 2 c, 2 c + 1, times 2^-24 over `unit`
-  float mids[G][NT][2];        // this lane's share of sum p (m + 8 s), rows 2 c, 2 c + 1
+  float mids[NT][4];           // sum p (m + 8 s) of group g % G, rows 2 c, 2 c + 1 (twice)
   float l[NT][2], ref[NT][2];
   float unit;                  // power of two that p * s is divided by
   uint32_t unit_limit;         // 16-bit pattern of the scale from which on it is raised
@@ -307,15 +356,13 @@ __device__ __forceinline__ void clear(Sums<D, NT>& x) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x.eights[nt][i] = 0.f;
+    for (int i = 0; i < 4; ++i) x.eights[nt][i] = x.mids[nt][i] = 0.f;
 #pragma unroll
     for (int j = 0; j < 2 * (D / 32); ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) x.o[j][nt][i] = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) x.mids[w][nt][i] = 0.f;
       x.l[nt][i] = 0.f;
       x.ref[nt][i] = kNoScore;
     }
@@ -324,17 +371,40 @@ __device__ __forceinline__ void clear(Sums<D, NT>& x) {
   x.unit_limit = 0;
 }
 
-// The second product of 16 tokens: p of tokens (g, g + 8).  kCareful: some scale is NaN, and hidden tokens must not show.
-template <int D, int NT, bool kBf16, bool kCareful>
+// Tokens of a block whose V pairs are NaN: a row that gives one of them weight gets NaN for the group, and the pairs
+// are made zeros, so that rows which do not see the token do not see NaN either.
+template <int D, int NT, bool kBf16>
+__device__ __noinline__ void defuse_block(uint8_t* rec, const float* p, float* mids) {
+  using R = Record<D>;
+  constexpr int G = D / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  for (int token = 0; token < 16; ++token) {
+    const uint32_t pair = *reinterpret_cast<const uint32_t*>(rec + token * R::kBytes + R::kVPairs + 4 * (g % G));
+    const float2 sm = to_f32x2<kBf16>(pair);
+    const bool nan = !(fabsf(sm.x) < INFINITY && fabsf(sm.y) < INFINITY);
+    for (int nt = 0; nt < NT; ++nt)
+      for (int i = 0; i < 2; ++i) {
+        const float w = __shfl_sync(0xffffffffu, p[4 * nt + 2 * (token >> 3) + i], 4 * (token & 7) + q4);
+        if (nan && w != 0.f) mids[4 * nt + i] = __int_as_float(0x7fffffff);
+      }
+    __syncwarp();
+    if (nan && q4 == 0 && g < G) *reinterpret_cast<uint32_t*>(rec + token * R::kBytes + R::kVPairs + 4 * g) = 0u;
+  }
+  __syncwarp();
+}
+
+// The second product of 16 tokens: p of tokens (g, g + 8).
+template <int D, int NT, bool kBf16>
 __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT][4], const uint8_t* rec, float per_unit) {
   using R = Record<D>;
   constexpr int G = D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   constexpr int kWords = G / 2;                  // 32-bit words of one token's V codes in a lane
-  uint32_t v[4][kWords], pl[G], ph[G];
+  uint32_t v[4][kWords], mid[4], pl[G], ph[G];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint8_t* at = rec + (2 * q4 + (j & 1) + 8 * (j >> 1)) * R::kBytes + R::kVCodes + g * (D / 16);
+    const uint8_t* token = rec + (2 * q4 + (j & 1) + 8 * (j >> 1)) * R::kBytes;
+    const uint8_t* at = token + R::kVCodes + g * (D / 16);
     if constexpr (kWords == 1) {
       v[j][0] = *reinterpret_cast<const uint32_t*>(at);
     } else if constexpr (kWords == 2) {
@@ -344,39 +414,45 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
       const uint4 u = *reinterpret_cast<const uint4*>(at);
       v[j][0] = u.x, v[j][1] = u.y, v[j][2] = u.z, v[j][3] = u.w;
     }
+    mid[j] = *reinterpret_cast<const uint32_t*>(token + R::kVPairs + 4 * (g % G));
   }
   const uint8_t* lo = rec + g * R::kBytes + R::kVPairs;
   const uint8_t* hi = lo + 8 * R::kBytes;
+  if constexpr (G == 2) {
+    const uint2 y = *reinterpret_cast<const uint2*>(lo), z = *reinterpret_cast<const uint2*>(hi);
+    pl[0] = y.x, pl[1] = y.y, ph[0] = z.x, ph[1] = z.y;
+  } else {
 #pragma unroll
-  for (int w = 0; w < G; w += 2) {
-    const uint2 y = *reinterpret_cast<const uint2*>(lo + 4 * w), z = *reinterpret_cast<const uint2*>(hi + 4 * w);
-    pl[w] = y.x, pl[w + 1] = y.y, ph[w] = z.x, ph[w + 1] = z.y;
+    for (int w = 0; w < G; w += 4) {
+      const uint4 y = *reinterpret_cast<const uint4*>(lo + 4 * w), z = *reinterpret_cast<const uint4*>(hi + 4 * w);
+      pl[w] = y.x, pl[w + 1] = y.y, pl[w + 2] = y.z, pl[w + 3] = y.w;
+      ph[w] = z.x, ph[w + 1] = z.y, ph[w + 2] = z.z, ph[w + 3] = z.w;
+    }
   }
+  const uint32_t mid_lo = middles<kBf16>(mid[0], mid[1]), mid_hi = middles<kBf16>(mid[2], mid[3]);
   float pu[NT][4];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) {
+    mma_own<kBf16>(x.mids[nt], mid_lo, mid_lo, mid_hi, mid_hi, transpose_8x8(from_f32x2<kBf16>(p[nt][0], p[nt][1])),
+                   transpose_8x8(from_f32x2<kBf16>(p[nt][2], p[nt][3])));
 #pragma unroll
     for (int j = 0; j < 4; ++j) pu[nt][j] = p[nt][j] * per_unit;
+  }
 #pragma unroll
   for (int w = 0; w < G; ++w) {
     // the half words of group w: low half token 2 c (2 c + 8), high half the token behind it
     const uint32_t pick = (w & 1) ? 0x7632u : 0x5410u;
     const uint32_t y = __byte_perm(v[0][w / 2], v[1][w / 2], pick), z = __byte_perm(v[2][w / 2], v[3][w / 2], pick);
     const uint32_t y8 = y >> 8, z8 = z >> 8;
-    const float2 sl = to_f32x2<kBf16>(pl[w]), sh = to_f32x2<kBf16>(ph[w]);
-    const float ml = fmaf(8.f, sl.x, sl.y), mh = fmaf(8.f, sh.x, sh.y);
+    const float sl = to_f32<kBf16>(static_cast<uint16_t>(pl[w])), sh = to_f32<kBf16>(static_cast<uint16_t>(ph[w]));
     const uint32_t eight = g == w ? 0x00080008u : 0u;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      auto part = [&](int j, float by) { return kCareful && p[nt][j] == 0.f ? 0.f : pu[nt][j] * by; };
-      auto mid = [&](int j, float by, float sum) { return kCareful && p[nt][j] == 0.f ? sum : fmaf(p[nt][j], by, sum); };
-      const uint32_t b0 = transpose_8x8(from_f32x2<false>(part(0, sl.x), part(1, sl.x)));
-      const uint32_t b1 = transpose_8x8(from_f32x2<false>(part(2, sh.x), part(3, sh.x)));
+      const uint32_t b0 = transpose_8x8(from_f32x2<false>(pu[nt][0] * sl, pu[nt][1] * sl));
+      const uint32_t b1 = transpose_8x8(from_f32x2<false>(pu[nt][2] * sh, pu[nt][3] * sh));
       mma_f16(x.o[2 * w][nt], y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, b0, b1);
       mma_f16(x.o[2 * w + 1][nt], y8 & 0x000f000fu, y8 & 0x00f000f0u, z8 & 0x000f000fu, z8 & 0x00f000f0u, b0, b1);
       mma_f16(x.eights[nt], eight, 0u, eight, 0u, b0, b1);
-      x.mids[w][nt][0] = mid(0, ml, mid(2, mh, x.mids[w][nt][0]));
-      x.mids[w][nt][1] = mid(1, ml, mid(3, mh, x.mids[w][nt][1]));
     }
   }
 }
@@ -396,20 +472,20 @@ __device__ __forceinline__ void raise_references(Sums<D, NT>& x, const float (&t
       x.ref[nt][i] = ref;
       x.l[nt][i] *= by;
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) x.mids[w][nt][i] *= by;
-#pragma unroll
       for (int j = 0; j < 2 * (D / 32); ++j) {
         x.o[j][nt][i] *= by;
         x.o[j][nt][i + 2] *= by;
       }
       x.eights[nt][i] *= by;
       x.eights[nt][i + 2] *= by;
+      x.mids[nt][i] *= by;
     }
 }
 
 // One tile of 32 tokens at `rec`, whose first slot is `slot`.  scores: where the tile's scores are kept, null: nowhere.
+// True if `rec` was written to.
 template <int D, int NT, bool kBf16>
-__device__ __forceinline__ void one_tile(Sums<D, NT>& x, const Query<D, NT>& f, const uint8_t* rec, int slot, float* scores, int score_rows) {
+__device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, uint8_t* rec, int slot, float* scores, int score_rows) {
   using R = Record<D>;
   constexpr int G = D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -482,11 +558,17 @@ __device__ __forceinline__ void one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
           if (r < score_rows) scores[r * kTile + 16 * k + g + 8 * (j >> 1)] = s[k][nt][j] * f.factor[nt][j & 1];
         }
     }
-    if (!odd)
-      block_output<D, NT, kBf16, false>(x, p, rec + 16 * k * R::kBytes, per_unit);
-    else
-      block_output<D, NT, kBf16, true>(x, p, rec + 16 * k * R::kBytes, per_unit);
+    if (odd) {
+      float weights[4 * NT], mids[4 * NT];
+#pragma unroll
+      for (int j = 0; j < 4 * NT; ++j) weights[j] = p[j / 4][j % 4], mids[j] = x.mids[j / 4][j % 4];
+      defuse_block<D, NT, kBf16>(rec + 16 * k * R::kBytes, weights, mids);
+#pragma unroll
+      for (int j = 0; j < 4 * NT; ++j) x.mids[j / 4][j % 4] = mids[j];
+    }
+    block_output<D, NT, kBf16>(x, p, rec + 16 * k * R::kBytes, per_unit);
   }
+  return odd;
 }
 
 // ------------------------------------------------------------------ results
@@ -506,17 +588,13 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      // sum p m: what is left of sum p (m + 8 s) without the eights of the group, which lane 4 w + q4 has
+      // what goes to every dim of a group: its mids without its eights, both of which lane 4 w + q4 has
       float l = x.l[nt][i], m[G];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      const float both = x.mids[nt][i] - low(x.eights[nt][i]);
 #pragma unroll
-      for (int w = 0; w < G; ++w) {
-        m[w] = x.mids[w][nt][i];
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) m[w] += __shfl_xor_sync(0xffffffffu, m[w], d);
-        m[w] -= low(__shfl_sync(0xffffffffu, x.eights[nt][i], 4 * w + q4));
-      }
+      for (int w = 0; w < G; ++w) m[w] = __shfl_sync(0xffffffffu, both, 4 * w + q4);
       const int r = 8 * nt + 2 * q4 + i, row = row0 + r;
       if (row < rows.count) {
         if (piece != nullptr) {
@@ -575,41 +653,47 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   const int mask = (1 << c.page_shift) - 1;
   const bool split = c.page_shift == 4;    // a tile is two pages
 
-  // Pages of tiles window .. window + 31 of sequence window_b, one per lane (two where a tile is two pages).
-  int window_b = -1, window = 0, page_lo = 0, page_hi = 0;
-  uint32_t have = 0;                       // two bits per slot: which halves of its tile have a page
+  // Pages of tiles window .. window + 31 of sequence window_b, one per lane (two where a tile is two pages); -1: none.
+  int window_b = -1, window = 0, page_lo = -1, page_hi = -1;
+  uint32_t have = 0;                       // two bits per slot: which halves of its tile have been asked for
+  int load_h = load.item / row_blocks;
   auto issue = [&](int stage) {
     if (load.b != window_b || load.t < window || load.t >= window + 32) {
       window_b = load.b;
       window = load.t;
       const int slot = (window + lane) * kTile;
       const int* row = c.table + static_cast<int64_t>(load.b) * c.table_stride;
-      page_lo = slot < load.n ? row[slot >> c.page_shift] : 0;
-      page_hi = split && slot + 16 < load.n ? row[(slot + 16) >> 4] : 0;
+      page_lo = slot < load.n ? row[slot >> c.page_shift] : -1;
+      page_hi = slot + 16 < load.n ? (split ? row[(slot + 16) >> 4] : page_lo) : -1;
+      if (slot < load.n && static_cast<unsigned>(page_lo) >= static_cast<unsigned>(c.pages)) {
+        report_bad_index(c.status, kTagCachePage);
+        page_lo = -1;
+      }
+      if (slot + 16 < load.n && static_cast<unsigned>(page_hi) >= static_cast<unsigned>(c.pages)) {
+        if (split) report_bad_index(c.status, kTagCachePage);
+        page_hi = -1;
+      }
     }
     const int lo = __shfl_sync(0xffffffffu, page_lo, load.t - window), hi = __shfl_sync(0xffffffffu, page_hi, load.t - window);
-    const int slot = load.t * kTile, left = load.n - slot;
-    const bool lo_ok = static_cast<unsigned>(lo) < static_cast<unsigned>(c.pages);
-    const bool hi_there = left > 16, hi_ok = split ? static_cast<unsigned>(hi) < static_cast<unsigned>(c.pages) : lo_ok;
-    if (!lo_ok || (hi_there && !hi_ok)) report_bad_index(c.status, kTagCachePage);
-    have = (have & ~(3u << (2 * stage))) | ((lo_ok ? 1u : 0u) | (hi_there && hi_ok ? 2u : 0u)) << (2 * stage);
+    have = (have & ~(3u << (2 * stage))) | (lo >= 0 ? 1u << (2 * stage) : 0u) | (hi >= 0 ? 2u << (2 * stage) : 0u);
     if (lane == 0) {
       constexpr uint32_t kHalf = 16 * R::kBytes;
       const uint32_t bar = my_bar + 8 * stage, dst = smem_u32(my_ring + stage * Sh::kSlotBytes);
-      const int h = load.item / row_blocks;
-      const uint8_t* head = c.kv + h * c.kv_stride[1] + static_cast<int64_t>(slot & mask) * R::kBytes;
-      if (split) {
-        mbar_arrive_expect_tx(bar, (lo_ok ? kHalf : 0u) + (hi_there && hi_ok ? kHalf : 0u));
-        if (lo_ok) bulk_load(dst, head + lo * c.kv_stride[0], bar, kHalf);
-        if (hi_there && hi_ok) bulk_load(dst + kHalf, head + hi * c.kv_stride[0], bar, kHalf);
+      const uint8_t* head = c.kv + load_h * c.kv_stride[1] + static_cast<int64_t>((load.t * kTile) & mask) * R::kBytes;
+      if (!split) {                        // a page holds whole tiles, whatever is in use of the last one
+        mbar_arrive_expect_tx(bar, lo >= 0 ? 2 * kHalf : 0u);
+        if (lo >= 0) bulk_load(dst, head + lo * c.kv_stride[0], bar, 2 * kHalf);
       } else {
-        const uint32_t bytes = !lo_ok ? 0u : hi_there ? 2 * kHalf : kHalf;
-        mbar_arrive_expect_tx(bar, bytes);
-        if (lo_ok) bulk_load(dst, head + lo * c.kv_stride[0], bar, bytes);
+        mbar_arrive_expect_tx(bar, (lo >= 0 ? kHalf : 0u) + (hi >= 0 ? kHalf : 0u));
+        if (lo >= 0) bulk_load(dst, head + lo * c.kv_stride[0], bar, kHalf);
+        if (hi >= 0) bulk_load(dst + kHalf, head + hi * c.kv_stride[0], bar, kHalf);
       }
     }
     --load.left;
-    if (++load.t == load.tiles && load.left > 0) next_item(load, c, a.counts, per_sequence);
+    if (++load.t == load.tiles && load.left > 0) {
+      next_item(load, c, a.counts, per_sequence);
+      load_h = load.item / row_blocks;
+    }
   };
 #pragma unroll 1
   for (int i = 0; i < Sh::kStages && load.left > 0; ++i) issue(i);
@@ -644,8 +728,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
         __syncwarp();
       }
       float* scores = kept != nullptr ? kept + (use.at + t - t0) * score_rows * kTile : nullptr;
-      one_tile<D, NT, kBf16>(x, f, slot, t * kTile, scores, score_rows);
-      if (patch) fence_proxy_async();      // before a copy writes where this warp has written
+      const bool written = one_tile<D, NT, kBf16>(x, f, slot, t * kTile, scores, score_rows);
+      if (patch || written) fence_proxy_async();      // before a copy writes where this warp has written
       __syncwarp();
       if (load.left > 0) issue(stage);
       if (++stage == Sh::kStages) {
