@@ -13,7 +13,7 @@
 // log2 units.  p * s is rounded to fp16 for the second product; p, its sum and the minima's term stay in 32 bits.
 //
 // What bounds it: HBM, 5 D / 4 bytes per token and K/V head, and close behind it the instructions that take the codes
-// apart.  The work is the list of all tiles of 32 tokens of all (sequence, K/V head, block of query rows), and every warp of
+// apart.  The work is the list of all tiles of 32 (64) tokens of all (sequence, K/V head, block of query rows), and every warp of
 // the device takes an equal, contiguous share of it, whatever the lengths are.  A share's first and last item may
 // continue in other warps: their sums go to a workspace and a second kernel joins them.
 #include "../../include/rsfa.h"
@@ -22,7 +22,6 @@
 namespace rsfa {
 namespace {
 
-constexpr int kTile = 32;            // tokens per tile
 constexpr int kWarps = 4;            // per CTA
 constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinThreads = 128, kJoinMost = 512;
@@ -30,11 +29,16 @@ constexpr int kJoinThreads = 128, kJoinMost = 512;
 #define C4_CTAS128 3
 #define C4_STAGES128 3
 #endif
+// Tokens per tile: what a tile costs apart from its tokens is spread over 5 KB (10 KB) of them.
+__host__ __device__ constexpr int tile_tokens(int D) { return D == 64 ? 64 : 32; }
 // CTAs per multiprocessor by the registers of their accumulators, and slots of a warp's ring by its shared memory.
 template <int D, int NT>
 struct Shape {
   static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : C4_CTAS128;
-  static constexpr int kStages = D == 64 ? 4 : D == 256 ? 2 : NT == 2 ? 4 : C4_STAGES128;
+  static constexpr int kStages = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 4) : C4_STAGES128;
+  static constexpr int kTile = tile_tokens(D);
+  static constexpr int kPieces = kTile / 16;     // loads per tile: a page holds whole ones
+  static constexpr int kPieceBytes = 16 * Record<D>::kBytes;
   static constexpr int kSlotBytes = kTile * Record<D>::kBytes;
   static constexpr int kRingBytes = kWarps * kStages * kSlotBytes;
 };
@@ -47,7 +51,21 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
 // The 16-bit numbers of the cache's own type.
+template <bool kBf16>
+__device__ __forceinline__ void mma_own_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  if constexpr (kBf16)
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(b0));
+  else
+    mma_f16_k8(c, a0, a1, b0);
+}
 template <bool kBf16>
 __device__ __forceinline__ void mma_own(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (kBf16)
@@ -91,7 +109,8 @@ __device__ __forceinline__ int visible_tokens(const Cache4& c, const int* counts
   return counts != nullptr && counts[b] <= 0 ? 0 : tokens_of(c, b);
 }
 __device__ __forceinline__ int tiles_of(const Cache4& c, const int* counts, int b) {
-  return (visible_tokens(c, counts, b) + kTile - 1) / kTile;
+  const int shift = c.D == 64 ? 6 : 5;
+  return (visible_tokens(c, counts, b) + (1 << shift) - 1) >> shift;
 }
 // One warp: tiles of all sequences and of those before b, per K/V head and block of rows.
 __device__ __forceinline__ long long all_tiles(const Cache4& c, const int* counts, int b, long long* before) {
@@ -184,8 +203,8 @@ struct Query {
   uint32_t frag[NT][G][4];
   // Sums of the groups times 2^-6, as three numbers of the cache's type each: B fragments of the product with the
   // minima, whose k index runs over (part, group).
-  static constexpr int kSumMmas = G == 8 ? 2 : 1;
-  uint32_t sums[NT][kSumMmas][2];
+  static constexpr int kSumMmas = (3 * G + 7) / 8;
+  uint32_t sums[NT][kSumMmas];
   float factor[NT][2];      // > 0, log2 units
   int last[NT][2];          // last visible slot
   int last_all;             // slots up to here are visible to every row
@@ -246,9 +265,9 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       rest[w] = sum * 0.015625f;
     }
-    // parts of (2 c, 2 c + 1) of 16 or 32 numbers (part, group)
+    // every lane has numbers 2 c, 2 c + 1 of each eight
 #pragma unroll
-    for (int k = 0; k < 2 * Query<D, NT>::kSumMmas; ++k) f.sums[nt][k >> 1][k & 1] = 0u;
+    for (int k = 0; k < Query<D, NT>::kSumMmas; ++k) f.sums[nt][k] = 0u;
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
 #pragma unroll
@@ -258,7 +277,7 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
         rest[w] -= taken.x;
         rest[w + 1] -= taken.y;
         const int at = part * G + w;                   // k index of the pair
-        if (2 * q4 == (at & 7)) f.sums[nt][at >> 4][(at >> 3) & 1] = pair;
+        if (2 * q4 == (at & 7)) f.sums[nt][at >> 3] = pair;
       }
     }
     const float factor = fmaxf(up * 16777216.f * (fabsf(a.sm_scale) * kLog2e), 1e-37f);   // -inf times it stays -inf
@@ -312,7 +331,7 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[nt][j] = 0.f;
 #pragma unroll
-    for (int k = 0; k < Query<D, NT>::kSumMmas; ++k) mma_own<kBf16>(s[nt], m_lo, m_hi, m_lo, m_hi, f.sums[nt][k][0], f.sums[nt][k][1]);
+    for (int k = 0; k < Query<D, NT>::kSumMmas; ++k) mma_own_k8<kBf16>(s[nt], m_lo, m_hi, f.sums[nt][k]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[nt][j] *= 3.814697265625e-6f;   // 2^6 and 2^-24
   }
@@ -452,7 +471,8 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
       const uint32_t b1 = transpose_8x8(from_f32x2<false>(pu[nt][2] * sh, pu[nt][3] * sh));
       mma_f16(x.o[2 * w][nt], y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, b0, b1);
       mma_f16(x.o[2 * w + 1][nt], y8 & 0x000f000fu, y8 & 0x00f000f0u, z8 & 0x000f000fu, z8 & 0x00f000f0u, b0, b1);
-      mma_f16(x.eights[nt], eight, 0u, eight, 0u, b0, b1);
+      mma_f16_k8(x.eights[nt], eight, eight, b0);
+      mma_f16_k8(x.eights[nt], eight, eight, b1);
     }
   }
 }
@@ -482,19 +502,19 @@ __device__ __forceinline__ void raise_references(Sums<D, NT>& x, const float (&t
     }
 }
 
-// One tile of 32 tokens at `rec`, whose first slot is `slot`.  scores: where the tile's scores are kept, null: nowhere.
+// One tile at `rec`, whose first slot is `slot`.  scores: where the tile's scores are kept, null: nowhere.
 // True if `rec` was written to.
 template <int D, int NT, bool kBf16>
 __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, uint8_t* rec, int slot, float* scores, int score_rows) {
   using R = Record<D>;
-  constexpr int G = D / 32;
+  constexpr int G = D / 32, kTile = tile_tokens(D), kBlocks = kTile / 16;
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-  float s[2][NT][4];
+  float s[kBlocks][NT][4];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) block_scores<D, NT, kBf16>(s[k], rec + 16 * k * R::kBytes, f);
+  for (int k = 0; k < kBlocks; ++k) block_scores<D, NT, kBf16>(s[k], rec + 16 * k * R::kBytes, f);
   if (slot + kTile - 1 > f.last_all) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < kBlocks; ++k)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -507,14 +527,17 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      top[nt][i] = fmaxf(fmaxf(s[0][nt][i], s[0][nt][i + 2]), fmaxf(s[1][nt][i], s[1][nt][i + 2])) * f.factor[nt][i];
+      float most = fmaxf(s[0][nt][i], s[0][nt][i + 2]);
+#pragma unroll
+      for (int k = 1; k < kBlocks; ++k) most = max3(most, s[k][nt][i], s[k][nt][i + 2]);
+      top[nt][i] = most * f.factor[nt][i];
       raise |= top[nt][i] > x.ref[nt][i] + kRaise;
     }
   if (__any_sync(0xffffffffu, raise)) raise_references<D, NT>(x, top);
   // a scale much above all before: each lane looks at its share of the tile's
   uint32_t widest = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2 * kBlocks; ++i)
 #pragma unroll
     for (int w = 0; w < (G + 3) / 4; ++w)
       widest = max(widest, *reinterpret_cast<const uint16_t*>(rec + (g + 8 * i) * R::kBytes + R::kVPairs + 4 * ((q4 + 4 * w) % G)) + 0u);
@@ -539,17 +562,9 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
     x.unit_limit = from_f32<kBf16>(unit * kRaiseScale);
   }
   const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(x.unit));   // 1 / a power of two
+  if (scores != nullptr) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float p[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[nt][j] = ex2(fmaf(s[k][nt][j], f.factor[nt][j & 1], -x.ref[nt][j & 1]));
-        x.l[nt][j & 1] += p[nt][j];
-      }
-    if (scores != nullptr) {
+    for (int k = 0; k < kBlocks; ++k)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -557,17 +572,29 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
           const int r = 8 * nt + 2 * q4 + (j & 1);
           if (r < score_rows) scores[r * kTile + 16 * k + g + 8 * (j >> 1)] = s[k][nt][j] * f.factor[nt][j & 1];
         }
-    }
-    if (odd) {
+  }
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[k][nt][j] = ex2(fmaf(s[k][nt][j], f.factor[nt][j & 1], -x.ref[nt][j & 1]));
+        x.l[nt][j & 1] += s[k][nt][j];
+      }
+  if (odd) {
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
       float weights[4 * NT], mids[4 * NT];
 #pragma unroll
-      for (int j = 0; j < 4 * NT; ++j) weights[j] = p[j / 4][j % 4], mids[j] = x.mids[j / 4][j % 4];
+      for (int j = 0; j < 4 * NT; ++j) weights[j] = s[k][j / 4][j % 4], mids[j] = x.mids[j / 4][j % 4];
       defuse_block<D, NT, kBf16>(rec + 16 * k * R::kBytes, weights, mids);
 #pragma unroll
       for (int j = 0; j < 4 * NT; ++j) x.mids[j / 4][j % 4] = mids[j];
     }
-    block_output<D, NT, kBf16>(x, p, rec + 16 * k * R::kBytes, per_unit);
   }
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k) block_output<D, NT, kBf16>(x, s[k], rec + 16 * k * R::kBytes, per_unit);
   return odd;
 }
 
@@ -630,6 +657,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
                                                                                         const int row_blocks, const unsigned long long wait_limit_ns) {
   using R = Record<D>;
   using Sh = Shape<D, NT>;
+  constexpr int kTile = Sh::kTile;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(8) uint64_t full_bar[kWarps * Sh::kStages];
   __shared__ int abort_word;
@@ -651,44 +679,31 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   uint8_t* const my_ring = ring + warp * Sh::kStages * Sh::kSlotBytes;
   const uint32_t my_bar = smem_u32(&full_bar[warp * Sh::kStages]);
   const int mask = (1 << c.page_shift) - 1;
-  const bool split = c.page_shift == 4;    // a tile is two pages
-
-  // Pages of tiles window .. window + 31 of sequence window_b, one per lane (two where a tile is two pages); -1: none.
-  int window_b = -1, window = 0, page_lo = -1, page_hi = -1;
-  uint32_t have = 0;                       // two bits per slot: which halves of its tile have been asked for
+  // Pages of pieces window .. window + 31 of sequence window_b, one per lane; -1: none.
+  int window_b = -1, window = 0, pages = -1;
+  uint32_t have = 0;                       // a bit per piece of every slot: asked for
   int load_h = load.item / row_blocks;
   auto issue = [&](int stage) {
-    if (load.b != window_b || load.t < window || load.t >= window + 32) {
+    const int first = load.t * Sh::kPieces;
+    if (load.b != window_b || first < window || first >= window + 32) {
       window_b = load.b;
-      window = load.t;
-      const int slot = (window + lane) * kTile;
-      const int* row = c.table + static_cast<int64_t>(load.b) * c.table_stride;
-      page_lo = slot < load.n ? row[slot >> c.page_shift] : -1;
-      page_hi = slot + 16 < load.n ? (split ? row[(slot + 16) >> 4] : page_lo) : -1;
-      if (slot < load.n && static_cast<unsigned>(page_lo) >= static_cast<unsigned>(c.pages)) {
+      window = first;
+      const int slot = (window + lane) * 16;
+      pages = slot < load.n ? c.table[static_cast<int64_t>(load.b) * c.table_stride + (slot >> c.page_shift)] : -1;
+      if (slot < load.n && static_cast<unsigned>(pages) >= static_cast<unsigned>(c.pages)) {
         report_bad_index(c.status, kTagCachePage);
-        page_lo = -1;
-      }
-      if (slot + 16 < load.n && static_cast<unsigned>(page_hi) >= static_cast<unsigned>(c.pages)) {
-        if (split) report_bad_index(c.status, kTagCachePage);
-        page_hi = -1;
+        pages = -1;
       }
     }
-    const int lo = __shfl_sync(0xffffffffu, page_lo, load.t - window), hi = __shfl_sync(0xffffffffu, page_hi, load.t - window);
-    have = (have & ~(3u << (2 * stage))) | (lo >= 0 ? 1u << (2 * stage) : 0u) | (hi >= 0 ? 2u << (2 * stage) : 0u);
-    if (lane == 0) {
-      constexpr uint32_t kHalf = 16 * R::kBytes;
-      const uint32_t bar = my_bar + 8 * stage, dst = smem_u32(my_ring + stage * Sh::kSlotBytes);
-      const uint8_t* head = c.kv + load_h * c.kv_stride[1] + static_cast<int64_t>((load.t * kTile) & mask) * R::kBytes;
-      if (!split) {                        // a page holds whole tiles, whatever is in use of the last one
-        mbar_arrive_expect_tx(bar, lo >= 0 ? 2 * kHalf : 0u);
-        if (lo >= 0) bulk_load(dst, head + lo * c.kv_stride[0], bar, 2 * kHalf);
-      } else {
-        mbar_arrive_expect_tx(bar, (lo >= 0 ? kHalf : 0u) + (hi >= 0 ? kHalf : 0u));
-        if (lo >= 0) bulk_load(dst, head + lo * c.kv_stride[0], bar, kHalf);
-        if (hi >= 0) bulk_load(dst + kHalf, head + hi * c.kv_stride[0], bar, kHalf);
-      }
-    }
+    const int page = __shfl_sync(0xffffffffu, pages, first - window + (lane & (Sh::kPieces - 1)));
+    const uint32_t asked = __ballot_sync(0xffffffffu, page >= 0) & ((1u << Sh::kPieces) - 1u);
+    have = (have & ~(((1u << Sh::kPieces) - 1u) << (Sh::kPieces * stage))) | asked << (Sh::kPieces * stage);
+    const uint32_t bar = my_bar + 8 * stage;
+    if (lane == 0) mbar_arrive_expect_tx(bar, __popc(asked) * Sh::kPieceBytes);
+    if (lane < Sh::kPieces && page >= 0)
+      bulk_load(smem_u32(my_ring + stage * Sh::kSlotBytes + lane * Sh::kPieceBytes),
+                c.kv + load_h * c.kv_stride[1] + page * c.kv_stride[0] + static_cast<int64_t>(((first + lane) * 16) & mask) * R::kBytes, bar,
+                Sh::kPieceBytes);
     --load.left;
     if (++load.t == load.tiles && load.left > 0) {
       next_item(load, c, a.counts, per_sequence);
@@ -718,8 +733,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
       uint8_t* const slot = my_ring + stage * Sh::kSlotBytes;
       // what is not there, tokens behind the last one and pages that do not exist, is made zeros
       const int left = min(n - t * kTile, kTile);
-      const uint32_t there = (have >> (2 * stage)) & 3u;
-      const bool patch = left < kTile || there != 3u;
+      const uint32_t there = (have >> (Sh::kPieces * stage)) & ((1u << Sh::kPieces) - 1u);
+      const bool patch = left < kTile || there != (1u << Sh::kPieces) - 1u;
       if (patch) {
         for (int i = lane; i < kTile * (R::kBytes / 16); i += 32) {
           const int token = i / (R::kBytes / 16);
@@ -844,8 +859,8 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
 
 // The weights: every token's softmax weights over all query rows of its K/V head, added to weight[].  A token belongs to
 // one warp, so nothing is added twice at once and the order is fixed.  This one reads the scores that the attention
-// kernel has kept, 4 bytes per row and token: one tile of 32 tokens per warp at a time, one token per lane.
-template <int NT>
+// kernel has kept, 4 bytes per row and token: 32 tokens per warp at a time, one per lane.
+template <int kTile>
 __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c, const Cache4Attention a, const Rows rows) {
   griddep_launch_dependents();
   griddep_wait();
@@ -865,12 +880,13 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
       if (lse == -INFINITY) lse = 0.f;                         // a row that sees nothing: its scores are -inf
     }
     const int run = min(k.tiles - k.t, k.left);
-    for (int i = 0; i < run; ++i) {
-      const float* scores = a.scores + (k.at + i) * rows.count * kTile + lane;
+    for (int i = 0; i < run * (kTile / 32); ++i) {
+      const int tile = i / (kTile / 32), part = i % (kTile / 32) * 32;
+      const float* scores = a.scores + (k.at + tile) * rows.count * kTile + part + lane;
       float sum = 0.f;
 #pragma unroll 8
       for (int r = 0; r < rows.count; ++r) sum += ex2(scores[r * kTile] - __shfl_sync(0xffffffffu, lse, r));
-      const int slot = (k.t + i) * kTile + lane;
+      const int slot = (k.t + tile) * kTile + part + lane;
       int64_t page;
       if (slot < k.n && find_page(c, k.b, slot, &page))
         c.weight[page * c.weight_stride[0] + k.item * c.weight_stride[1] + (slot & mask)] += sum;
@@ -885,6 +901,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
 template <int D, int NT, bool kBf16>
 __global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks) {
   using R = Record<D>;
+  constexpr int kTile = tile_tokens(D);
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -908,7 +925,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cac
           if (row >= rows.count) f.last[nt][i] = -1;
           lse[nt][i] = f.last[nt][i] >= 0 ? a.lse[(static_cast<int64_t>(k.b) * a.Hq + hq) * a.S + t] * kLog2e : 0.f;
         }
-      for (int t = 2 * k.t; t < 2 * (k.t + run); ++t) {
+      for (int t = kTile / 16 * k.t; t < kTile / 16 * (k.t + run); ++t) {
         const int slot = 16 * t;
         int64_t page;
         if (slot >= k.n || !find_page(c, k.b, slot, &page)) continue;
@@ -967,7 +984,7 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   *launches += 1;
   if (c.weight != nullptr) {
     if (row_blocks == 1)
-      e = launch_persistent(cache4_weight_kernel<NT>, 8 * sm_count, kThreads, 0, stream, pdl, c, a, rows);
+      e = launch_persistent(cache4_weight_kernel<tile_tokens(D)>, 8 * sm_count, kThreads, 0, stream, pdl, c, a, rows);
     else
       e = launch_persistent(cache4_weight_again_kernel<D, NT, kBf16>, 4 * sm_count, kThreads, 0, stream, pdl, c, a, rows, row_blocks);
     if (e == cudaSuccess) *launches += 1;
@@ -1003,8 +1020,8 @@ Cache4Workspace cache4_attention_workspace(const Cache4& c, int Hq, int S, int s
              : c.D == 128 ? (wide ? pieces_bytes<128, 2>(sm_count) : pieces_bytes<128, 1>(sm_count))
                           : pieces_bytes<256, 1>(sm_count);
   const bool one_block = rows <= (wide ? 16 : 8);
-  const size_t tiles = static_cast<size_t>(c.B) * c.H * (((static_cast<size_t>(c.max_pages) << c.page_shift) + kTile - 1) / kTile);
-  w.total = w.pieces + (c.weight != nullptr && one_block ? tiles * rows * kTile * sizeof(float) : 0);
+  const size_t tiles = static_cast<size_t>(c.B) * c.H * (((static_cast<size_t>(c.max_pages) << c.page_shift) + tile_tokens(c.D) - 1) / tile_tokens(c.D));
+  w.total = w.pieces + (c.weight != nullptr && one_block ? tiles * rows * tile_tokens(c.D) * sizeof(float) : 0);
   return w;
 }
 
