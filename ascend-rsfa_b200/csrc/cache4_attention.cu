@@ -75,6 +75,15 @@ __device__ __forceinline__ void mma_own(float (&c)[4], uint32_t a0, uint32_t a1,
   else
     mma_f16(c, a0, a1, a2, a3, b0, b1);
 }
+// sum + one half of a pair of fp16 numbers, in one instruction.
+__device__ __forceinline__ float add_low(float sum, uint32_t pair) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nadd.f32.f16 %0, l, %0;\n}\n" : "+f"(sum) : "r"(pair));
+  return sum;
+}
+__device__ __forceinline__ float add_high(float sum, uint32_t pair) {
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nadd.f32.f16 %0, h, %0;\n}\n" : "+f"(sum) : "r"(pair));
+  return sum;
+}
 // 8 s + m of two neighbouring tokens' pairs (low half scale, high half minimum).
 template <bool kBf16>
 __device__ __forceinline__ uint32_t middles(uint32_t first, uint32_t second) {
@@ -354,14 +363,13 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
 
 // The sums of one piece of an item.  A code u enters the second product as it is, but the rounding of p * s would then
 // show times u: sum p s u + sum p m is taken as sum P u - 8 sum P + sum p (m + 8 s), P = fp16(p s), which leaves it
-// times u - 8, half as much on average.  The sum of P comes out of an MMA of its own (`eights`), whose row w is group w, and
-// so does the last sum (`mids`), with p and m + 8 s rounded to the cache's type like the weights and values of any
-// 16-bit attention.
+// times u - 8, half as much on average.  The last sum (`mids`) comes out of an MMA of its own, whose row w is group w, with
+// p and m + 8 s rounded to the cache's type like the weights and values of any 16-bit attention.
 template <int D, int NT>
 struct Sums {
   static constexpr int G = D / 32;
   float o[2 * G][NT][4];       // tile 2 w + t: dims 32 w + 4 g + 2 t (times 2^-24) and + 1 (times 2^-20), both over `unit`
-  float eights[NT][4];         // 8 sum P of group g = lane / 4, rows 2 c, 2 c + 1, times 2^-24 over `unit`
+  float rounded[NT][G][2];     // this lane's share of sum P, rows 2 c, 2 c + 1, over `unit`
   float mids[NT][4];           // sum p (m + 8 s) of group g % G, rows 2 c, 2 c + 1 (twice)
   float l[NT][2], ref[NT][2];
   float unit;                  // power of two that p * s is divided by
@@ -375,7 +383,9 @@ __device__ __forceinline__ void clear(Sums<D, NT>& x) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x.eights[nt][i] = x.mids[nt][i] = 0.f;
+    for (int i = 0; i < 4; ++i) x.mids[nt][i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) x.rounded[nt][w][0] = x.rounded[nt][w][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < 2 * (D / 32); ++j)
 #pragma unroll
@@ -464,22 +474,32 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
     const uint32_t y = __byte_perm(v[0][w / 2], v[1][w / 2], pick), z = __byte_perm(v[2][w / 2], v[3][w / 2], pick);
     const uint32_t y8 = y >> 8, z8 = z >> 8;
     const float sl = to_f32<kBf16>(static_cast<uint16_t>(pl[w])), sh = to_f32<kBf16>(static_cast<uint16_t>(ph[w]));
-    const uint32_t eight = g == w ? 0x00080008u : 0u;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t b0 = transpose_8x8(from_f32x2<false>(pu[nt][0] * sl, pu[nt][1] * sl));
-      const uint32_t b1 = transpose_8x8(from_f32x2<false>(pu[nt][2] * sh, pu[nt][3] * sh));
+      const uint32_t pl2 = from_f32x2<false>(pu[nt][0] * sl, pu[nt][1] * sl), ph2 = from_f32x2<false>(pu[nt][2] * sh, pu[nt][3] * sh);
+      const uint32_t b0 = transpose_8x8(pl2), b1 = transpose_8x8(ph2);
       mma_f16(x.o[2 * w][nt], y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, b0, b1);
       mma_f16(x.o[2 * w + 1][nt], y8 & 0x000f000fu, y8 & 0x00f000f0u, z8 & 0x000f000fu, z8 & 0x00f000f0u, b0, b1);
-      mma_f16_k8(x.eights[nt], eight, eight, b0);
-      mma_f16_k8(x.eights[nt], eight, eight, b1);
+      x.rounded[nt][w][0] = add_low(add_low(x.rounded[nt][w][0], pl2), ph2);
+      x.rounded[nt][w][1] = add_high(add_high(x.rounded[nt][w][1], pl2), ph2);
     }
   }
 }
 
-// Raises the references of the rows.
-template <int D, int NT>
-__device__ __forceinline__ void raise_references(Sums<D, NT>& x, const float (&top)[NT][2]) {
+// Raises the references of the rows to the largest score of a tile, and the unit to its widest scale.  Both in one
+// place: with a branch each the sums were copied from register to register in every tile (16 of 344 instructions per 16
+// tokens).
+template <int D, int NT, bool kBf16>
+__device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2], uint32_t widest) {
+  float scale = to_f32<kBf16>(static_cast<uint16_t>(widest));
+  scale = scale < INFINITY ? scale : 0.f;                         // NaN is left to the products
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, d));
+  // the power of two below it, where it is above what the unit is for
+  const float unit = scale > x.unit * kRaiseScale ? __uint_as_float(__float_as_uint(scale) & 0x7f800000u) : x.unit;
+  const float by_unit = x.unit / unit;
+  x.unit = unit;
+  x.unit_limit = from_f32<kBf16>(unit * kRaiseScale);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -487,18 +507,18 @@ __device__ __forceinline__ void raise_references(Sums<D, NT>& x, const float (&t
       float m = top[nt][i];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      const float ref = fmaxf(m, x.ref[nt][i]);
-      const float by = ex2(x.ref[nt][i] - ref);
+      const float ref = m > x.ref[nt][i] + kRaise ? m : x.ref[nt][i];
+      const float by = ex2(x.ref[nt][i] - ref), by_both = by * by_unit;
       x.ref[nt][i] = ref;
       x.l[nt][i] *= by;
+      x.mids[nt][i] *= by;
 #pragma unroll
       for (int j = 0; j < 2 * (D / 32); ++j) {
-        x.o[j][nt][i] *= by;
-        x.o[j][nt][i + 2] *= by;
+        x.o[j][nt][i] *= by_both;
+        x.o[j][nt][i + 2] *= by_both;
       }
-      x.eights[nt][i] *= by;
-      x.eights[nt][i + 2] *= by;
-      x.mids[nt][i] *= by;
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) x.rounded[nt][w][i] *= by_both;
     }
 }
 
@@ -521,7 +541,7 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
         for (int j = 0; j < 4; ++j)
           if (slot + 16 * k + g + 8 * (j >> 1) > f.last[nt][j & 1]) s[k][nt][j] = -INFINITY;
   }
-  bool raise = false;
+  bool higher = false;
   float top[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -531,9 +551,8 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
 #pragma unroll
       for (int k = 1; k < kBlocks; ++k) most = max3(most, s[k][nt][i], s[k][nt][i + 2]);
       top[nt][i] = most * f.factor[nt][i];
-      raise |= top[nt][i] > x.ref[nt][i] + kRaise;
+      higher |= top[nt][i] > x.ref[nt][i] + kRaise;
     }
-  if (__any_sync(0xffffffffu, raise)) raise_references<D, NT>(x, top);
   // a scale much above all before: each lane looks at its share of the tile's
   uint32_t widest = 0;
 #pragma unroll
@@ -542,24 +561,9 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
     for (int w = 0; w < (G + 3) / 4; ++w)
       widest = max(widest, *reinterpret_cast<const uint16_t*>(rec + (g + 8 * i) * R::kBytes + R::kVPairs + 4 * ((q4 + 4 * w) % G)) + 0u);
   bool odd = false;
-  if (__any_sync(0xffffffffu, widest > x.unit_limit)) {
+  if (__any_sync(0xffffffffu, higher || widest > x.unit_limit)) {
     odd = __any_sync(0xffffffffu, widest > (kBf16 ? 0x7f80u : 0x7c00u));
-    float top_scale = to_f32<kBf16>(static_cast<uint16_t>(widest));
-    top_scale = top_scale < INFINITY ? top_scale : 0.f;             // NaN is left to the products
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) top_scale = fmaxf(top_scale, __shfl_xor_sync(0xffffffffu, top_scale, d));
-    const float unit = fmaxf(__uint_as_float(__float_as_uint(top_scale) & 0x7f800000u), x.unit);   // the power of two below it
-    const float by = x.unit / unit;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2 * G; ++j) x.o[j][nt][i] *= by;
-        x.eights[nt][i] *= by;
-      }
-    x.unit = unit;
-    x.unit_limit = from_f32<kBf16>(unit * kRaiseScale);
+    raise<D, NT, kBf16>(x, top, widest);
   }
   const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(x.unit));   // 1 / a power of two
   if (scores != nullptr) {
@@ -615,13 +619,17 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      // what goes to every dim of a group: its mids without its eights, both of which lane 4 w + q4 has
+      // what goes to every dim of a group: its mids, which lane 4 w + q4 has, without eight times its sum of P
       float l = x.l[nt][i], m[G];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-      const float both = x.mids[nt][i] - low(x.eights[nt][i]);
 #pragma unroll
-      for (int w = 0; w < G; ++w) m[w] = __shfl_sync(0xffffffffu, both, 4 * w + q4);
+      for (int w = 0; w < G; ++w) {
+        float sum = x.rounded[nt][w][i];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        m[w] = __shfl_sync(0xffffffffu, x.mids[nt][i], 4 * w + q4) - 8.f * sum * x.unit;
+      }
       const int r = 8 * nt + 2 * q4 + i, row = row0 + r;
       if (row < rows.count) {
         if (piece != nullptr) {
@@ -679,35 +687,47 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   uint8_t* const my_ring = ring + warp * Sh::kStages * Sh::kSlotBytes;
   const uint32_t my_bar = smem_u32(&full_bar[warp * Sh::kStages]);
   const int mask = (1 << c.page_shift) - 1;
-  // Pages of pieces window .. window + 31 of sequence window_b, one per lane; -1: none.
-  int window_b = -1, window = 0, pages = -1;
+  // The pieces window .. window + 31 of the item in `load`, one per lane: its page (-1: none) and address; the pages
+  // behind them are on their way.
+  int window = 0, pages = -1, pages_next = -1;
+  const uint8_t* piece_at = nullptr;
+  uint32_t there = 0;                      // lanes that have a page
   uint32_t have = 0;                       // a bit per piece of every slot: asked for
-  int load_h = load.item / row_blocks;
+  constexpr uint32_t kAll = (1u << Sh::kPieces) - 1u;
+  auto page_of = [&](int piece) {
+    const int slot = piece * 16;
+    return slot < load.n ? c.table[static_cast<int64_t>(load.b) * c.table_stride + (slot >> c.page_shift)] : -1;
+  };
+  auto open_window = [&](int first, int known) {
+    window = first;
+    pages = known;
+    const bool used = (window + lane) * 16 < load.n, ok = used && static_cast<unsigned>(pages) < static_cast<unsigned>(c.pages);
+    if (used && !ok) report_bad_index(c.status, kTagCachePage);
+    there = __ballot_sync(0xffffffffu, ok);
+    piece_at = c.kv + load.item / row_blocks * c.kv_stride[1] + (ok ? pages : 0) * c.kv_stride[0] +
+               static_cast<int64_t>((window + lane) * 16 & mask) * R::kBytes;
+    pages_next = page_of(window + 32 + lane);
+  };
+  open_window(load.t * Sh::kPieces, page_of(load.t * Sh::kPieces + lane));
   auto issue = [&](int stage) {
-    const int first = load.t * Sh::kPieces;
-    if (load.b != window_b || first < window || first >= window + 32) {
-      window_b = load.b;
-      window = first;
-      const int slot = (window + lane) * 16;
-      pages = slot < load.n ? c.table[static_cast<int64_t>(load.b) * c.table_stride + (slot >> c.page_shift)] : -1;
-      if (slot < load.n && static_cast<unsigned>(pages) >= static_cast<unsigned>(c.pages)) {
-        report_bad_index(c.status, kTagCachePage);
-        pages = -1;
-      }
-    }
-    const int page = __shfl_sync(0xffffffffu, pages, first - window + (lane & (Sh::kPieces - 1)));
-    const uint32_t asked = __ballot_sync(0xffffffffu, page >= 0) & ((1u << Sh::kPieces) - 1u);
-    have = (have & ~(((1u << Sh::kPieces) - 1u) << (Sh::kPieces * stage))) | asked << (Sh::kPieces * stage);
+    const int off = load.t * Sh::kPieces - window;
+    const uint32_t asked = (there >> off) & kAll;
+    have = (have & ~(kAll << (Sh::kPieces * stage))) | asked << (Sh::kPieces * stage);
     const uint32_t bar = my_bar + 8 * stage;
     if (lane == 0) mbar_arrive_expect_tx(bar, __popc(asked) * Sh::kPieceBytes);
-    if (lane < Sh::kPieces && page >= 0)
-      bulk_load(smem_u32(my_ring + stage * Sh::kSlotBytes + lane * Sh::kPieceBytes),
-                c.kv + load_h * c.kv_stride[1] + page * c.kv_stride[0] + static_cast<int64_t>(((first + lane) * 16) & mask) * R::kBytes, bar,
-                Sh::kPieceBytes);
+    const int i = lane - off;
+    if (static_cast<unsigned>(i) < Sh::kPieces && ((there >> lane) & 1))
+      bulk_load(smem_u32(my_ring + stage * Sh::kSlotBytes) + i * Sh::kPieceBytes, piece_at, bar, Sh::kPieceBytes);
     --load.left;
-    if (++load.t == load.tiles && load.left > 0) {
-      next_item(load, c, a.counts, per_sequence);
-      load_h = load.item / row_blocks;
+    if (++load.t == load.tiles) {
+      if (load.left > 0) {
+        const int b = load.b;
+        next_item(load, c, a.counts, per_sequence);
+        // the next head of a short sequence has the same pages
+        open_window(0, load.b == b && window == 0 ? pages : page_of(lane));
+      }
+    } else if (off + Sh::kPieces == 32) {
+      open_window(window + 32, pages_next);
     }
   };
 #pragma unroll 1
@@ -733,12 +753,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
       uint8_t* const slot = my_ring + stage * Sh::kSlotBytes;
       // what is not there, tokens behind the last one and pages that do not exist, is made zeros
       const int left = min(n - t * kTile, kTile);
-      const uint32_t there = (have >> (Sh::kPieces * stage)) & ((1u << Sh::kPieces) - 1u);
-      const bool patch = left < kTile || there != (1u << Sh::kPieces) - 1u;
+      const uint32_t asked = (have >> (Sh::kPieces * stage)) & kAll;
+      const bool patch = left < kTile || asked != kAll;
       if (patch) {
         for (int i = lane; i < kTile * (R::kBytes / 16); i += 32) {
           const int token = i / (R::kBytes / 16);
-          if (token >= left || !((there >> (token >> 4)) & 1)) *reinterpret_cast<uint4*>(slot + 16 * i) = make_uint4(0, 0, 0, 0);
+          if (token >= left || !((asked >> (token >> 4)) & 1)) *reinterpret_cast<uint4*>(slot + 16 * i) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
       }
