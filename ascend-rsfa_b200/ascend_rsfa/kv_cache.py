@@ -21,7 +21,7 @@ import torch
 
 from . import _capi
 from .flash_attention_forward import _DTYPES
-from .rotary import _call, _readable, _rows
+from .rotary import _call, _ordinary, _readable, _rows
 
 _lib = _capi.load()
 _HEAD_DIMS = (64, 128, 256)
@@ -100,6 +100,8 @@ def cache4_append(k, v, kv, table, lengths, counts=None, weight=None, position=N
     weight is set to 0 for the new tokens, position to positions [B, S] (int32), the number by which
     cache4_evict() knows the newest ones.
     """
+    if _ordinary("cache4_append", k, v, kv, table, lengths, counts, weight, position, positions) is not None:
+        return
     if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DTYPES:
         raise ValueError("k and v must share one shape and be both float16 or both bfloat16")
     c, lengths = _cache(kv, table, lengths, k.dtype, weight, position)
@@ -126,6 +128,9 @@ def cache4_read(kv, table, lengths, n, dtype, starts=None):
     cache's dtype; slots that are not in use are zero."""
     if dtype not in _DTYPES:
         raise ValueError("dtype must be float16 or bfloat16")
+    done = _ordinary("cache4_read", kv, table, lengths, n, dtype is torch.bfloat16, starts)
+    if done is not None:
+        return done
     c, lengths = _cache(kv, table, lengths, dtype)
     if starts is not None:
         starts = _int32(starts, (c.batch,), "starts", kv.device).contiguous()
@@ -145,6 +150,9 @@ def cache4_attention(q, kv, table, lengths, sm_scale, counts=None, weight=None, 
     weight: grows, per token and K/V head, by the softmax weights that all query rows of that head give the token.
     lse: [B, Hq, S] fp32, m + log(l).  There is no gradient.
     """
+    done = _ordinary("cache4_attention", q, kv, table, lengths, sm_scale, counts, weight, want_lse)
+    if done is not None:
+        return done if want_lse else done[0]
     if q.dtype not in _DTYPES:
         raise ValueError("q must be float16 or bfloat16")
     c, lengths = _cache(kv, table, lengths, q.dtype, weight)
@@ -185,6 +193,9 @@ def cache4_evict(kv, weight, position, table, lengths, budget, recent=0):
     weight and position; each head keeps its own choice.  Returns the new lengths, min(lengths, budget); `lengths`
     itself is left for the other layers.  No page may belong to two sequences.
     """
+    done = _ordinary("cache4_evict", kv, weight, position, table, lengths, budget, recent)
+    if done is not None:
+        return done
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget or budget > 2 ** 31 - 1:
         raise ValueError("cache4_evict() needs 0 <= recent <= budget and a budget of at least 1")

@@ -13,9 +13,14 @@ import math
 import torch
 
 from . import _capi
-from .flash_attention_forward import _DTYPES, _current_stream, _dense
+from .flash_attention_forward import _DTYPES, _current_stream, _dense, _rsfa_torch
 
 _lib = _capi.load()
+_native = _rsfa_torch   # the ordinary calls in native code (csrc/torch_binding.cpp), where that is built
+if _native is not None:
+    _native.bind_ops(*(ctypes.cast(getattr(_lib, "rsfa_" + n), ctypes.c_void_p).value for n in (
+        "rotary", "cache4_append", "cache4_read", "cache4_attention_workspace", "cache4_attention",
+        "cache4_evict_workspace", "cache4_evict")))
 _TURNS = {"yarn": (1.0, 32.0), "bands": (1.0, 4.0)}   # usual (low, high) numbers of turns over the original length
 
 
@@ -73,7 +78,20 @@ def _rows(t):
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _ordinary(what, *args):
+    """What the native form of a call returns, None where it is not an ordinary one."""
+    if _native is None:
+        return None
+    done = getattr(_native, what)(*args)
+    if type(done) is int:
+        _capi.check(done, "rsfa_" + what)
+    return done
+
+
 def _turn(q, k, table, positions, interleaved, inverse):
+    done = _ordinary("rotary", q, k, table, positions, interleaved, inverse)
+    if done is not None:
+        return done
     if q.numel() == 0 and (k is None or k.numel() == 0):
         return torch.empty_like(q), None if k is None else torch.empty_like(k)
     if k is not None and (q.numel() == 0 or k.numel() == 0):       # no heads on one side
@@ -114,11 +132,12 @@ class _rotary(torch.autograd.Function):
         # the transposed rotation of the gradients; it can be differentiated again
         table, positions = ctx.saved_tensors
         interleaved, inverse = ctx.how
+        turn = _rotary.apply if torch.is_grad_enabled() else _turn
         if dq is None:
             if dk is not None:
-                dk = _rotary.apply(dk, None, table, positions, interleaved, not inverse)[0]
+                dk = turn(dk, None, table, positions, interleaved, not inverse)[0]
         else:
-            dq, dk = _rotary.apply(dq, dk, table, positions, interleaved, not inverse)
+            dq, dk = turn(dq, dk, table, positions, interleaved, not inverse)
         return dq, dk, None, None, None, None
 
 
@@ -133,6 +152,9 @@ def rotary(q, k, table, positions=None, interleaved=False):
     Forward and backward can be captured in a CUDA graph; torch refuses that, for any operation, while a graph of the
     same leaves that was recorded on another stream is alive.
     """
+    done = _ordinary("rotary", q, k, table, positions, interleaved, False)
+    if done is not None:
+        return done
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
         raise ValueError("q and k must be [B, H, S, D] and share B, S and D")
     if q.shape[-1] not in {16, 32, 64, 128, 256}:

@@ -797,7 +797,7 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
                                                                 const long long all_workers, const int rows_each) {
   constexpr int kEach = D / 32;
   __shared__ float part[kJoinMost / 32][D];
-  __shared__ float sums[kJoinMost / 32];
+  __shared__ float2 sums[kJoinMost / 32];
   griddep_launch_dependents();
   griddep_wait();
   const int item = blockIdx.x % (c.H * row_blocks), b = blockIdx.x / (c.H * row_blocks), h = item / row_blocks;
@@ -833,38 +833,53 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
   for (int r0 = 0; r0 < count; r0 += teams) {
     const int r = r0 + team;
     const bool busy = r < count && member < members;
-    float ref = kNoScore;
     if (busy) {
       auto piece_of = [&](int i) {            // the first one is its worker's last item, the others their workers' first
         return a.pieces + ((w0 + i) * 2 + (i == 0)) * piece_floats<D, NT>() + (from + r) * (D + 2);
       };
-      for (int i = lane; i < pieces; i += 32) ref = fmaxf(ref, piece_of(i)[D]);
-#pragma unroll
-      for (int d = 16; d; d >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, d));
-      float sum[kEach], l = 0.f;
+      float ref = kNoScore, l = 0.f, sum[kEach];
 #pragma unroll
       for (int j = 0; j < kEach; ++j) sum[j] = 0.f;
-#pragma unroll 4
-      for (int i = member; i < pieces; i += members) {
-        const float* p = piece_of(i);
-        const float by = ex2(p[D] - ref);
-        l += by * p[D + 1];
+      // 32 pieces at a time: references and weights one piece per lane, the sums piece by piece
+      for (int i0 = member; i0 < pieces; i0 += 32 * members) {
+        const int mine = i0 + lane * members;
+        const float2 ml = mine < pieces ? *reinterpret_cast<const float2*>(piece_of(mine) + D) : make_float2(kNoScore, 0.f);
+        float top = ml.x;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) sum[j] += by * p[lane + 32 * j];
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        top = fmaxf(top, ref);
+        const float before = ex2(ref - top), by = ex2(ml.x - top);
+        ref = top;
+        l = l * before + by * ml.y;           // of this lane's pieces
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) sum[j] *= before;
+        const int here = min(32, (pieces - i0 + members - 1) / members);
+#pragma unroll 8
+        for (int k = 0; k < here; ++k) {
+          const float* p = piece_of(i0 + k * members);
+          const float share = __shfl_sync(0xffffffffu, by, k);
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) sum[j] = fmaf(share, p[lane + 32 * j], sum[j]);
+        }
       }
 #pragma unroll
+      for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
       for (int j = 0; j < kEach; ++j) part[warp][lane + 32 * j] = sum[j];
-      if (lane == 0) sums[warp] = l;
+      if (lane == 0) sums[warp] = make_float2(ref, l);
     }
     __syncthreads();
     if (busy && member == 0) {
-      float o[kEach], l = 0.f;
+      float ref = kNoScore, o[kEach], l = 0.f;
+      for (int m = 0; m < members; ++m) ref = fmaxf(ref, sums[team + m * teams].x);
 #pragma unroll
       for (int j = 0; j < kEach; ++j) o[j] = 0.f;
       for (int m = 0; m < members; ++m) {
-        l += sums[team + m * teams];
+        const float2 ml = sums[team + m * teams];
+        const float by = ex2(ml.x - ref);
+        l += by * ml.y;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) o[j] += part[team + m * teams][lane + 32 * j];
+        for (int j = 0; j < kEach; ++j) o[j] += by * part[team + m * teams][lane + 32 * j];
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       int64_t at_lse;
@@ -986,13 +1001,16 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, kThreads, Sh::kRingBytes, stream, pdl, c, a, rows, row_blocks, option_wait_limit_ns());
   if (e != cudaSuccess) return e;
   *launches += 1;
-  // Few items are cut into many pieces each: then every row gets a large CTA of its own.
+  // Where items are cut into many pieces, every row gets a CTA of its own, with a warp for every eight pieces.
   const int items = c.B * c.H * row_blocks;
-  const bool many_pieces = static_cast<long long>(grid) * kWarps > 8ll * items;
+  const long long pieces = static_cast<long long>(grid) * kWarps / items;
+  const bool many_pieces = pieces > 8;
   const int rows_each = many_pieces ? 1 : 8 * NT;
+  int join_threads = kJoinThreads;
+  while (join_threads < kJoinMost && many_pieces && pieces > join_threads / 4) join_threads *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items), static_cast<unsigned>(many_pieces ? (rows.count < 8 * NT ? rows.count : 8 * NT) : 1));
-  cfg.blockDim = dim3(many_pieces ? kJoinMost : kJoinThreads);
+  cfg.blockDim = dim3(join_threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

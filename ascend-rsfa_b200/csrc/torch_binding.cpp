@@ -1,4 +1,4 @@
-// The ordinary attention() call from PyTorch in native code: check the tensors, allocate the result, find the
+// The ordinary calls of attention() and of the operators around it from PyTorch in native code.  attention(): check the tensors, allocate the result, find the
 // current stream, call rsfa_fwd.  The same steps in Python (flash_attention_forward.py, _forward) take 10 us of
 // the host's time per call, three times what the launch itself takes, which is what a call of a few heads or
 // of a short sequence costs its caller; here they take about 1.5 us.
@@ -9,8 +9,11 @@
 // So nothing is accepted, refused or seen by a mode differently than without this file.
 #include <Python.h>
 
+#include <cstring>
+
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -132,6 +135,332 @@ PyObject* forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- the operators around attention
+// The same bargain: None for whatever is not the ordinary call, and rotary.py and kv_cache.py decide.
+struct Ops {
+  decltype(&rsfa_rotary) rotary = nullptr;
+  decltype(&rsfa_cache4_append) append = nullptr;
+  decltype(&rsfa_cache4_read) read = nullptr;
+  decltype(&rsfa_cache4_attention_workspace) attention_workspace = nullptr;
+  decltype(&rsfa_cache4_attention) attention = nullptr;
+  decltype(&rsfa_cache4_evict_workspace) evict_workspace = nullptr;
+  decltype(&rsfa_cache4_evict) evict = nullptr;
+} g_ops;
+
+// The current device, if the tensor lives on it; -1: it does not (there may be no device at all).
+int device_of(PyObject* obj) {
+  if (!THPVariable_CheckExact(obj)) return -1;
+  const at::Tensor& t = THPVariable_Unpack(obj);
+  if (!t.defined() || !t.is_cuda()) return -1;
+  const int device = c10::cuda::current_device();
+  return t.device().index() == device ? device : -1;
+}
+// A plain CUDA tensor of `type` with `dims` dimensions on the current device; null: something else.
+const at::Tensor* plain_cuda(PyObject* obj, at::ScalarType type, int64_t dims, int device) {
+  if (!THPVariable_CheckExact(obj)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(obj);
+  const c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                     c10::DispatchKey::Batched, c10::DispatchKey::Functionalize, c10::DispatchKey::Negative,
+                                     c10::DispatchKey::Conjugate, c10::DispatchKey::ZeroTensor, c10::DispatchKey::Python});
+  if (!t.defined() || t.key_set().has_any(wrapped) || t.layout() != c10::kStrided || !t.is_cuda() || t.dim() != dims ||
+      !t.has_storage() || t.scalar_type() != type || t.device().index() != device)
+    return nullptr;
+  return &t;
+}
+// The same for [B, H, S, D] rows that the library reads as they are (plain_tensor) and that are not empty.
+const at::Tensor* plain_rows(PyObject* obj, int device) {
+  if (!plain_tensor(obj)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(obj);
+  if (t.device().index() != device || t.numel() == 0 || t.size(0) > INT32_MAX || t.size(1) > INT32_MAX || t.size(2) > INT32_MAX) return nullptr;
+  return &t;
+}
+bool records_grad(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// An output like t whose rows the library can write.
+at::Tensor rows_like(const at::Tensor& t) {
+  at::Tensor o = at::empty_like(t);
+  bool fits = o.stride(3) == 1;
+  for (int i = 0; i < 3; ++i) fits = fits && (o.size(i) == 1 || o.stride(i) % 8 == 0);
+  return fits ? o : at::empty(t.sizes(), t.options());
+}
+void copy_strides(int64_t* to, const at::Tensor& t) {
+  for (int i = 0; i < 4; ++i) to[i] = t.stride(i);
+}
+int dtype_of(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? RSFA_DTYPE_BF16 : RSFA_DTYPE_F16; }
+// (a, b or None) of two new tensors.
+PyObject* tensor_pair(at::Tensor a, at::Tensor b) {
+  PyObject* pa = THPVariable_Wrap(std::move(a));
+  if (pa == nullptr) return nullptr;
+  PyObject* pb = Py_None;
+  if (b.defined())
+    pb = THPVariable_Wrap(std::move(b));
+  else
+    Py_INCREF(pb);
+  PyObject* pair = pb == nullptr ? nullptr : PyTuple_New(2);
+  if (pair == nullptr) {
+    Py_DECREF(pa);
+    Py_XDECREF(pb);
+    return nullptr;
+  }
+  PyTuple_SET_ITEM(pair, 0, pa);
+  PyTuple_SET_ITEM(pair, 1, pb);
+  return pair;
+}
+
+// rotary(q, k or None, table, positions or None, interleaved, inverse) -> (q', k' or None), an error code, or None.
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (g_ops.rotary == nullptr || n != 6 || !plain_mode() || !PyBool_Check(args[4]) || !PyBool_Check(args[5])) Py_RETURN_NONE;
+  const int device = device_of(args[0]);
+  if (device < 0) Py_RETURN_NONE;
+  const at::Tensor* q = plain_rows(args[0], device);
+  const at::Tensor* k = args[1] == Py_None ? nullptr : plain_rows(args[1], device);
+  const at::Tensor* table = plain_cuda(args[2], at::kFloat, 3, device);
+  if (q == nullptr || (k == nullptr && args[1] != Py_None) || table == nullptr || records_grad(*q) || (k != nullptr && records_grad(*k)))
+    Py_RETURN_NONE;
+  const int64_t B = q->size(0), S = q->size(2), D = q->size(3), R = 2 * table->size(1);
+  if (!(D == 16 || D == 32 || D == 64 || D == 128 || D == 256) || R > D || R < 2 || table->size(2) != 2 || !table->is_contiguous() ||
+      table->size(0) < 1 || table->size(0) > INT32_MAX || table->requires_grad())
+    Py_RETURN_NONE;
+  if (k != nullptr && (k->size(0) != B || k->size(2) != S || k->size(3) != D || k->scalar_type() != q->scalar_type())) Py_RETURN_NONE;
+  const at::Tensor* pos = nullptr;
+  int64_t pos_strides[2] = {0, 0};
+  if (args[3] != Py_None) {
+    if (!THPVariable_CheckExact(args[3])) Py_RETURN_NONE;
+    const at::Tensor& p = THPVariable_Unpack(args[3]);
+    if (!p.defined() || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong)) Py_RETURN_NONE;
+    pos = plain_cuda(args[3], p.scalar_type(), p.dim(), device);
+    if (pos == nullptr || (p.dim() != 1 && p.dim() != 2) || p.size(-1) != S || (p.dim() == 2 && p.size(0) != 1 && p.size(0) != B)) Py_RETURN_NONE;
+    pos_strides[0] = p.dim() == 1 || p.size(0) == 1 ? 0 : p.stride(0);
+    pos_strides[1] = p.stride(-1);
+  }
+  at::Tensor qo = rows_like(*q), ko;
+  if (k != nullptr) ko = rows_like(*k);
+  int64_t strides[16] = {};
+  copy_strides(strides, *q);
+  copy_strides(strides + 8, qo);
+  if (k != nullptr) {
+    copy_strides(strides + 4, *k);
+    copy_strides(strides + 12, ko);
+  }
+  const void* kp = k != nullptr ? k->const_data_ptr() : nullptr;
+  void* kop = k != nullptr ? ko.mutable_data_ptr() : nullptr;
+  const int Hk = k != nullptr ? static_cast<int>(k->size(1)) : 0;
+  void* stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_ops.rotary(q->const_data_ptr(), kp, qo.mutable_data_ptr(), kop, static_cast<int>(B), static_cast<int>(q->size(1)), Hk,
+                    static_cast<int>(S), static_cast<int>(D), strides, static_cast<const float*>(table->const_data_ptr()),
+                    static_cast<int>(table->size(0)), static_cast<int>(R), pos != nullptr ? pos->const_data_ptr() : nullptr,
+                    pos != nullptr && pos->scalar_type() == at::kLong ? 1 : 0, pos != nullptr ? pos_strides : nullptr, args[4] == Py_True,
+                    args[5] == Py_True, dtype_of(*q), stream);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return PyLong_FromLong(rc);
+  return tensor_pair(std::move(qo), std::move(ko));
+  END_HANDLE_TH_ERRORS
+}
+
+// int32 [n] or None; false: something else.
+bool plain_ints(PyObject* obj, int64_t n, int device, const int** out) {
+  *out = nullptr;
+  if (obj == Py_None) return true;
+  const at::Tensor* t = plain_cuda(obj, at::kInt, 1, device);
+  if (t == nullptr || t->size(0) != n || (n > 1 && t->stride(0) != 1)) return false;
+  *out = static_cast<const int*>(t->const_data_ptr());
+  return true;
+}
+
+// The cache of kv, table, lengths, weight or None and position or None; false: something else.
+bool plain_cache(PyObject* kv_obj, PyObject* table_obj, PyObject* lengths_obj, PyObject* weight_obj, PyObject* position_obj, int dtype, int device,
+                 rsfa_cache4* c) {
+  const at::Tensor* kv = plain_cuda(kv_obj, at::kByte, 4, device);
+  const at::Tensor* table = plain_cuda(table_obj, at::kInt, 2, device);
+  if (kv == nullptr || table == nullptr) return false;
+  const int64_t rec = kv->size(3), page = kv->size(2);
+  if (!(rec == 80 || rec == 160 || rec == 320) || kv->size(0) < 1 || kv->size(1) < 1 || kv->stride(3) != 1 || kv->stride(2) != rec ||
+      kv->stride(0) % 16 != 0 || kv->stride(1) % 16 != 0 || (reinterpret_cast<uintptr_t>(kv->const_data_ptr()) & 15u) != 0)
+    return false;
+  if (table->size(0) < 1 || table->size(1) < 1 || table->stride(1) != 1 || kv->size(0) > INT32_MAX || kv->size(1) > INT32_MAX || page > 1024 ||
+      table->size(0) > INT32_MAX || table->size(1) > INT32_MAX)
+    return false;
+  std::memset(c, 0, sizeof(*c));
+  if (lengths_obj == Py_None || !plain_ints(lengths_obj, table->size(0), device, &c->lengths)) return false;
+  PyObject* extra[2] = {weight_obj, position_obj};
+  for (int i = 0; i < 2; ++i) {
+    if (extra[i] == Py_None) continue;
+    const at::Tensor* t = plain_cuda(extra[i], i == 0 ? at::kFloat : at::kInt, 3, device);
+    if (t == nullptr || t->size(0) != kv->size(0) || t->size(1) != kv->size(1) || t->size(2) != page || t->stride(2) != 1) return false;
+    int64_t* st = i == 0 ? c->weight_stride : c->position_stride;
+    st[0] = t->stride(0);
+    st[1] = t->stride(1);
+    if (i == 0)
+      c->weight = static_cast<float*>(t->mutable_data_ptr());
+    else
+      c->position = static_cast<int*>(t->mutable_data_ptr());
+  }
+  c->kv = kv->mutable_data_ptr();
+  c->kv_stride[0] = kv->stride(0);
+  c->kv_stride[1] = kv->stride(1);
+  c->table = static_cast<const int*>(table->const_data_ptr());
+  c->table_stride = table->stride(0);
+  c->batch = static_cast<int>(table->size(0));
+  c->heads = static_cast<int>(kv->size(1));
+  c->head_dim = static_cast<int>(rec / 5 * 4);
+  c->page_size = static_cast<int>(page);
+  c->pages = static_cast<int>(kv->size(0));
+  c->max_pages = static_cast<int>(table->size(1));
+  c->dtype = dtype;
+  return true;
+}
+
+// append(k, v, kv, table, lengths, counts, weight, position, positions) -> True, an error code, or None.
+PyObject* cache4_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (g_ops.append == nullptr || n != 9 || !plain_mode()) Py_RETURN_NONE;
+  const int device = device_of(args[0]);
+  if (device < 0) Py_RETURN_NONE;
+  const at::Tensor* k = plain_rows(args[0], device);
+  const at::Tensor* v = plain_rows(args[1], device);
+  rsfa_cache4 c;
+  if (k == nullptr || v == nullptr || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() ||
+      !plain_cache(args[2], args[3], args[4], args[6], args[7], dtype_of(*k), device, &c))
+    Py_RETURN_NONE;
+  const int64_t S = k->size(2);
+  const int* counts = nullptr;
+  if (k->size(0) != c.batch || k->size(1) != c.heads || k->size(3) != c.head_dim || !plain_ints(args[5], c.batch, device, &counts) ||
+      (args[7] == Py_None) != (args[8] == Py_None))
+    Py_RETURN_NONE;
+  int64_t pos_strides[2] = {0, 0};
+  const int* positions = nullptr;
+  if (args[8] != Py_None) {
+    const at::Tensor* p = plain_cuda(args[8], at::kInt, 2, device);
+    if (p == nullptr || p->size(0) != c.batch || p->size(1) != S) Py_RETURN_NONE;
+    pos_strides[0] = p->stride(0);
+    pos_strides[1] = p->stride(1);
+    positions = static_cast<const int*>(p->const_data_ptr());
+  }
+  int64_t strides[8];
+  copy_strides(strides, *k);
+  copy_strides(strides + 4, *v);
+  void* stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_ops.append(&c, k->const_data_ptr(), v->const_data_ptr(), static_cast<int>(S), strides, counts, positions,
+                    positions != nullptr ? pos_strides : nullptr, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return PyLong_FromLong(rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// read(kv, table, lengths, n, bf16, starts) -> (k, v), an error code, or None.
+PyObject* cache4_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int rows = 0;
+  if (g_ops.read == nullptr || n != 6 || !plain_mode() || !plain_int(args[3], &rows) || rows < 1 || !PyBool_Check(args[4])) Py_RETURN_NONE;
+  const int device = device_of(args[0]);
+  if (device < 0) Py_RETURN_NONE;
+  rsfa_cache4 c;
+  const int* starts = nullptr;
+  if (!plain_cache(args[0], args[1], args[2], Py_None, Py_None, args[4] == Py_True ? RSFA_DTYPE_BF16 : RSFA_DTYPE_F16, device, &c) ||
+      !plain_ints(args[5], c.batch, device, &starts))
+    Py_RETURN_NONE;
+  const at::TensorOptions options = THPVariable_Unpack(args[0]).options().dtype(args[4] == Py_True ? at::kBFloat16 : at::kHalf);
+  at::Tensor k = at::empty({c.batch, c.heads, rows, c.head_dim}, options), v = at::empty({c.batch, c.heads, rows, c.head_dim}, options);
+  int64_t strides[8];
+  copy_strides(strides, k);
+  copy_strides(strides + 4, v);
+  void* stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_ops.read(&c, k.mutable_data_ptr(), v.mutable_data_ptr(), rows, strides, starts, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return PyLong_FromLong(rc);
+  return tensor_pair(std::move(k), std::move(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// attention(q, kv, table, lengths, sm_scale, counts, weight, want_lse) -> (o, lse or None), an error code, or None.
+PyObject* cache4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (g_ops.attention == nullptr || n != 8 || !plain_mode() || !PyFloat_CheckExact(args[4]) || !PyBool_Check(args[7])) Py_RETURN_NONE;
+  const int device = device_of(args[0]);
+  if (device < 0) Py_RETURN_NONE;
+  const at::Tensor* q = plain_rows(args[0], device);
+  rsfa_cache4 c;
+  if (q == nullptr || !plain_cache(args[1], args[2], args[3], args[6], Py_None, dtype_of(*q), device, &c)) Py_RETURN_NONE;
+  const int64_t Hq = q->size(1), S = q->size(2);
+  const int* counts = nullptr;
+  if (q->size(0) != c.batch || q->size(3) != c.head_dim || Hq % c.heads != 0 || !plain_ints(args[5], c.batch, device, &counts)) Py_RETURN_NONE;
+  const long long bytes = g_ops.attention_workspace(&c, static_cast<int>(Hq), static_cast<int>(S));
+  if (bytes < 0) Py_RETURN_NONE;
+  at::Tensor o = rows_like(*q), lse;
+  if (args[7] == Py_True || c.weight != nullptr) lse = at::empty({q->size(0), Hq, S}, q->options().dtype(at::kFloat));
+  // the call's own scratch, from the pool of the current stream or of the graph that is being captured
+  at::Tensor scratch = at::empty({bytes}, q->options().dtype(at::kByte));
+  int64_t strides[8];
+  copy_strides(strides, *q);
+  copy_strides(strides + 4, o);
+  float* lp = lse.defined() ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr;
+  const float scale = static_cast<float>(PyFloat_AS_DOUBLE(args[4]));
+  void* stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_ops.attention(&c, q->const_data_ptr(), o.mutable_data_ptr(), lp, static_cast<int>(Hq), static_cast<int>(S), strides, counts, scale,
+                       scratch.mutable_data_ptr(), bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return PyLong_FromLong(rc);
+  if (args[7] != Py_True) lse.reset();
+  return tensor_pair(std::move(o), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// evict(kv, weight, position, table, lengths, budget, recent) -> new lengths, an error code, or None.
+PyObject* cache4_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int budget = 0, recent = 0;
+  if (g_ops.evict == nullptr || n != 7 || !plain_mode() || !plain_int(args[5], &budget) || !plain_int(args[6], &recent) || budget < 1 ||
+      recent < 0 || recent > budget || args[1] == Py_None || args[2] == Py_None)
+    Py_RETURN_NONE;
+  const int device = device_of(args[0]);
+  if (device < 0) Py_RETURN_NONE;
+  rsfa_cache4 c;
+  if (!plain_cache(args[0], args[3], args[4], args[1], args[2], RSFA_DTYPE_F16, device, &c)) Py_RETURN_NONE;
+  const at::Tensor& lengths = THPVariable_Unpack(args[4]);
+  const long long bytes = g_ops.evict_workspace(c.batch, c.heads, budget);
+  if (bytes < 0) Py_RETURN_NONE;
+  at::Tensor out = at::empty({c.batch}, lengths.options());
+  at::Tensor scratch = at::empty({bytes}, lengths.options().dtype(at::kByte));
+  void* stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_ops.evict(&c, budget, recent, static_cast<int*>(out.mutable_data_ptr()), scratch.mutable_data_ptr(), bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_ops(addresses of the functions of Ops, in its order)
+PyObject* bind_ops(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "bind_ops takes seven addresses");
+    return nullptr;
+  }
+  void* p[7];
+  for (int i = 0; i < 7; ++i) {
+    p[i] = PyLong_AsVoidPtr(args[i]);
+    if (p[i] == nullptr && PyErr_Occurred()) return nullptr;
+  }
+  g_ops.rotary = reinterpret_cast<decltype(g_ops.rotary)>(p[0]);
+  g_ops.append = reinterpret_cast<decltype(g_ops.append)>(p[1]);
+  g_ops.read = reinterpret_cast<decltype(g_ops.read)>(p[2]);
+  g_ops.attention_workspace = reinterpret_cast<decltype(g_ops.attention_workspace)>(p[3]);
+  g_ops.attention = reinterpret_cast<decltype(g_ops.attention)>(p[4]);
+  g_ops.evict_workspace = reinterpret_cast<decltype(g_ops.evict_workspace)>(p[5]);
+  g_ops.evict = reinterpret_cast<decltype(g_ops.evict)>(p[6]);
+  Py_RETURN_NONE;
+}
+
 // bind(address of rsfa_fwd)
 PyObject* bind(PyObject*, PyObject* arg) {
   void* p = PyLong_AsVoidPtr(arg);
@@ -143,6 +472,12 @@ PyObject* bind(PyObject*, PyObject* arg) {
 PyMethodDef methods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(forward)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_O, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rotary)), METH_FASTCALL, nullptr},
+    {"cache4_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(cache4_append)), METH_FASTCALL, nullptr},
+    {"cache4_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(cache4_read)), METH_FASTCALL, nullptr},
+    {"cache4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(cache4_attention)), METH_FASTCALL, nullptr},
+    {"cache4_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(cache4_evict)), METH_FASTCALL, nullptr},
+    {"bind_ops", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind_ops)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rsfa_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -539,3 +539,47 @@ def test_refusals_on_the_device(cuda_device):
     assert kc.cache4_attention(q[:, :, :0], kv, table, n, 0.1).shape == (2, 4, 0, 64)
     assert kc.cache4_read(kv, table, n, 0, dtype)[0].shape == (2, 2, 0, 64)
     kc.cache4_append(k[:, :, :0], k[:, :, :0], kv, table, n)
+
+
+# ------------------------------------------------------------------ the native form of the calls
+
+@pytest.mark.gpu
+def test_native_and_python_routes_agree(cuda_device, monkeypatch):
+    """Ordinary calls are answered by the native code, others are not, and both give the same bits."""
+    dtype, H, D, page = torch.bfloat16, 2, 64, 16
+    native = ro._native
+    q, k = rows(cuda_device, (2, 4, 3, D), dtype, 1), rows(cuda_device, (2, 3, H, D), dtype, 2).transpose(1, 2)
+    rope = ro.rotary_table(64, D, device=cuda_device)
+    pos = torch.randint(0, 64, (2, 3), device=cuda_device, dtype=torch.int32)
+    counts, starts = (torch.tensor(x, dtype=torch.int32, device=cuda_device) for x in ([3, 2], [1, 0]))
+
+    def everything():
+        kv, table, n = make(cuda_device, [40, 20], H, D, page, dtype, room=60)
+        weight, position = torch.zeros(kv.shape[:3], device=cuda_device), torch.zeros(kv.shape[:3], dtype=torch.int32, device=cuda_device)
+        out = [*ro.rotary(q, k, rope, pos), *ro.rotary(q, k, rope, pos.long(), True), ro.rotary(q, None, rope)[0]]
+        kc.cache4_append(k, k, kv, table, n, counts=counts, weight=weight, position=position, positions=pos)
+        out += [*kc.cache4_read(kv, table, n, 7, dtype, starts=starts), *kc.cache4_attention(q, kv, table, n, 0.1, counts=counts, weight=weight, want_lse=True),
+                kc.cache4_attention(q, kv, table, n, 0.1)]
+        out += [kc.cache4_evict(kv, weight, position, table, n, 24, 5), *kc.cache4_read(kv, table, torch.clamp(n, max=24), 24, dtype), weight, position]
+        return out
+
+    seen = []
+    for name in ("rotary", "cache4_append", "cache4_read", "cache4_attention", "cache4_evict"):
+        fn = getattr(native, name)
+        monkeypatch.setattr(native, name, lambda *a, fn=fn, name=name: seen.append((name, fn(*a))) or seen[-1][1])
+    first = everything()
+    assert len(seen) == 9 and all(r is not None for _, r in seen)
+    monkeypatch.undo()
+    monkeypatch.setattr(ro, "_native", None)
+    for a, b in zip(first, everything()):
+        assert torch.equal(a, b) and a.dtype == b.dtype and a.stride() == b.stride()
+    # what is not ordinary
+    kv, table, n = make(cuda_device, [40, 20], H, D, page, dtype, room=60)
+    assert native.rotary(q.clone().requires_grad_(), k, rope, pos, False, False) is None
+    assert native.rotary(q, k, rope.double(), pos, False, False) is None and native.rotary(q, k, rope, pos[:, :2], False, False) is None
+    assert native.rotary(q[..., ::2], None, rope, None, False, False) is None and native.rotary(q, k.half(), rope, pos, False, False) is None
+    assert native.cache4_attention(q, kv, table, n, 1, None, None, False) is None and native.cache4_attention(q, kv, table, n[:1], 0.1, None, None, False) is None
+    assert native.cache4_attention(q[:, :3], kv, table, n, 0.1, None, None, False) is None and native.cache4_attention(q, kv[..., :64], table, n, 0.1, None, None, False) is None
+    assert native.cache4_append(k, k, kv, table, n, None, None, None, pos) is None and native.cache4_append(q, q, kv, table, n, None, None, None, None) is None
+    assert native.cache4_read(kv, table, n, 0, True, None) is None and native.cache4_read(kv, table.long(), n, 4, True, None) is None
+    assert native.cache4_evict(kv, None, None, table, n, 4, 2) is None
