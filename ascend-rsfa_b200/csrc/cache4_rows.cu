@@ -14,15 +14,42 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// Packed minimum and maximum of 16-bit numbers; NaN wins.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (kBf16)
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+template <bool kBf16>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (kBf16)
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
+}
+template <bool kBf16>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  if constexpr (kBf16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// Codes 2 j and 2 j + 1 of a word as a pair of 16-bit numbers: put where the mantissa of 1024 (fp16) or 128 (bf16) ends,
+// which then comes off exactly.  (An integer conversion per code is four times as slow as all the rest.)
+template <bool kBf16>
+__device__ __forceinline__ uint32_t code_pair(uint32_t codes, int j) {
+  const uint32_t both = __byte_perm(codes, 0u, 0x4040 + 0x0101 * j);   // byte j in either half
+  if constexpr (kBf16) return fma2<true>((both & 0x0000000fu) | ((both >> 4) & 0x000f0000u) | 0x43004300u, 0x3f803f80u, 0xc300c300u);
+  // the second code stands four bits higher: 1024 + 16 u
+  return fma2<false>((both & 0x00f0000fu) | 0x64006400u, 0x2c003c00u, 0xd400e400u);
 }
 
 // A CTA has kTokens tokens of one head, two rows of D / 8 lanes each, and a thread the same lane of several of them,
@@ -91,25 +118,17 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
     for (int i = 0; i < kAtOnce; ++i) {
       const int s = k.first + t0 + i * k.step + k.sub;
       const uint32_t words[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = to_f32x2<kBf16>(words[j]);
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
-      }
-      float lo = x[0], hi = x[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) {
-        lo = min_nan(lo, x[j]);
-        hi = max_nan(hi, x[j]);
-      }
+      uint32_t lo2 = min2<kBf16>(min2<kBf16>(words[0], words[1]), min2<kBf16>(words[2], words[3]));
+      uint32_t hi2 = max2<kBf16>(max2<kBf16>(words[0], words[1]), max2<kBf16>(words[2], words[3]));
+      // the smaller of each half in the low half, the larger in the high one
+      uint32_t ends = __byte_perm(min2<kBf16>(lo2, lo2 >> 16), max2<kBf16>(hi2, hi2 >> 16), 0x5410);
 #pragma unroll
       for (int m = 1; m <= 2; m <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, ends, m);
+        ends = __byte_perm(min2<kBf16>(ends, other), max2<kBf16>(ends, other), 0x7610);
       }
-      const float range = hi - lo;
+      const float2 range2 = to_f32x2<kBf16>(ends);
+      const float lo = range2.x, range = range2.y - range2.x;
       const bool finite = range < INFINITY;                       // false for NaN as well
       // The scale is stored in the rows' own type: 11 (8) bits of it are enough for codes of 4 bits, whose
       // rounding is half a scale; the code is chosen for the scale as stored.
@@ -119,18 +138,22 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
         scale = 0.f;
         s16 = 0;
       }
-      const float inv = scale > 0.f ? __fdiv_rn(1.0f, scale) : 0.f;
+      const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;
+      // (x - lo) / scale is rounded to an integer by the sum with 1.5 * 2^23, whose low bits it then is; those of the
+      // eight sums, each four bits further up, make the word, and what 1.5 * 2^23 adds to it is one constant.
       uint32_t codes = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float u = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[j], lo), inv)), 0.f), 15.f);   // NaN: 0
-        codes |= static_cast<uint32_t>(u) << (4 * j);
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = to_f32x2<kBf16>(words[j]);
+        const float a = fminf(__fmul_rn(__fsub_rn(x.x, lo), inv), 15.f), b = fminf(__fmul_rn(__fsub_rn(x.y, lo), inv), 15.f);
+        codes += (__float_as_uint(__fadd_rn(a, 12582912.f)) << (8 * j)) + (__float_as_uint(__fadd_rn(b, 12582912.f)) << (8 * j + 4));
       }
+      codes -= 0x4b400000u * 0x11111111u;
       if (!finite) codes = 0;
       const uint32_t turned = exchange_halves<D>(codes, w);
       if (!live[i]) continue;
       const uint32_t nan16 = kBf16 ? 0x7fc0u : 0x7e00u;
-      const uint32_t pair = finite ? (s16 | (static_cast<uint32_t>(from_f32<kBf16>(lo)) << 16)) : (nan16 | (nan16 << 16));
+      const uint32_t pair = finite ? (s16 | (ends << 16)) : (nan16 | (nan16 << 16));
       const int off = (slot0 + s) & ((1 << c.page_shift) - 1);
       uint8_t* rec = c.kv + page[i] * c.kv_stride[0] + k.h * c.kv_stride[1] + static_cast<int64_t>(off) * R::kBytes;
       *reinterpret_cast<uint32_t*>(rec + code_word<D>(k.kv, w, q)) = k.kv ? turned : codes;
@@ -177,12 +200,11 @@ __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const Cache4 c, c
       const int t = t0 + i * k.step + k.sub;
       const uint32_t turned = exchange_halves<D>(codes[i], w);
       const uint32_t u = k.kv ? turned : codes[i];
-      const float2 sm = to_f32x2<kBf16>(pair[i]);
+      // one rounding, to the rows' type
+      const uint32_t scales = __byte_perm(pair[i], pair[i], 0x1010), minima = __byte_perm(pair[i], pair[i], 0x3232);
       uint32_t words[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        words[j] = from_f32x2<kBf16>(fmaf(static_cast<float>((u >> (8 * j)) & 15u), sm.x, sm.y),
-                                     fmaf(static_cast<float>((u >> (8 * j + 4)) & 15u), sm.x, sm.y));
+      for (int j = 0; j < 4; ++j) words[j] = fma2<kBf16>(code_pair<kBf16>(u, j), scales, minima);
       if (t < k.tokens) *reinterpret_cast<uint4*>(dst + (k.first + t) * st[2]) = make_uint4(words[0], words[1], words[2], words[3]);
     }
   }
