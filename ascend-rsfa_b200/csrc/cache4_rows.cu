@@ -65,17 +65,35 @@ template <int D>
 __device__ __forceinline__ Chunk chunk_of(const Cache4& c, int S) {
   constexpr int kLanes = D / 8;
   const int chunks = (S + kTokens - 1) / kTokens;
-  const int bh = blockIdx.x / chunks;
   Chunk k;
-  k.first = (blockIdx.x - bh * chunks) * kTokens;
+  // heads first: in a [B, S, H, D] projection their rows of a token lie side by side
+  const int bc = blockIdx.x / c.H;
+  k.h = blockIdx.x - bc * c.H;
+  k.b = bc / chunks;
+  k.first = (bc - k.b * chunks) * kTokens;
   k.tokens = min(kTokens, S - k.first);
-  k.b = bh / c.H;
-  k.h = bh - k.b * c.H;
   k.lane = threadIdx.x % kLanes;
   k.kv = (threadIdx.x / kLanes) & 1;
   k.sub = threadIdx.x / (2 * kLanes);
   k.step = blockDim.x / (2 * kLanes);
   return k;
+}
+
+// The pages that slots first .. first + kTokens - 1 of a sequence lie in, looked up once for all rows of the CTA.
+constexpr int kChunkPages = kTokens / 16 + 1;
+struct ChunkPages {
+  int64_t page[kChunkPages];       // -1: none
+  uint8_t* records[kChunkPages];   // of the CTA's head
+};
+__device__ __forceinline__ void find_pages(ChunkPages& at, const Cache4& c, const Chunk& k, int first, int end) {
+  if (threadIdx.x < kChunkPages) {
+    const int slot = ((first >> c.page_shift) + static_cast<int>(threadIdx.x)) << c.page_shift;   // the first of the page
+    int64_t page = -1;
+    if (slot >= end || !find_page(c, k.b, slot, &page)) page = -1;
+    at.page[threadIdx.x] = page;
+    at.records[threadIdx.x] = c.kv + (page < 0 ? 0 : page) * c.kv_stride[0] + k.h * c.kv_stride[1];
+  }
+  __syncthreads();
 }
 
 // The V codes of a lane, eight dims of group w, to and from memory order: even groups store the low halves of two
@@ -100,23 +118,31 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
   const Chunk k = chunk_of<D>(c, rows.S);
   // rows behind the count are padding; a slot below zero is no token (a sequence that is not in use)
   const int count = rows.counts != nullptr ? min(max(rows.counts[k.b], 0), rows.S) : rows.S;
-  const int slot0 = tokens_of(c, k.b) - count;
+  const int slot0 = tokens_of(c, k.b) - count + k.first;       // of the CTA's first token
+  const int from = max(0, -slot0), to = min(k.tokens, count - k.first);
+  if (from >= to) return;
+  __shared__ ChunkPages at;
+  const int page0 = (slot0 + from) >> c.page_shift;
+  find_pages(at, c, k, slot0 + from, slot0 + to);
   const int64_t* st = k.kv ? rows.v_stride : rows.k_stride;
-  const uint16_t* src = static_cast<const uint16_t*>(k.kv ? rows.v : rows.k) + k.b * st[0] + k.h * st[1] + 8 * k.lane;
+  const int64_t step_bytes = st[2] * 2 * k.step;
+  const uint8_t* src = static_cast<const uint8_t*>(k.kv ? rows.v : rows.k) + 2 * (k.b * st[0] + k.h * st[1] + 8 * k.lane + (k.first + k.sub) * st[2]);
   const int w = k.lane >> 2, q = k.lane & 3;
-  for (int t0 = 0; t0 < k.tokens; t0 += kAtOnce * k.step) {
+  const int at_codes = code_word<D>(k.kv, w, q), at_pair = (k.kv ? R::kVPairs : R::kKPairs) + 4 * w;
+  const int mask = (1 << c.page_shift) - 1;
+  for (int t0 = 0; t0 < to; t0 += kAtOnce * k.step) {
     uint4 in[kAtOnce];
-    int64_t page[kAtOnce];
     bool live[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int t = t0 + i * k.step + k.sub, s = k.first + t;
-      live[i] = t < k.tokens && s < count && slot0 + s >= 0 && find_page(c, k.b, slot0 + s, &page[i]);
-      in[i] = live[i] ? __ldg(reinterpret_cast<const uint4*>(src + s * st[2])) : make_uint4(0, 0, 0, 0);
+      const int t = t0 + i * k.step + k.sub;
+      live[i] = t >= from && t < to && at.page[((slot0 + t) >> c.page_shift) - page0] >= 0;
+      in[i] = live[i] ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+      src += step_bytes;
     }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int s = k.first + t0 + i * k.step + k.sub;
+      const int slot = slot0 + t0 + i * k.step + k.sub;
       const uint32_t words[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
       uint32_t lo2 = min2<kBf16>(min2<kBf16>(words[0], words[1]), min2<kBf16>(words[2], words[3]));
       uint32_t hi2 = max2<kBf16>(max2<kBf16>(words[0], words[1]), max2<kBf16>(words[2], words[3]));
@@ -154,17 +180,21 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
       if (!live[i]) continue;
       const uint32_t nan16 = kBf16 ? 0x7fc0u : 0x7e00u;
       const uint32_t pair = finite ? (s16 | (ends << 16)) : (nan16 | (nan16 << 16));
-      const int off = (slot0 + s) & ((1 << c.page_shift) - 1);
-      uint8_t* rec = c.kv + page[i] * c.kv_stride[0] + k.h * c.kv_stride[1] + static_cast<int64_t>(off) * R::kBytes;
-      *reinterpret_cast<uint32_t*>(rec + code_word<D>(k.kv, w, q)) = k.kv ? turned : codes;
-      if (q == 0) *reinterpret_cast<uint32_t*>(rec + (k.kv ? R::kVPairs : R::kKPairs) + 4 * w) = pair;
-      if (k.lane == 0 && k.kv == 0) {
-        if (c.weight != nullptr) c.weight[page[i] * c.weight_stride[0] + k.h * c.weight_stride[1] + off] = 0.f;
-        if (c.position != nullptr && rows.positions != nullptr)
-          c.position[page[i] * c.position_stride[0] + k.h * c.position_stride[1] + off] =
-              rows.positions[k.b * rows.positions_stride[0] + s * rows.positions_stride[1]];
-      }
+      const int off = slot & mask, which = (slot >> c.page_shift) - page0;
+      uint8_t* rec = at.records[which] + off * R::kBytes;
+      *reinterpret_cast<uint32_t*>(rec + at_codes) = k.kv ? turned : codes;
+      if (q == 0) *reinterpret_cast<uint32_t*>(rec + at_pair) = pair;
     }
+  }
+  // what else there is of the tokens, one per thread
+  for (int t = from + threadIdx.x; t < to; t += blockDim.x) {
+    const int slot = slot0 + t;
+    const int64_t page = at.page[(slot >> c.page_shift) - page0];
+    if (page < 0) continue;
+    if (c.weight != nullptr) c.weight[page * c.weight_stride[0] + k.h * c.weight_stride[1] + (slot & mask)] = 0.f;
+    if (c.position != nullptr && rows.positions != nullptr)
+      c.position[page * c.position_stride[0] + k.h * c.position_stride[1] + (slot & mask)] =
+          rows.positions[k.b * rows.positions_stride[0] + (k.first + t) * rows.positions_stride[1]];
   }
 }
 
@@ -174,25 +204,33 @@ __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const Cache4 c, c
   griddep_launch_dependents();
   griddep_wait();
   const Chunk k = chunk_of<D>(c, rows.S);
-  const long long start = rows.starts != nullptr ? rows.starts[k.b] : 0;
+  // slots of the CTA's tokens: `from` to `to` are in use, the others read as zeros
+  const long long slot0 = static_cast<long long>(rows.starts != nullptr ? rows.starts[k.b] : 0) + k.first;
   const int n = tokens_of(c, k.b);
+  const int from = static_cast<int>(min(static_cast<long long>(k.tokens), max(0ll, -slot0)));
+  const int to = static_cast<int>(max(static_cast<long long>(from), min(static_cast<long long>(k.tokens), n - slot0)));
+  __shared__ ChunkPages at;
+  const int first = from < to ? static_cast<int>(slot0 + from) : 0, page0 = first >> c.page_shift;
+  find_pages(at, c, k, first, first + to - from);
   const int64_t* st = k.kv ? rows.v_stride : rows.k_stride;
-  uint16_t* dst = static_cast<uint16_t*>(k.kv ? rows.v : rows.k) + k.b * st[0] + k.h * st[1] + 8 * k.lane;
+  const int64_t step_bytes = st[2] * 2 * k.step;
+  uint8_t* dst = static_cast<uint8_t*>(k.kv ? rows.v : rows.k) + 2 * (k.b * st[0] + k.h * st[1] + 8 * k.lane + (k.first + k.sub) * st[2]);
   const int w = k.lane >> 2, q = k.lane & 3;
   const int at_codes = code_word<D>(k.kv, w, q), at_pair = (k.kv ? R::kVPairs : R::kKPairs) + 4 * w;
+  const int mask = (1 << c.page_shift) - 1;
   for (int t0 = 0; t0 < k.tokens; t0 += kAtOnce * k.step) {
     uint32_t codes[kAtOnce], pair[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const int t = t0 + i * k.step + k.sub;
-      const long long slot = start + k.first + t;
-      int64_t page;
       codes[i] = pair[i] = 0;
-      if (t < k.tokens && slot >= 0 && slot < n && find_page(c, k.b, static_cast<int>(slot), &page)) {
-        const uint8_t* rec = c.kv + page * c.kv_stride[0] + k.h * c.kv_stride[1] +
-                             (slot & ((1 << c.page_shift) - 1)) * static_cast<int64_t>(R::kBytes);
-        codes[i] = *reinterpret_cast<const uint32_t*>(rec + at_codes);
-        pair[i] = *reinterpret_cast<const uint32_t*>(rec + at_pair);
+      if (t >= from && t < to) {
+        const int slot = first + t - from, which = (slot >> c.page_shift) - page0;
+        if (at.page[which] >= 0) {
+          const uint8_t* rec = at.records[which] + (slot & mask) * R::kBytes;
+          codes[i] = *reinterpret_cast<const uint32_t*>(rec + at_codes);
+          pair[i] = *reinterpret_cast<const uint32_t*>(rec + at_pair);
+        }
       }
     }
 #pragma unroll
@@ -205,7 +243,8 @@ __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const Cache4 c, c
       uint32_t words[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) words[j] = fma2<kBf16>(code_pair<kBf16>(u, j), scales, minima);
-      if (t < k.tokens) *reinterpret_cast<uint4*>(dst + (k.first + t) * st[2]) = make_uint4(words[0], words[1], words[2], words[3]);
+      if (t < k.tokens) *reinterpret_cast<uint4*>(dst) = make_uint4(words[0], words[1], words[2], words[3]);
+      dst += step_bytes;
     }
   }
 }
