@@ -19,7 +19,10 @@ namespace {
 constexpr int kSelectThreads = 1024;
 constexpr int kSlotsEach = 4;              // neighbouring slots of a thread in the listing pass
 constexpr int kBins = 2048;
-constexpr int kKeysInShared = 40 * 1024;   // keys kept in shared memory; longer sequences read them again
+constexpr int kKeysInShared = 20 * 1024;   // slots whose keys and positions are kept in shared memory; of longer sequences
+                                           // the others are read again in every pass
+constexpr int kPagesInShared = 2048;       // and page numbers
+constexpr int kSelectBytes = kKeysInShared * 8 + kPagesInShared * 4;
 constexpr int kMoveThreads = 256;
 constexpr uint32_t kProtected = 0xffffffffu;
 
@@ -50,7 +53,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
 }
 
 __global__ void __launch_bounds__(kSelectThreads) cache4_select_kernel(const Cache4 c, const Cache4Evict e) {
-  extern __shared__ uint32_t keys[];            // min(n, kKeysInShared)
+  extern __shared__ uint32_t kept_slots[];      // keys, then positions of the first `in_shared` slots, then page numbers
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t warp_sums[32];
   __shared__ int newest_word;
@@ -68,29 +71,53 @@ __global__ void __launch_bounds__(kSelectThreads) cache4_select_kernel(const Cac
     return;
   }
   const int mask = (1 << c.page_shift) - 1;
-  auto position_of = [&](int slot) {
-    int64_t page;
-    if (!find_page(c, b, slot, &page)) return INT_MIN;
-    return c.position[page * c.position_stride[0] + h * c.position_stride[1] + (slot & mask)];
-  };
+  const int in_shared = min(n, kKeysInShared), pages_in_shared = min((n + mask) >> c.page_shift, kPagesInShared);
+  uint32_t* const keys = kept_slots;
+  int* const positions = reinterpret_cast<int*>(kept_slots + in_shared);
+  int* const page_ids = positions + in_shared;
   if (tid == 0) newest_word = INT_MIN;
+  for (int i = tid; i < pages_in_shared; i += kSelectThreads) {
+    int64_t page;
+    page_ids[i] = find_page(c, b, i << c.page_shift, &page) ? static_cast<int>(page) : -1;
+  }
   __syncthreads();
+  auto page_of = [&](int slot) -> int64_t {
+    if ((slot >> c.page_shift) < pages_in_shared) return page_ids[slot >> c.page_shift];
+    int64_t page;
+    return find_page(c, b, slot, &page) ? page : -1;
+  };
+  // position and weight of a slot; one whose page is not there is the oldest and lightest
+  auto read_slot = [&](int slot, int* position, float* weight) {
+    const int64_t page = page_of(slot);
+    *position = page < 0 ? INT_MIN : c.position[page * c.position_stride[0] + h * c.position_stride[1] + (slot & mask)];
+    *weight = page < 0 ? 0.f : c.weight[page * c.weight_stride[0] + h * c.weight_stride[1] + (slot & mask)];
+  };
+  auto weight_key = [](float w) { return w > 0.f ? __float_as_uint(w) : 0u; };   // NaN, negative: as no weight
   int newest = INT_MIN;
-  for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, position_of(i));
+#pragma unroll 4
+  for (int i = tid; i < n; i += kSelectThreads) {
+    int position;
+    float weight;
+    read_slot(i, &position, &weight);
+    newest = max(newest, position);
+    if (i < in_shared) {
+      keys[i] = weight_key(weight);
+      positions[i] = position;
+    }
+  }
   newest = __reduce_max_sync(0xffffffffu, newest);
   if ((tid & 31) == 0) atomicMax(&newest_word, newest);
   __syncthreads();
   const long long oldest_kept = static_cast<long long>(newest_word) - e.recent;
-  auto key_of = [&](int slot) -> uint32_t {
-    int64_t page;
-    if (!find_page(c, b, slot, &page)) return 0u;
-    const int pos = c.position[page * c.position_stride[0] + h * c.position_stride[1] + (slot & mask)];
-    const float w = c.weight[page * c.weight_stride[0] + h * c.weight_stride[1] + (slot & mask)];
-    if (static_cast<long long>(pos) > oldest_kept) return kProtected;
-    return w > 0.f ? __float_as_uint(w) : 0u;   // NaN, negative: as no weight
+  for (int i = tid; i < in_shared; i += kSelectThreads)            // each thread's own slots
+    if (static_cast<long long>(positions[i]) > oldest_kept) keys[i] = kProtected;
+  auto key_at = [&](int slot) -> uint32_t {
+    if (slot < in_shared) return keys[slot];
+    int position;
+    float weight;
+    read_slot(slot, &position, &weight);
+    return static_cast<long long>(position) > oldest_kept ? kProtected : weight_key(weight);
   };
-  for (int i = tid; i < min(n, kKeysInShared); i += kSelectThreads) keys[i] = key_of(i);
-  auto key_at = [&](int slot) { return slot < kKeysInShared ? keys[slot] : key_of(slot); };
 
   // ---- the budget-th largest key, by digits from the top
   uint32_t prefix = 0, want = e.budget;         // `want` keys are to come from those that share the prefix
@@ -101,6 +128,7 @@ __global__ void __launch_bounds__(kSelectThreads) cache4_select_kernel(const Cac
     const uint32_t above = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;
     for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
     __syncthreads();
+#pragma unroll 4
     for (int i = tid; i < n; i += kSelectThreads) {
       const uint32_t key = key_at(i);
       if (((key ^ prefix) & above) == 0) atomicAdd(&hist[(key >> shift) & digit_mask], 1u);
@@ -198,9 +226,9 @@ size_t cache4_evict_workspace(int B, int H, int budget) {
 
 cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& ev, int sm_count, cudaStream_t stream, long long* launches) {
   const long long room = static_cast<long long>(c.max_pages) << c.page_shift;
-  const int smem = static_cast<int>(room < kKeysInShared ? room : kKeysInShared) * 4;
+  const int smem = static_cast<int>(room < kKeysInShared ? room : kKeysInShared) * 8 + (c.max_pages < kPagesInShared ? c.max_pages : kPagesInShared) * 4;
   static std::atomic<unsigned long long> smem_done{0};
-  cudaError_t e = set_dynamic_smem_once(smem_done, reinterpret_cast<const void*>(cache4_select_kernel), kKeysInShared * 4);
+  cudaError_t e = set_dynamic_smem_once(smem_done, reinterpret_cast<const void*>(cache4_select_kernel), kSelectBytes);
   if (e != cudaSuccess) return e;
   const int heads = c.B * c.H;
   e = launch_persistent(cache4_select_kernel, heads, kSelectThreads, smem, stream, option_pdl() != 0, c, ev);
