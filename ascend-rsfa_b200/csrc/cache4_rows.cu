@@ -56,6 +56,7 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t codes, int j) {
 // whose loads go out together: one row at a time, each behind its own lookup of length and page, took twice as long.
 constexpr int kTokens = 64;
 constexpr int kAtOnce = 4;
+constexpr int kAppendAtOnce = 2;   // and as many on their way
 
 struct Chunk {
   int b, h, first, tokens;   // tokens: of this CTA
@@ -83,15 +84,19 @@ __device__ __forceinline__ Chunk chunk_of(const Cache4& c, int S) {
 constexpr int kChunkPages = kTokens / 16 + 1;
 struct ChunkPages {
   int64_t page[kChunkPages];       // -1: none
-  uint8_t* records[kChunkPages];   // of the CTA's head
+  int64_t records[kChunkPages];    // bytes from the start of the cache, for the CTA's head
+  int missing;                     // whether any is none
 };
 __device__ __forceinline__ void find_pages(ChunkPages& at, const Cache4& c, const Chunk& k, int first, int end) {
+  if (threadIdx.x == 0) at.missing = 0;
+  __syncwarp();                    // the first warp has all of them
   if (threadIdx.x < kChunkPages) {
     const int slot = ((first >> c.page_shift) + static_cast<int>(threadIdx.x)) << c.page_shift;   // the first of the page
     int64_t page = -1;
     if (slot >= end || !find_page(c, k.b, slot, &page)) page = -1;
+    if (slot < end && page < 0) at.missing = 1;
     at.page[threadIdx.x] = page;
-    at.records[threadIdx.x] = c.kv + (page < 0 ? 0 : page) * c.kv_stride[0] + k.h * c.kv_stride[1];
+    at.records[threadIdx.x] = (page < 0 ? 0 : page) * c.kv_stride[0] + k.h * c.kv_stride[1];
   }
   __syncthreads();
 }
@@ -118,30 +123,44 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
   const Chunk k = chunk_of<D>(c, rows.S);
   // rows behind the count are padding; a slot below zero is no token (a sequence that is not in use)
   const int count = rows.counts != nullptr ? min(max(rows.counts[k.b], 0), rows.S) : rows.S;
+  const int to = min(k.tokens, count - k.first);
+  if (to <= 0) return;
+  // The first rows are asked for before the sequence's length and pages are.
+  const int64_t* st = k.kv ? rows.v_stride : rows.k_stride;
+  const int64_t step_bytes = st[2] * 2 * k.step;
+  const uint8_t* src = static_cast<const uint8_t*>(k.kv ? rows.v : rows.k) + 2 * (k.b * st[0] + k.h * st[1] + 8 * k.lane + (k.first + k.sub) * st[2]);
+  uint4 next[kAppendAtOnce];
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < kAppendAtOnce; ++i) {
+      next[i] = t0 + i * k.step + k.sub < to ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+      src += step_bytes;
+    }
+  };
+  load(0);
   const int slot0 = tokens_of(c, k.b) - count + k.first;       // of the CTA's first token
-  const int from = max(0, -slot0), to = min(k.tokens, count - k.first);
+  const int from = max(0, -slot0);
   if (from >= to) return;
   __shared__ ChunkPages at;
   const int page0 = (slot0 + from) >> c.page_shift;
   find_pages(at, c, k, slot0 + from, slot0 + to);
-  const int64_t* st = k.kv ? rows.v_stride : rows.k_stride;
-  const int64_t step_bytes = st[2] * 2 * k.step;
-  const uint8_t* src = static_cast<const uint8_t*>(k.kv ? rows.v : rows.k) + 2 * (k.b * st[0] + k.h * st[1] + 8 * k.lane + (k.first + k.sub) * st[2]);
   const int w = k.lane >> 2, q = k.lane & 3;
   const int at_codes = code_word<D>(k.kv, w, q), at_pair = (k.kv ? R::kVPairs : R::kKPairs) + 4 * w;
   const int mask = (1 << c.page_shift) - 1;
-  for (int t0 = 0; t0 < to; t0 += kAtOnce * k.step) {
-    uint4 in[kAtOnce];
-    bool live[kAtOnce];
+  const bool missing = at.missing != 0;
+  uint8_t* const kv_codes = c.kv + at_codes;
+  for (int t0 = 0; t0 < to; t0 += kAppendAtOnce * k.step) {
+    uint4 in[kAppendAtOnce];
+    bool live[kAppendAtOnce];
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
+    for (int i = 0; i < kAppendAtOnce; ++i) {
       const int t = t0 + i * k.step + k.sub;
-      live[i] = t >= from && t < to && at.page[((slot0 + t) >> c.page_shift) - page0] >= 0;
-      in[i] = live[i] ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
-      src += step_bytes;
+      in[i] = next[i];
+      live[i] = t >= from && t < to && !(missing && at.page[((slot0 + t) >> c.page_shift) - page0] < 0);
     }
+    if (t0 + kAppendAtOnce * k.step < to) load(t0 + kAppendAtOnce * k.step);
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
+    for (int i = 0; i < kAppendAtOnce; ++i) {
       const int slot = slot0 + t0 + i * k.step + k.sub;
       const uint32_t words[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
       uint32_t lo2 = min2<kBf16>(min2<kBf16>(words[0], words[1]), min2<kBf16>(words[2], words[3]));
@@ -181,9 +200,9 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
       const uint32_t nan16 = kBf16 ? 0x7fc0u : 0x7e00u;
       const uint32_t pair = finite ? (s16 | (ends << 16)) : (nan16 | (nan16 << 16));
       const int off = slot & mask, which = (slot >> c.page_shift) - page0;
-      uint8_t* rec = at.records[which] + off * R::kBytes;
-      *reinterpret_cast<uint32_t*>(rec + at_codes) = k.kv ? turned : codes;
-      if (q == 0) *reinterpret_cast<uint32_t*>(rec + at_pair) = pair;
+      uint8_t* rec = kv_codes + (at.records[which] + off * R::kBytes);
+      *reinterpret_cast<uint32_t*>(rec) = k.kv ? turned : codes;
+      if (q == 0) *reinterpret_cast<uint32_t*>(rec + (at_pair - at_codes)) = pair;
     }
   }
   // what else there is of the tokens, one per thread
@@ -218,6 +237,7 @@ __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const Cache4 c, c
   const int w = k.lane >> 2, q = k.lane & 3;
   const int at_codes = code_word<D>(k.kv, w, q), at_pair = (k.kv ? R::kVPairs : R::kKPairs) + 4 * w;
   const int mask = (1 << c.page_shift) - 1;
+  const bool missing = at.missing != 0;
   for (int t0 = 0; t0 < k.tokens; t0 += kAtOnce * k.step) {
     uint32_t codes[kAtOnce], pair[kAtOnce];
 #pragma unroll
@@ -226,8 +246,8 @@ __global__ void __launch_bounds__(kThreads) cache4_read_kernel(const Cache4 c, c
       codes[i] = pair[i] = 0;
       if (t >= from && t < to) {
         const int slot = first + t - from, which = (slot >> c.page_shift) - page0;
-        if (at.page[which] >= 0) {
-          const uint8_t* rec = at.records[which] + (slot & mask) * R::kBytes;
+        if (!(missing && at.page[which] < 0)) {
+          const uint8_t* rec = c.kv + (at.records[which] + (slot & mask) * R::kBytes);
           codes[i] = *reinterpret_cast<const uint32_t*>(rec + at_codes);
           pair[i] = *reinterpret_cast<const uint32_t*>(rec + at_pair);
         }
