@@ -915,16 +915,33 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
       if (lse == -INFINITY) lse = 0.f;                         // a row that sees nothing: its scores are -inf
     }
     const int run = min(k.tiles - k.t, k.left);
-    for (int i = 0; i < run * (kTile / 32); ++i) {
-      const int tile = i / (kTile / 32), part = i % (kTile / 32) * 32;
-      const float* scores = a.scores + (k.at + tile) * rows.count * kTile + part + lane;
-      float sum = 0.f;
-#pragma unroll 8
-      for (int r = 0; r < rows.count; ++r) sum += ex2(scores[r * kTile] - __shfl_sync(0xffffffffu, lse, r));
-      const int slot = (k.t + tile) * kTile + part + lane;
-      int64_t page;
-      if (slot < k.n && find_page(c, k.b, slot, &page))
-        c.weight[page * c.weight_stride[0] + k.item * c.weight_stride[1] + (slot & mask)] += sum;
+    // 32 tokens are a group; the loads of four groups go out together
+    constexpr int kGroups = 4, kPerTile = kTile / 32;
+    for (int i = 0; i < run * kPerTile; i += kGroups) {
+      const float* scores[kGroups];
+      float* weight[kGroups];
+      float sum[kGroups], old[kGroups];
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        const int g = min(i + j, run * kPerTile - 1), tile = g / kPerTile, part = g % kPerTile * 32;
+        scores[j] = a.scores + (k.at + tile) * rows.count * kTile + part + lane;
+        const int slot = (k.t + tile) * kTile + part + lane;
+        int64_t page;
+        const bool ours = i + j < run * kPerTile && slot < k.n && find_page(c, k.b, slot, &page);
+        weight[j] = ours ? c.weight + page * c.weight_stride[0] + k.item * c.weight_stride[1] + (slot & mask) : nullptr;
+        sum[j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) old[j] = weight[j] != nullptr ? *weight[j] : 0.f;
+#pragma unroll 4
+      for (int r = 0; r < rows.count; ++r) {
+        const float of_row = __shfl_sync(0xffffffffu, lse, r);
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) sum[j] += ex2(scores[j][r * kTile] - of_row);
+      }
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j)
+        if (weight[j] != nullptr) *weight[j] = old[j] + sum[j];
     }
     k.left -= run;
     k.at += run;
