@@ -42,6 +42,7 @@ struct Shape {
   static constexpr int kSlotBytes = kTile * Record<D>::kBytes;
   static constexpr int kRingBytes = kWarps * kStages * kSlotBytes;
 };
+constexpr int kItemCost = 2;         // tiles that an item takes as long as beside its own, see all_units
 constexpr int kTagCache4Load = 40;   // of a bounded wait, in the status word
 constexpr float kRaise = 8.f;        // log2 units above the reference at which it is raised
 constexpr float kRaiseScale = 64.f;  // and the scales' one
@@ -84,6 +85,16 @@ __device__ __forceinline__ float add_high(float sum, uint32_t pair) {
   asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nadd.f32.f16 %0, h, %0;\n}\n" : "+f"(sum) : "r"(pair));
   return sum;
 }
+// The low half of a pair, a number of the cache's type, times another such number: conversion and factor in one.
+template <bool kBf16>
+__device__ __forceinline__ float scale_of(uint32_t pair, uint16_t by) {
+  float r;
+  if constexpr (kBf16)
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nfma.rn.f32.bf16 %0, l, %2, %3;\n}\n" : "=f"(r) : "r"(pair), "h"(by), "f"(0.f));
+  else
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nfma.rn.f32.f16 %0, l, %2, %3;\n}\n" : "=f"(r) : "r"(pair), "h"(by), "f"(0.f));
+  return r;
+}
 // 8 s + m of two neighbouring tokens' pairs (low half scale, high half minimum).
 template <bool kBf16>
 __device__ __forceinline__ uint32_t middles(uint32_t first, uint32_t second) {
@@ -121,13 +132,17 @@ __device__ __forceinline__ int tiles_of(const Cache4& c, const int* counts, int 
   const int shift = c.D == 64 ? 6 : 5;
   return (visible_tokens(c, counts, b) + (1 << shift) - 1) >> shift;
 }
-// One warp: tiles of all sequences and of those before b, per K/V head and block of rows.
-__device__ __forceinline__ long long all_tiles(const Cache4& c, const int* counts, int b, long long* before) {
+// What is divided among the warps: an item of n tiles is n + cost units, cost of them in front for what an item takes by
+// itself (its query rows, its results).  Short items would otherwise make the shares that have many of them the last
+// ones: 64 sequences of 1 to 8192 tokens 103 -> 86 us (94 with a cost of one tile, 85 and 86 with three and four).
+//
+// One warp: units of all sequences and of those before b, per K/V head and block of rows.
+__device__ __forceinline__ long long all_units(const Cache4& c, const int* counts, int cost, int b, long long* before) {
   long long n = 0, m = 0;
   for (int i = threadIdx.x & 31; i < c.B; i += 32) {
-    const int tiles = tiles_of(c, counts, i);
-    n += tiles;
-    m += i < b ? tiles : 0;
+    const int tiles = tiles_of(c, counts, i), units = tiles > 0 ? tiles + cost : 0;
+    n += units;
+    m += i < b ? units : 0;
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
@@ -137,65 +152,84 @@ __device__ __forceinline__ long long all_tiles(const Cache4& c, const int* count
   *before = m;
   return n;
 }
-// One warp: the sequence that tile `at` belongs to and the first tile of that sequence.
-__device__ __forceinline__ int sequence_of(const Cache4& c, const int* counts, int per_sequence, long long at, long long* first, int* tiles) {
-  const int lane = threadIdx.x & 31;
-  long long before = 0;
-  for (int base = 0; base < c.B; base += 32) {
-    const int mine = base + lane < c.B ? tiles_of(c, counts, base + lane) : 0;
-    long long sum = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += u;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, (before + sum) * per_sequence > at);
-    if (past != 0) {
-      const int l = __ffs(past) - 1;
-      *tiles = __shfl_sync(0xffffffffu, mine, l);
-      *first = (before + __shfl_sync(0xffffffffu, sum, l) - *tiles) * per_sequence;
-      return base + l;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  return -1;
-}
-// Worker w of `workers`, no more than there are tiles, has the tiles from share_begin(w) to share_begin(w + 1).  Its number
-// goes over the CTAs first, so that a few tiles are spread over all multiprocessors.
+// Worker w of `workers`, no more than there are units, has the units from share_begin(w) to share_begin(w + 1).  Its number
+// goes over the CTAs first, so that a few units are spread over all multiprocessors.
 __device__ __forceinline__ long long worker_here() { return static_cast<long long>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; }
 __device__ __forceinline__ long long workers_used(long long total, long long all) { return total < all ? total : all; }
 __device__ __forceinline__ long long share_begin(long long total, long long worker, long long workers) {
   return total * worker / workers;
 }
-__device__ __forceinline__ long long worker_of(long long total, long long tile, long long workers) {
-  return ((tile + 1) * workers - 1) / total;
+__device__ __forceinline__ long long worker_of(long long total, long long unit, long long workers) {
+  return ((unit + 1) * workers - 1) / total;
 }
 
-// A place in the list: item `item` of sequence b, tile t of `tiles`, and the tiles of the share from here on.
+// A place in the list: tiles t to end of item `item` of sequence b are the share's.
 struct Cursor {
-  int b, n, tiles, item, t, left;
-  long long at;
+  int b, n, tiles, item, t, end;
+  int left;                // units of the share behind this item
+  long long at;            // the item's first tile in the list of tiles alone
 };
-__device__ __forceinline__ Cursor cursor_at(const Cache4& c, const int* counts, int per_sequence, long long at, long long end) {
-  Cursor k;
-  long long first;
-  k.b = sequence_of(c, counts, per_sequence, at, &first, &k.tiles);
-  k.n = tokens_of(c, k.b);
-  k.item = static_cast<int>((at - first) / k.tiles);
-  k.t = static_cast<int>(at - first - static_cast<long long>(k.item) * k.tiles);
-  k.left = static_cast<int>(end - at);
-  k.at = at;
-  return k;
+// To the next item of the share that has tiles of it; t = end if there is none.
+__device__ __forceinline__ void next_item(Cursor& k, const Cache4& c, const int* counts, int per_sequence, int cost) {
+  while (k.left > 0) {
+    k.at += k.tiles;
+    if (++k.item == per_sequence) {
+      k.item = 0;
+      do {
+        if (++k.b >= c.B) {
+          k.left = k.t = k.end = 0;
+          return;
+        }
+        k.tiles = tiles_of(c, counts, k.b);
+      } while (k.tiles == 0);
+      k.n = tokens_of(c, k.b);
+    }
+    const int units = min(k.tiles + cost, k.left);
+    k.left -= units;
+    k.t = 0;
+    k.end = units - cost;
+    if (k.end > 0) return;
+  }
+  k.t = k.end = 0;
 }
-// To the next item, for which tiles are left.
-__device__ __forceinline__ void next_item(Cursor& k, const Cache4& c, const int* counts, int per_sequence) {
-  k.t = 0;
-  if (++k.item < per_sequence) return;
-  k.item = 0;
-  do {                     // a sequence that has tokens: there is one
-    k.tiles = tiles_of(c, counts, ++k.b);
-  } while (k.tiles == 0);
+// One warp: the cursor of the units from `from` to `to`.
+__device__ __forceinline__ Cursor cursor_at(const Cache4& c, const int* counts, int per_sequence, int cost, long long from, long long to) {
+  const int lane = threadIdx.x & 31;
+  Cursor k;
+  long long before = 0, first = 0;      // units before the sequences looked at; of the sequence
+  int sequences = 0;                    // with tokens, before it
+  k.b = -1;
+  for (int base = 0; base < c.B && k.b < 0; base += 32) {
+    const int tiles = base + lane < c.B ? tiles_of(c, counts, base + lane) : 0, units = tiles > 0 ? tiles + cost : 0;
+    long long sum = units;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += u;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, (before + sum) * per_sequence > from), filled = __ballot_sync(0xffffffffu, tiles > 0);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      k.tiles = __shfl_sync(0xffffffffu, tiles, l);
+      first = (before + __shfl_sync(0xffffffffu, sum, l) - (k.tiles + cost)) * per_sequence;
+      sequences += __popc(filled & ((1u << l) - 1u));
+      k.b = base + l;
+    } else {
+      before += __shfl_sync(0xffffffffu, sum, 31);
+      sequences += __popc(filled);
+    }
+  }
   k.n = tokens_of(c, k.b);
+  const int length = k.tiles + cost;
+  k.item = static_cast<int>((from - first) / length);
+  const int unit = static_cast<int>(from - first - static_cast<long long>(k.item) * length);
+  const int units = static_cast<int>(min(static_cast<long long>(length - unit), to - from));
+  k.at = first - static_cast<long long>(sequences) * per_sequence * cost + static_cast<long long>(k.item) * k.tiles;
+  k.t = max(unit - cost, 0);
+  k.end = max(unit + units - cost, 0);
+  k.left = static_cast<int>(to - from) - units;
+  if (k.t >= k.end) next_item(k, c, counts, per_sequence, cost);
+  return k;
 }
 
 // ------------------------------------------------------------------ query rows
@@ -210,7 +244,7 @@ template <int D, int NT>
 struct Query {
   static constexpr int G = D / 32;
   uint32_t frag[NT][G][4];
-  // Sums of the groups times 2^-6, as three numbers of the cache's type each: B fragments of the product with the
+  // Sums of the groups times 2^-9, as three numbers of the cache's type each: B fragments of the product with the
   // minima, whose k index runs over (part, group).
   static constexpr int kSumMmas = (3 * G + 7) / 8;
   uint32_t sums[NT][kSumMmas];
@@ -272,7 +306,7 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
       f.frag[nt][w][3] = from_f32x2<false>(x[w][3] * 0.0625f, x[w][7] * 0.0625f);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      rest[w] = sum * 0.015625f;
+      rest[w] = sum * 0.001953125f;
     }
     // every lane has numbers 2 c, 2 c + 1 of each eight
 #pragma unroll
@@ -289,7 +323,7 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
         if (2 * q4 == (at & 7)) f.sums[nt][at >> 3] = pair;
       }
     }
-    const float factor = fmaxf(up * 16777216.f * (fabsf(a.sm_scale) * kLog2e), 1e-37f);   // -inf times it stays -inf
+    const float factor = fmaxf(up * 512.f * (fabsf(a.sm_scale) * kLog2e), 1e-37f);   // -inf times it stays -inf
     f.factor[nt][0] = __shfl_sync(0xffffffffu, factor, 8 * q4);
     f.factor[nt][1] = __shfl_sync(0xffffffffu, factor, 8 * q4 + 4);
 #pragma unroll
@@ -341,13 +375,12 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
     for (int j = 0; j < 4; ++j) s[nt][j] = 0.f;
 #pragma unroll
     for (int k = 0; k < Query<D, NT>::kSumMmas; ++k) mma_own_k8<kBf16>(s[nt], m_lo, m_hi, f.sums[nt][k]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[nt][j] *= 3.814697265625e-6f;   // 2^6 and 2^-24
   }
 #pragma unroll
   for (int w = 0; w < G; ++w) {
     const uint32_t a8 = kl[w] >> 8, b8 = kh[w] >> 8;
-    const float sl = to_f32<kBf16>(static_cast<uint16_t>(pl[w])), sh = to_f32<kBf16>(static_cast<uint16_t>(ph[w]));
+    // codes count 2^-24, the sums 2^-9
+    const float sl = scale_of<kBf16>(pl[w], kBf16 ? 0x4700 : 0x7800), sh = scale_of<kBf16>(ph[w], kBf16 ? 0x4700 : 0x7800);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float acc[4];
@@ -368,17 +401,20 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
 template <int D, int NT>
 struct Sums {
   static constexpr int G = D / 32;
-  float o[2 * G][NT][4];       // tile 2 w + t: dims 32 w + 4 g + 2 t (times 2^-24) and + 1 (times 2^-20), both over `unit`
+  float o[2 * G][NT][4];       // tile 2 w + t, times 2^-24 over `unit`: dim 32 w + 4 g + 2 t, and that plus 16 times the next
   float rounded[NT][G][2];     // this lane's share of sum P, rows 2 c, 2 c + 1, over `unit`
   float mids[NT][4];           // sum p (m + 8 s) of group g % G, rows 2 c, 2 c + 1 (twice)
   float l[NT][2], ref[NT][2];
-  float unit;                  // power of two that p * s is divided by
+  float unit;                  // power of two that s is divided by
+  uint32_t per_unit;           // 1 / unit, a 16-bit number of the cache's type
   uint32_t unit_limit;         // 16-bit pattern of the scale from which on it is raised
 };
-constexpr float kLeastUnit = 7.888609052210118e-31f;   // 2^-100
+// 1 / unit has to be a number of the cache's type: 2^-15 and 2^-100.  Scales below that are fp16's subnormal ones.
+template <bool kBf16>
+constexpr float kLeastUnit = kBf16 ? 7.888609052210118e-31f : 3.0517578125e-5f;
 constexpr float kNoScore = -3.4028234663852886e38f;    // reference of a row that has seen nothing
 
-template <int D, int NT>
+template <int D, int NT, bool kBf16>
 __device__ __forceinline__ void clear(Sums<D, NT>& x) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -396,8 +432,9 @@ __device__ __forceinline__ void clear(Sums<D, NT>& x) {
       x.ref[nt][i] = kNoScore;
     }
   }
-  x.unit = kLeastUnit;
-  x.unit_limit = 0;
+  x.unit = kLeastUnit<kBf16>;
+  x.per_unit = from_f32<kBf16>(1.f / kLeastUnit<kBf16>);
+  x.unit_limit = from_f32<kBf16>(kLeastUnit<kBf16> * kRaiseScale);
 }
 
 // Tokens of a block whose V pairs are NaN: a row that gives one of them weight gets NaN for the group, and the pairs
@@ -424,7 +461,7 @@ __device__ __noinline__ void defuse_block(uint8_t* rec, const float* p, float* m
 
 // The second product of 16 tokens: p of tokens (g, g + 8).
 template <int D, int NT, bool kBf16>
-__device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT][4], const uint8_t* rec, float per_unit) {
+__device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT][4], const uint8_t* rec) {
   using R = Record<D>;
   constexpr int G = D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -459,27 +496,24 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
     }
   }
   const uint32_t mid_lo = middles<kBf16>(mid[0], mid[1]), mid_hi = middles<kBf16>(mid[2], mid[3]);
-  float pu[NT][4];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int nt = 0; nt < NT; ++nt)
     mma_own<kBf16>(x.mids[nt], mid_lo, mid_lo, mid_hi, mid_hi, transpose_8x8(from_f32x2<kBf16>(p[nt][0], p[nt][1])),
                    transpose_8x8(from_f32x2<kBf16>(p[nt][2], p[nt][3])));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pu[nt][j] = p[nt][j] * per_unit;
-  }
-#pragma unroll
   for (int w = 0; w < G; ++w) {
-    // the half words of group w: low half token 2 c (2 c + 8), high half the token behind it
+    // The half words of group w: low half token 2 c (2 c + 8), high half the token behind it.  A byte is two codes; taken
+    // whole and with the first one alone it needs an operation less than with each by itself.
     const uint32_t pick = (w & 1) ? 0x7632u : 0x5410u;
     const uint32_t y = __byte_perm(v[0][w / 2], v[1][w / 2], pick), z = __byte_perm(v[2][w / 2], v[3][w / 2], pick);
-    const uint32_t y8 = y >> 8, z8 = z >> 8;
-    const float sl = to_f32<kBf16>(static_cast<uint16_t>(pl[w])), sh = to_f32<kBf16>(static_cast<uint16_t>(ph[w]));
+    const uint32_t y1 = __byte_perm(y, 0u, 0x4341), z1 = __byte_perm(z, 0u, 0x4341);
+    const float sl = scale_of<kBf16>(pl[w], static_cast<uint16_t>(x.per_unit)), sh = scale_of<kBf16>(ph[w], static_cast<uint16_t>(x.per_unit));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t pl2 = from_f32x2<false>(pu[nt][0] * sl, pu[nt][1] * sl), ph2 = from_f32x2<false>(pu[nt][2] * sh, pu[nt][3] * sh);
+      const uint32_t pl2 = from_f32x2<false>(p[nt][0] * sl, p[nt][1] * sl), ph2 = from_f32x2<false>(p[nt][2] * sh, p[nt][3] * sh);
       const uint32_t b0 = transpose_8x8(pl2), b1 = transpose_8x8(ph2);
-      mma_f16(x.o[2 * w][nt], y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, b0, b1);
-      mma_f16(x.o[2 * w + 1][nt], y8 & 0x000f000fu, y8 & 0x00f000f0u, z8 & 0x000f000fu, z8 & 0x00f000f0u, b0, b1);
+      mma_f16(x.o[2 * w][nt], y & 0x000f000fu, y & 0x00ff00ffu, z & 0x000f000fu, z & 0x00ff00ffu, b0, b1);
+      mma_f16(x.o[2 * w + 1][nt], y1 & 0x000f000fu, y1, z1 & 0x000f000fu, z1, b0, b1);
       x.rounded[nt][w][0] = add_low(add_low(x.rounded[nt][w][0], pl2), ph2);
       x.rounded[nt][w][1] = add_high(add_high(x.rounded[nt][w][1], pl2), ph2);
     }
@@ -499,6 +533,7 @@ __device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2],
   const float unit = scale > x.unit * kRaiseScale ? __uint_as_float(__float_as_uint(scale) & 0x7f800000u) : x.unit;
   const float by_unit = x.unit / unit;
   x.unit = unit;
+  x.per_unit = from_f32<kBf16>(1.f / unit);
   x.unit_limit = from_f32<kBf16>(unit * kRaiseScale);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -565,7 +600,6 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
     odd = __any_sync(0xffffffffu, widest > (kBf16 ? 0x7f80u : 0x7c00u));
     raise<D, NT, kBf16>(x, top, widest);
   }
-  const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(x.unit));   // 1 / a power of two
   if (scores != nullptr) {
 #pragma unroll
     for (int k = 0; k < kBlocks; ++k)
@@ -598,7 +632,7 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
     }
   }
 #pragma unroll
-  for (int k = 0; k < kBlocks; ++k) block_output<D, NT, kBf16>(x, s[k], rec + 16 * k * R::kBytes, per_unit);
+  for (int k = 0; k < kBlocks; ++k) block_output<D, NT, kBf16>(x, s[k], rec + 16 * k * R::kBytes);
   return odd;
 }
 
@@ -614,7 +648,7 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   // codes back from their places in a word, then what p * s was divided by
   auto low = [&](float v) { return v * 16777216.f * x.unit; };
-  auto high = [&](float v) { return v * 1048576.f * x.unit; };
+  auto high = [&](float first, float both) { return (both - first) * 1048576.f * x.unit; };
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -636,9 +670,9 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
           float* dst = piece + r * (D + 2);
 #pragma unroll
           for (int w = 0; w < G; ++w) {
-            *reinterpret_cast<float2*>(dst + 32 * w + 4 * g) = make_float2(low(x.o[2 * w][nt][i]) + m[w], high(x.o[2 * w][nt][i + 2]) + m[w]);
+            *reinterpret_cast<float2*>(dst + 32 * w + 4 * g) = make_float2(low(x.o[2 * w][nt][i]) + m[w], high(x.o[2 * w][nt][i], x.o[2 * w][nt][i + 2]) + m[w]);
             *reinterpret_cast<float2*>(dst + 32 * w + 4 * g + 2) =
-                make_float2(low(x.o[2 * w + 1][nt][i]) + m[w], high(x.o[2 * w + 1][nt][i + 2]) + m[w]);
+                make_float2(low(x.o[2 * w + 1][nt][i]) + m[w], high(x.o[2 * w + 1][nt][i], x.o[2 * w + 1][nt][i + 2]) + m[w]);
           }
           if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(x.ref[nt][i], l);
         } else {
@@ -648,8 +682,8 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
 #pragma unroll
           for (int w = 0; w < G; ++w)
             *reinterpret_cast<uint2*>(dst + 32 * w + 4 * g) =
-                make_uint2(from_f32x2<kBf16>((low(x.o[2 * w][nt][i]) + m[w]) * inv, (high(x.o[2 * w][nt][i + 2]) + m[w]) * inv),
-                           from_f32x2<kBf16>((low(x.o[2 * w + 1][nt][i]) + m[w]) * inv, (high(x.o[2 * w + 1][nt][i + 2]) + m[w]) * inv));
+                make_uint2(from_f32x2<kBf16>((low(x.o[2 * w][nt][i]) + m[w]) * inv, (high(x.o[2 * w][nt][i], x.o[2 * w][nt][i + 2]) + m[w]) * inv),
+                           from_f32x2<kBf16>((low(x.o[2 * w + 1][nt][i]) + m[w]) * inv, (high(x.o[2 * w + 1][nt][i], x.o[2 * w + 1][nt][i + 2]) + m[w]) * inv));
           if (g == 0 && a.lse != nullptr)
             a.lse[(static_cast<int64_t>(b) * a.Hq + hq) * a.S + t] = l == 0.f ? -INFINITY : (x.ref[nt][i] + __log2f(l)) * kLn2;
         }
@@ -679,10 +713,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   griddep_wait();
   const int per_sequence = c.H * row_blocks;
   long long none;
-  const long long total = all_tiles(c, a.counts, 0, &none) * per_sequence;
+  const long long total = all_units(c, a.counts, kItemCost, 0, &none) * per_sequence;
   const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
   if (worker >= workers) return;
-  Cursor use = cursor_at(c, a.counts, per_sequence, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  Cursor use = cursor_at(c, a.counts, per_sequence, kItemCost, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  if (use.t >= use.end) return;            // nothing but an item's cost
   Cursor load = use;
   uint8_t* const my_ring = ring + warp * Sh::kStages * Sh::kSlotBytes;
   const uint32_t my_bar = smem_u32(&full_bar[warp * Sh::kStages]);
@@ -718,34 +753,31 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
     const int i = lane - off;
     if (static_cast<unsigned>(i) < Sh::kPieces && ((there >> lane) & 1))
       bulk_load(smem_u32(my_ring + stage * Sh::kSlotBytes) + i * Sh::kPieceBytes, piece_at, bar, Sh::kPieceBytes);
-    --load.left;
-    if (++load.t == load.tiles) {
-      if (load.left > 0) {
-        const int b = load.b;
-        next_item(load, c, a.counts, per_sequence);
-        // the next head of a short sequence has the same pages
-        open_window(0, load.b == b && window == 0 ? pages : page_of(lane));
-      }
+    if (++load.t == load.end) {
+      const int b = load.b;
+      next_item(load, c, a.counts, per_sequence, kItemCost);
+      // the next head of a short sequence has the same pages
+      if (load.t < load.end) open_window(0, load.b == b && window == 0 ? pages : page_of(lane));
     } else if (off + Sh::kPieces == 32) {
       open_window(window + 32, pages_next);
     }
   };
 #pragma unroll 1
-  for (int i = 0; i < Sh::kStages && load.left > 0; ++i) issue(i);
+  for (int i = 0; i < Sh::kStages && load.t < load.end; ++i) issue(i);
 
   const int score_rows = min(8 * NT, rows.count);     // of a tile; as many as an item has
   float* const kept = c.weight != nullptr && row_blocks == 1 ? a.scores : nullptr;
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
-  while (use.left > 0) {
+  while (use.t < use.end) {
     // one piece: the tiles of one item that belong to this share
     const int b = use.b, t0 = use.t, tiles = use.tiles, h = use.item / row_blocks, row0 = (use.item - h * row_blocks) * 8 * NT, n = use.n;
-    const int t1 = min(tiles, t0 + use.left);
+    const int t1 = use.end;
     Query<D, NT> f;
     load_query<D, NT, kBf16>(f, c, a, rows, b, h, row0, n);
     Sums<D, NT> x;
-    clear(x);
+    clear<D, NT, kBf16>(x);
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
       ok = mbar_wait_warp(my_bar + 8 * stage, phase, &abort_word, wait_limit_ns, kTagCache4Load);
@@ -762,11 +794,11 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
         }
         __syncwarp();
       }
-      float* scores = kept != nullptr ? kept + (use.at + t - t0) * score_rows * kTile : nullptr;
+      float* scores = kept != nullptr ? kept + (use.at + t) * score_rows * kTile : nullptr;
       const bool written = one_tile<D, NT, kBf16>(x, f, slot, t * kTile, scores, score_rows);
       if (patch || written) fence_proxy_async();      // before a copy writes where this warp has written
       __syncwarp();
-      if (load.left > 0) issue(stage);
+      if (load.t < load.end) issue(stage);
       if (++stage == Sh::kStages) {
         stage = 0;
         phase ^= 1;
@@ -776,9 +808,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
     float* piece = nullptr;
     if (t0 > 0 || t1 < tiles) piece = a.pieces + (worker * 2 + (t0 == 0)) * piece_floats<D, NT>();
     store_sums<D, NT, kBf16>(x, a, rows, b, h, row0, piece);
-    use.left -= t1 - t0;
-    use.at += t1 - t0;
-    if (use.left > 0) next_item(use, c, a.counts, per_sequence);
+    next_item(use, c, a.counts, per_sequence, kItemCost);
   }
   if (!ok) {
     // a copy did not arrive in time: said in the status word; no copy is left behind without a second wait
@@ -822,9 +852,9 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
   }
   const int per_sequence = c.H * row_blocks;
   long long before;
-  const long long total = all_tiles(c, a.counts, b, &before) * per_sequence;
+  const long long total = all_units(c, a.counts, kItemCost, b, &before) * per_sequence;
   const long long workers = workers_used(total, all_workers);
-  const long long first = before * per_sequence + static_cast<long long>(item) * tiles;
+  const long long first = before * per_sequence + static_cast<long long>(item) * (tiles + kItemCost) + kItemCost;   // unit of its first tile
   const long long w0 = worker_of(total, first, workers), w1 = worker_of(total, first + tiles - 1, workers);
   if (w0 == w1) return;                       // in one piece: answered already
   const int pieces = static_cast<int>(w1 - w0) + 1;
@@ -901,12 +931,12 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
   griddep_wait();
   const int lane = threadIdx.x & 31;
   long long none;
-  const long long total = all_tiles(c, a.counts, 0, &none) * c.H;
+  const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
   const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
   if (worker >= workers) return;
-  Cursor k = cursor_at(c, a.counts, c.H, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  Cursor k = cursor_at(c, a.counts, c.H, 0, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
   const int mask = (1 << c.page_shift) - 1;
-  while (k.left > 0) {
+  while (k.t < k.end) {
     // log-sum-exps of the item's rows, one per lane (there are no more than 16)
     float lse = 0.f;
     if (lane < rows.count) {
@@ -914,7 +944,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
       lse = a.lse[(static_cast<int64_t>(k.b) * a.Hq + hq) * a.S + t] * kLog2e;
       if (lse == -INFINITY) lse = 0.f;                         // a row that sees nothing: its scores are -inf
     }
-    const int run = min(k.tiles - k.t, k.left);
+    const int run = k.end - k.t;
     // 32 tokens are a group; the loads of four groups go out together
     constexpr int kGroups = 4, kPerTile = kTile / 32;
     for (int i = 0; i < run * kPerTile; i += kGroups) {
@@ -924,7 +954,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
 #pragma unroll
       for (int j = 0; j < kGroups; ++j) {
         const int g = min(i + j, run * kPerTile - 1), tile = g / kPerTile, part = g % kPerTile * 32;
-        scores[j] = a.scores + (k.at + tile) * rows.count * kTile + part + lane;
+        scores[j] = a.scores + (k.at + k.t + tile) * rows.count * kTile + part + lane;
         const int slot = (k.t + tile) * kTile + part + lane;
         int64_t page;
         const bool ours = i + j < run * kPerTile && slot < k.n && find_page(c, k.b, slot, &page);
@@ -943,9 +973,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
       for (int j = 0; j < kGroups; ++j)
         if (weight[j] != nullptr) *weight[j] = old[j] + sum[j];
     }
-    k.left -= run;
-    k.at += run;
-    if (k.left > 0) next_item(k, c, a.counts, c.H);
+    next_item(k, c, a.counts, c.H, 0);
   }
 }
 
@@ -958,13 +986,13 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cac
   griddep_wait();
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   long long none;
-  const long long total = all_tiles(c, a.counts, 0, &none) * c.H;
+  const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
   const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
   if (worker >= workers) return;
-  Cursor k = cursor_at(c, a.counts, c.H, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  Cursor k = cursor_at(c, a.counts, c.H, 0, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
   const int mask = (1 << c.page_shift) - 1;
-  while (k.left > 0) {
-    const int run = min(k.tiles - k.t, k.left);
+  while (k.t < k.end) {
+    const int run = k.end - k.t;
     for (int block = 0; block < row_blocks; ++block) {
       Query<D, NT> f;
       load_query<D, NT, kBf16>(f, c, a, rows, k.b, k.item, 8 * NT * block, k.n);
@@ -998,8 +1026,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cac
         }
       }
     }
-    k.left -= run;
-    if (k.left > 0) next_item(k, c, a.counts, c.H);
+    next_item(k, c, a.counts, c.H, 0);
   }
 }
 
