@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <cstring>
+#include <optional>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -19,6 +20,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/rsfa.h"
@@ -206,6 +208,92 @@ PyObject* tensor_pair(at::Tensor a, at::Tensor b) {
   return pair;
 }
 
+// The GIL is released while a launch may block; what is thrown in between comes out with it held again.
+template <typename F>
+void without_gil(F f) {
+  PyThreadState* state = PyEval_SaveThread();
+  try {
+    f();
+  } catch (...) {
+    PyEval_RestoreThread(state);
+    throw;
+  }
+  PyEval_RestoreThread(state);
+}
+
+// rsfa_rotary on tensors that it can read; k and pos may be undefined.
+int turn(const at::Tensor& q, const at::Tensor& k, const at::Tensor& table, const at::Tensor& pos, bool interleaved, bool inverse, at::Tensor* qo,
+         at::Tensor* ko) {
+  *qo = rows_like(q);
+  if (k.defined()) *ko = rows_like(k);
+  int64_t strides[16] = {}, pos_strides[2] = {0, 0};
+  copy_strides(strides, q);
+  copy_strides(strides + 8, *qo);
+  if (k.defined()) {
+    copy_strides(strides + 4, k);
+    copy_strides(strides + 12, *ko);
+  }
+  if (pos.defined()) {
+    pos_strides[0] = pos.dim() == 1 || pos.size(0) == 1 ? 0 : pos.stride(0);
+    pos_strides[1] = pos.stride(-1);
+  }
+  return g_ops.rotary(q.const_data_ptr(), k.defined() ? k.const_data_ptr() : nullptr, qo->mutable_data_ptr(),
+                      k.defined() ? ko->mutable_data_ptr() : nullptr, static_cast<int>(q.size(0)), static_cast<int>(q.size(1)),
+                      k.defined() ? static_cast<int>(k.size(1)) : 0, static_cast<int>(q.size(2)), static_cast<int>(q.size(3)), strides,
+                      static_cast<const float*>(table.const_data_ptr()), static_cast<int>(table.size(0)), static_cast<int>(2 * table.size(1)),
+                      pos.defined() ? pos.const_data_ptr() : nullptr, pos.defined() && pos.scalar_type() == at::kLong ? 1 : 0,
+                      pos.defined() ? pos_strides : nullptr, interleaved, inverse, dtype_of(q),
+                      c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+}
+
+// The same as an operation that autograd records: its gradient is the transposed rotation, which can be recorded again.
+// (As a Python function the two calls of a training step took 40 us more of the host's time.)
+struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const std::optional<at::Tensor>& k_or,
+                                                const at::Tensor& table, const std::optional<at::Tensor>& pos_or, bool interleaved, bool inverse) {
+    const at::Tensor k = k_or.value_or(at::Tensor()), pos = pos_or.value_or(at::Tensor());
+    at::Tensor qo, ko;
+    const int rc = turn(q, k, table, pos, interleaved, inverse, &qo, &ko);
+    TORCH_CHECK(rc == 0, "rsfa_rotary failed with code ", rc);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({table, pos});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    if (!k.defined()) return {qo};
+    return {qo, ko};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
+    at::Tensor of_q = readable(grads[0]), of_k = grads.size() > 1 ? readable(grads[1]) : at::Tensor();
+    torch::autograd::variable_list out(6);
+    if (!of_q.defined() && !of_k.defined()) return out;
+    const bool q_first = of_q.defined();                       // the library wants the first of its two tensors
+    const at::Tensor first = q_first ? of_q : of_k, second = q_first ? of_k : at::Tensor();
+    at::Tensor a, b;
+    if (c10::GradMode::is_enabled() && (first.requires_grad() || (second.defined() && second.requires_grad()))) {
+      const auto again = RotaryFunction::apply(first, given(second), saved[0], given(saved[1]), interleaved, inverse);
+      a = again[0];
+      if (second.defined()) b = again[1];
+    } else {
+      const int rc = turn(first, second, saved[0], saved[1], interleaved, inverse, &a, &b);
+      TORCH_CHECK(rc == 0, "rsfa_rotary failed with code ", rc);
+    }
+    out[q_first ? 0 : 1] = a;
+    if (q_first) out[1] = b;
+    return out;
+  }
+  static std::optional<at::Tensor> given(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+  // Rows as the library reads them, copied once if need be.
+  static at::Tensor readable(const at::Tensor& t) {
+    if (!t.defined()) return t;
+    bool ok = t.stride(3) == 1;
+    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) % 8 == 0 && t.stride(i) >= t.size(3)));
+    at::Tensor r = ok ? t : t.contiguous();
+    return (reinterpret_cast<uintptr_t>(r.const_data_ptr()) & 15u) == 0 ? r : r.clone(at::MemoryFormat::Contiguous);
+  }
+};
+
 // rotary(q, k or None, table, positions or None, interleaved, inverse) -> (q', k' or None), an error code, or None.
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -215,45 +303,33 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* q = plain_rows(args[0], device);
   const at::Tensor* k = args[1] == Py_None ? nullptr : plain_rows(args[1], device);
   const at::Tensor* table = plain_cuda(args[2], at::kFloat, 3, device);
-  if (q == nullptr || (k == nullptr && args[1] != Py_None) || table == nullptr || records_grad(*q) || (k != nullptr && records_grad(*k)))
-    Py_RETURN_NONE;
+  if (q == nullptr || (k == nullptr && args[1] != Py_None) || table == nullptr) Py_RETURN_NONE;
   const int64_t B = q->size(0), S = q->size(2), D = q->size(3), R = 2 * table->size(1);
   if (!(D == 16 || D == 32 || D == 64 || D == 128 || D == 256) || R > D || R < 2 || table->size(2) != 2 || !table->is_contiguous() ||
       table->size(0) < 1 || table->size(0) > INT32_MAX || table->requires_grad())
     Py_RETURN_NONE;
   if (k != nullptr && (k->size(0) != B || k->size(2) != S || k->size(3) != D || k->scalar_type() != q->scalar_type())) Py_RETURN_NONE;
   const at::Tensor* pos = nullptr;
-  int64_t pos_strides[2] = {0, 0};
   if (args[3] != Py_None) {
     if (!THPVariable_CheckExact(args[3])) Py_RETURN_NONE;
     const at::Tensor& p = THPVariable_Unpack(args[3]);
     if (!p.defined() || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong)) Py_RETURN_NONE;
     pos = plain_cuda(args[3], p.scalar_type(), p.dim(), device);
     if (pos == nullptr || (p.dim() != 1 && p.dim() != 2) || p.size(-1) != S || (p.dim() == 2 && p.size(0) != 1 && p.size(0) != B)) Py_RETURN_NONE;
-    pos_strides[0] = p.dim() == 1 || p.size(0) == 1 ? 0 : p.stride(0);
-    pos_strides[1] = p.stride(-1);
   }
-  at::Tensor qo = rows_like(*q), ko;
-  if (k != nullptr) ko = rows_like(*k);
-  int64_t strides[16] = {};
-  copy_strides(strides, *q);
-  copy_strides(strides + 8, qo);
-  if (k != nullptr) {
-    copy_strides(strides + 4, *k);
-    copy_strides(strides + 12, ko);
+  const at::Tensor none;
+  if (records_grad(*q) || (k != nullptr && records_grad(*k))) {
+    torch::autograd::variable_list out;
+    without_gil([&] {
+      out = RotaryFunction::apply(*q, RotaryFunction::given(k != nullptr ? *k : none), *table, RotaryFunction::given(pos != nullptr ? *pos : none), args[4] == Py_True, args[5] == Py_True);
+    });
+    return tensor_pair(out[0], k != nullptr ? out[1] : none);
   }
-  const void* kp = k != nullptr ? k->const_data_ptr() : nullptr;
-  void* kop = k != nullptr ? ko.mutable_data_ptr() : nullptr;
-  const int Hk = k != nullptr ? static_cast<int>(k->size(1)) : 0;
-  void* stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  at::Tensor qo, ko;
   int rc = 0;
-  Py_BEGIN_ALLOW_THREADS
-  rc = g_ops.rotary(q->const_data_ptr(), kp, qo.mutable_data_ptr(), kop, static_cast<int>(B), static_cast<int>(q->size(1)), Hk,
-                    static_cast<int>(S), static_cast<int>(D), strides, static_cast<const float*>(table->const_data_ptr()),
-                    static_cast<int>(table->size(0)), static_cast<int>(R), pos != nullptr ? pos->const_data_ptr() : nullptr,
-                    pos != nullptr && pos->scalar_type() == at::kLong ? 1 : 0, pos != nullptr ? pos_strides : nullptr, args[4] == Py_True,
-                    args[5] == Py_True, dtype_of(*q), stream);
-  Py_END_ALLOW_THREADS
+  without_gil([&] {
+    rc = turn(*q, k != nullptr ? *k : none, *table, pos != nullptr ? *pos : none, args[4] == Py_True, args[5] == Py_True, &qo, &ko);
+  });
   if (rc != 0) return PyLong_FromLong(rc);
   return tensor_pair(std::move(qo), std::move(ko));
   END_HANDLE_TH_ERRORS

@@ -575,7 +575,7 @@ def test_native_and_python_routes_agree(cuda_device, monkeypatch):
         assert torch.equal(a, b) and a.dtype == b.dtype and a.stride() == b.stride()
     # what is not ordinary
     kv, table, n = make(cuda_device, [40, 20], H, D, page, dtype, room=60)
-    assert native.rotary(q.clone().requires_grad_(), k, rope, pos, False, False) is None
+    assert native.rotary(q.clone().requires_grad_(), k, rope, pos, False, False)[0].requires_grad
     assert native.rotary(q, k, rope.double(), pos, False, False) is None and native.rotary(q, k, rope, pos[:, :2], False, False) is None
     assert native.rotary(q[..., ::2], None, rope, None, False, False) is None and native.rotary(q, k.half(), rope, pos, False, False) is None
     assert native.cache4_attention(q, kv, table, n, 1, None, None, False) is None and native.cache4_attention(q, kv, table, n[:1], 0.1, None, None, False) is None

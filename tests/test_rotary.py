@@ -139,9 +139,12 @@ def test_storage_orders(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("route", ["native", "python"])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("R", [64, 24, 10])
-def test_gradient(cuda_device, interleaved, R):
+def test_gradient(cuda_device, monkeypatch, route, interleaved, R):
+    if route == "python":
+        monkeypatch.setattr(ro, "_native", None)
     B, Hq, Hk, S, D = 2, 4, 2, 11, 64
     g = torch.Generator(device=cuda_device).manual_seed(3)
     rand = lambda *s: torch.randn(s, generator=g, device=cuda_device).half()  # noqa: E731
@@ -165,8 +168,16 @@ def test_gradient(cuda_device, interleaved, R):
     a = ro.rotary(q, None, table, pos, interleaved)[0]
     seed = dq.clone().requires_grad_()
     first = torch.autograd.grad(a, q, seed, create_graph=True)[0]
-    again = torch.autograd.grad(first, seed, rand(B, Hq, S, D))[0]
-    assert again.shape == seed.shape and bool(torch.isfinite(again).all())
+    dd = rand(B, Hq, S, D)
+    again = torch.autograd.grad(first, seed, dd)[0]
+    close(again, dd, table, ref.rotary(dd, table, pos, interleaved), torch.float16, pos, interleaved)
+    # gradients that the library cannot read as they are: no strides, columns apart, an unaligned base
+    flat = rand(B * Hq * S * D + 1)[1:].view(B, Hq, S, D)
+    for odd in (rand(1, 1, 1, 1).expand(B, Hq, S, D), rand(B, Hq, D, S).transpose(2, 3), flat):
+        got = torch.autograd.grad(ro.rotary(q, k, table, pos, interleaved)[0], q, odd)[0]
+        close(got, odd, table, ref.rotary(odd, table, pos, interleaved, inverse=True), torch.float16, pos, interleaved, True)
+    with torch.no_grad():
+        assert not ro.rotary(q, k, table, pos, interleaved)[0].requires_grad
 
 
 @pytest.mark.gpu
