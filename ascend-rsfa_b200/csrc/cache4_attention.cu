@@ -156,11 +156,14 @@ __device__ __forceinline__ long long all_units(const Cache4& c, const int* count
 // goes over the CTAs first, so that a few units are spread over all multiprocessors.
 __device__ __forceinline__ long long worker_here() { return static_cast<long long>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; }
 __device__ __forceinline__ long long workers_used(long long total, long long all) { return total < all ? total : all; }
-__device__ __forceinline__ long long share_begin(long long total, long long worker, long long workers) {
-  return total * worker / workers;
+// a / b for a >= 0, b > 0: 32-bit division, a quarter of the instructions, where that is enough.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
 }
+__device__ __forceinline__ long long share_begin(long long total, long long worker, long long workers) { return quotient(total * worker, workers); }
 __device__ __forceinline__ long long worker_of(long long total, long long unit, long long workers) {
-  return ((unit + 1) * workers - 1) / total;
+  return quotient((unit + 1) * workers - 1, total);
 }
 
 // A place in the list: tiles t to end of item `item` of sequence b are the share's.
@@ -221,7 +224,7 @@ __device__ __forceinline__ Cursor cursor_at(const Cache4& c, const int* counts, 
   }
   k.n = tokens_of(c, k.b);
   const int length = k.tiles + cost;
-  k.item = static_cast<int>((from - first) / length);
+  k.item = static_cast<int>(quotient(from - first, length));
   const int unit = static_cast<int>(from - first - static_cast<long long>(k.item) * length);
   const int units = static_cast<int>(min(static_cast<long long>(length - unit), to - from));
   k.at = first - static_cast<long long>(sequences) * per_sequence * cost + static_cast<long long>(k.item) * k.tiles;

@@ -188,24 +188,31 @@ __device__ double frequency(const TableArgs& t, int i) {
   return f;
 }
 
-// One thread: kTableRows positions of one frequency.  The first angle goes through sincos, the others follow by
-// turning in 64 bits: an error of 64 roundings of 2^-53 each, nothing next to the entries' 2^-24.
+// One thread: kTableRows positions of one frequency.  The first angle goes through sincospi, the others follow by
+// turning in 64 bits: an error of 64 roundings of 2^-53 each, nothing next to the entries' 2^-24.  The powers that a frequency
+// takes are worked out once per CTA; with one per thread they took as long as the table's way to memory.
 __global__ void __launch_bounds__(kThreads) rotary_table_kernel(float2* table, const TableArgs t) {
+  __shared__ double turns[128];            // per position, in halves
+  const int half = t.dim >> 1;
+  for (int i = threadIdx.x; i < half; i += kThreads) turns[i] = frequency(t, i) * 0.31830988618379067153776752674503;
+  __syncthreads();
   griddep_launch_dependents();
   griddep_wait();
-  const int half = t.dim >> 1;
   const long long unit = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
   const int block = static_cast<int>(unit / half), i = static_cast<int>(unit - static_cast<long long>(block) * half);
   const long long first = static_cast<long long>(block) * kTableRows;
   if (first >= t.length) return;
-  const double f = frequency(t, i);
+  const double f = turns[i];
   double s, c, ds, dc;
-  sincos(static_cast<double>(first) * f, &s, &c);
-  sincos(f, &ds, &dc);
+  sincospi(static_cast<double>(first) * f, &s, &c);
+  sincospi(f, &ds, &dc);
+  s *= t.multiplier;
+  c *= t.multiplier;
   const int rows = static_cast<int>(min(static_cast<long long>(kTableRows), t.length - first));
   float2* out = table + first * half + i;
   for (int r = 0; r < rows; ++r) {
-    out[static_cast<int64_t>(r) * half] = make_float2(static_cast<float>(c * t.multiplier), static_cast<float>(s * t.multiplier));
+    *out = make_float2(static_cast<float>(c), static_cast<float>(s));
+    out += half;
     const double n = c * dc - s * ds;
     s = s * dc + c * ds;
     c = n;
