@@ -9,7 +9,7 @@
 // word ARE the fp16 number u * 2^-24, one position further up u * 2^-20, and MMAs take subnormal operands as they are;
 // the powers of two come out in the scores' factor and in the accumulators' final one.
 //
-// Rows of scores are handed on by a flash recurrence whose reference is raised only when a score exceeds it by 8
+// Rows of scores are handed on by a flash recurrence whose reference is raised only when a score exceeds it by 13
 // log2 units.  p * s is rounded to fp16 for the second product; p, its sum and the minima's term stay in 32 bits.
 //
 // What bounds it: HBM, 5 D / 4 bytes per token and K/V head, and close behind it the instructions that take the codes
@@ -44,8 +44,11 @@ struct Shape {
 };
 constexpr int kItemCost = 2;         // tiles that an item takes as long as beside its own, see all_units
 constexpr int kTagCache4Load = 40;   // of a bounded wait, in the status word
-constexpr float kRaise = 8.f;        // log2 units above the reference at which it is raised
-constexpr float kRaiseScale = 64.f;  // and the scales' one
+// A reference is set kHeadroom log2 units below its row's largest score and raised when a score is kRaise above it; the
+// scales' unit is raised when one is kRaiseScale of it.  So a product p * s is at most 2^13 * 4 in fp16, whose normal numbers
+// then reach weights of 2^-19 of the largest.
+constexpr float kHeadroom = 5.f, kRaise = 13.f;
+constexpr float kRaiseScale = 4.f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -76,14 +79,12 @@ __device__ __forceinline__ void mma_own(float (&c)[4], uint32_t a0, uint32_t a1,
   else
     mma_f16(c, a0, a1, a2, a3, b0, b1);
 }
-// sum + one half of a pair of fp16 numbers, in one instruction.
-__device__ __forceinline__ float add_low(float sum, uint32_t pair) {
-  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nadd.f32.f16 %0, l, %0;\n}\n" : "+f"(sum) : "r"(pair));
-  return sum;
-}
-__device__ __forceinline__ float add_high(float sum, uint32_t pair) {
-  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nadd.f32.f16 %0, h, %0;\n}\n" : "+f"(sum) : "r"(pair));
-  return sum;
+// Pairs of codes as (u - 8) * 2^-9: as the numbers u * 2^-24 that they are (kUp: u * 2^-20, four bits further up).
+template <bool kUp>
+__device__ __forceinline__ uint32_t centred(uint32_t codes) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(codes), "r"(kUp ? 0x68006800u : 0x78007800u), "r"(0xa400a400u));
+  return r;
 }
 // The low half of a pair, a number of the cache's type, times another such number: conversion and factor in one.
 template <bool kBf16>
@@ -397,15 +398,16 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
   }
 }
 
-// The sums of one piece of an item.  A code u enters the second product as it is, but the rounding of p * s would then
-// show times u: sum p s u + sum p m is taken as sum P u - 8 sum P + sum p (m + 8 s), P = fp16(p s), which leaves it
-// times u - 8, half as much on average.  The last sum (`mids`) comes out of an MMA of its own, whose row w is group w, with
-// p and m + 8 s rounded to the cache's type like the weights and values of any 16-bit attention.
+// The sums of one piece of an item.  sum p s u + sum p m is taken as sum P (u - 8) + sum p (m + 8 s), P = fp16(p s): the
+// rounding of P then shows times u - 8 instead of u, and neither it nor an MMA's own (which cuts its sums off, at 2^-24 of what
+// its operands' exponents allow) comes up against a sum that is mostly the codes' middle.  With u * 2^-24 as the operand
+// here, too, results were off by 4.5e-4 over 60000 tokens, with u - 8 by 2.8e-4 (fp16, whose own rounding is 2.1e-4).
+// The last sum (`mids`) comes out of an MMA of its own, whose row w is group w, with p and m + 8 s rounded to the
+// cache's type like the weights and values of any 16-bit attention.
 template <int D, int NT>
 struct Sums {
   static constexpr int G = D / 32;
-  float o[2 * G][NT][4];       // tile 2 w + t, times 2^-24 over `unit`: dim 32 w + 4 g + 2 t, and that plus 16 times the next
-  float rounded[NT][G][2];     // this lane's share of sum P, rows 2 c, 2 c + 1, over `unit`
+  float o[2 * G][NT][4];       // tile 2 w + t: dims 32 w + 4 g + 2 t and + 1, times 2^-9 over `unit`
   float mids[NT][4];           // sum p (m + 8 s) of group g % G, rows 2 c, 2 c + 1 (twice)
   float l[NT][2], ref[NT][2];
   float unit;                  // power of two that s is divided by
@@ -423,8 +425,6 @@ __device__ __forceinline__ void clear(Sums<D, NT>& x) {
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x.mids[nt][i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < D / 32; ++w) x.rounded[nt][w][0] = x.rounded[nt][w][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < 2 * (D / 32); ++j)
 #pragma unroll
@@ -505,20 +505,21 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
                    transpose_8x8(from_f32x2<kBf16>(p[nt][2], p[nt][3])));
 #pragma unroll
   for (int w = 0; w < G; ++w) {
-    // The half words of group w: low half token 2 c (2 c + 8), high half the token behind it.  A byte is two codes; taken
-    // whole and with the first one alone it needs an operation less than with each by itself.
+    // the half words of group w: low half token 2 c (2 c + 8), high half the token behind it
     const uint32_t pick = (w & 1) ? 0x7632u : 0x5410u;
     const uint32_t y = __byte_perm(v[0][w / 2], v[1][w / 2], pick), z = __byte_perm(v[2][w / 2], v[3][w / 2], pick);
-    const uint32_t y1 = __byte_perm(y, 0u, 0x4341), z1 = __byte_perm(z, 0u, 0x4341);
+    const uint32_t y8 = y >> 8, z8 = z >> 8;
+    const uint32_t ya = centred<false>(y & 0x000f000fu), yb = centred<true>(y & 0x00f000f0u), za = centred<false>(z & 0x000f000fu),
+                   zb = centred<true>(z & 0x00f000f0u);
+    const uint32_t yc = centred<false>(y8 & 0x000f000fu), yd = centred<true>(y8 & 0x00f000f0u), zc = centred<false>(z8 & 0x000f000fu),
+                   zd = centred<true>(z8 & 0x00f000f0u);
     const float sl = scale_of<kBf16>(pl[w], static_cast<uint16_t>(x.per_unit)), sh = scale_of<kBf16>(ph[w], static_cast<uint16_t>(x.per_unit));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint32_t pl2 = from_f32x2<false>(p[nt][0] * sl, p[nt][1] * sl), ph2 = from_f32x2<false>(p[nt][2] * sh, p[nt][3] * sh);
       const uint32_t b0 = transpose_8x8(pl2), b1 = transpose_8x8(ph2);
-      mma_f16(x.o[2 * w][nt], y & 0x000f000fu, y & 0x00ff00ffu, z & 0x000f000fu, z & 0x00ff00ffu, b0, b1);
-      mma_f16(x.o[2 * w + 1][nt], y1 & 0x000f000fu, y1, z1 & 0x000f000fu, z1, b0, b1);
-      x.rounded[nt][w][0] = add_low(add_low(x.rounded[nt][w][0], pl2), ph2);
-      x.rounded[nt][w][1] = add_high(add_high(x.rounded[nt][w][1], pl2), ph2);
+      mma_f16(x.o[2 * w][nt], ya, yb, za, zb, b0, b1);
+      mma_f16(x.o[2 * w + 1][nt], yc, yd, zc, zd, b0, b1);
     }
   }
 }
@@ -545,7 +546,7 @@ __device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2],
       float m = top[nt][i];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      const float ref = m > x.ref[nt][i] + kRaise ? m : x.ref[nt][i];
+      const float ref = m > x.ref[nt][i] + kRaise ? m - kHeadroom : x.ref[nt][i];
       const float by = ex2(x.ref[nt][i] - ref), by_both = by * by_unit;
       x.ref[nt][i] = ref;
       x.l[nt][i] *= by;
@@ -555,8 +556,6 @@ __device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2],
         x.o[j][nt][i] *= by_both;
         x.o[j][nt][i + 2] *= by_both;
       }
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) x.rounded[nt][w][i] *= by_both;
     }
 }
 
@@ -649,33 +648,26 @@ template <int D, int NT, bool kBf16>
 __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention& a, const Rows& rows, int b, int h, int row0, float* piece) {
   constexpr int G = D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-  // codes back from their places in a word, then what p * s was divided by
-  auto low = [&](float v) { return v * 16777216.f * x.unit; };
-  auto high = [&](float first, float both) { return (both - first) * 1048576.f * x.unit; };
+  auto whole = [&](float v) { return v * 512.f * x.unit; };
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      // what goes to every dim of a group: its mids, which lane 4 w + q4 has, without eight times its sum of P
+      // what goes to every dim of a group: its mids, which lane 4 w + q4 has
       float l = x.l[nt][i], m[G];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
 #pragma unroll
-      for (int w = 0; w < G; ++w) {
-        float sum = x.rounded[nt][w][i];
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        m[w] = __shfl_sync(0xffffffffu, x.mids[nt][i], 4 * w + q4) - 8.f * sum * x.unit;
-      }
+      for (int w = 0; w < G; ++w) m[w] = __shfl_sync(0xffffffffu, x.mids[nt][i], 4 * w + q4);
       const int r = 8 * nt + 2 * q4 + i, row = row0 + r;
       if (row < rows.count) {
         if (piece != nullptr) {
           float* dst = piece + r * (D + 2);
 #pragma unroll
           for (int w = 0; w < G; ++w) {
-            *reinterpret_cast<float2*>(dst + 32 * w + 4 * g) = make_float2(low(x.o[2 * w][nt][i]) + m[w], high(x.o[2 * w][nt][i], x.o[2 * w][nt][i + 2]) + m[w]);
+            *reinterpret_cast<float2*>(dst + 32 * w + 4 * g) = make_float2(whole(x.o[2 * w][nt][i]) + m[w], whole(x.o[2 * w][nt][i + 2]) + m[w]);
             *reinterpret_cast<float2*>(dst + 32 * w + 4 * g + 2) =
-                make_float2(low(x.o[2 * w + 1][nt][i]) + m[w], high(x.o[2 * w + 1][nt][i], x.o[2 * w + 1][nt][i + 2]) + m[w]);
+                make_float2(whole(x.o[2 * w + 1][nt][i]) + m[w], whole(x.o[2 * w + 1][nt][i + 2]) + m[w]);
           }
           if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(x.ref[nt][i], l);
         } else {
@@ -685,8 +677,8 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
 #pragma unroll
           for (int w = 0; w < G; ++w)
             *reinterpret_cast<uint2*>(dst + 32 * w + 4 * g) =
-                make_uint2(from_f32x2<kBf16>((low(x.o[2 * w][nt][i]) + m[w]) * inv, (high(x.o[2 * w][nt][i], x.o[2 * w][nt][i + 2]) + m[w]) * inv),
-                           from_f32x2<kBf16>((low(x.o[2 * w + 1][nt][i]) + m[w]) * inv, (high(x.o[2 * w + 1][nt][i], x.o[2 * w + 1][nt][i + 2]) + m[w]) * inv));
+                make_uint2(from_f32x2<kBf16>((whole(x.o[2 * w][nt][i]) + m[w]) * inv, (whole(x.o[2 * w][nt][i + 2]) + m[w]) * inv),
+                           from_f32x2<kBf16>((whole(x.o[2 * w + 1][nt][i]) + m[w]) * inv, (whole(x.o[2 * w + 1][nt][i + 2]) + m[w]) * inv));
           if (g == 0 && a.lse != nullptr)
             a.lse[(static_cast<int64_t>(b) * a.Hq + hq) * a.S + t] = l == 0.f ? -INFINITY : (x.ref[nt][i] + __log2f(l)) * kLn2;
         }
