@@ -9,8 +9,8 @@
 // word ARE the fp16 number u * 2^-24, one position further up u * 2^-20, and MMAs take subnormal operands as they are;
 // the powers of two come out in the scores' factor and in the accumulators' final one.
 //
-// Rows of scores are handed on by a flash recurrence whose reference is raised only when a score exceeds it by 13
-// log2 units.  p * s is rounded to fp16 for the second product; p, its sum and the minima's term stay in 32 bits.
+// Rows of scores are handed on by a flash recurrence whose reference is raised only when a score exceeds what it
+// was set for by a log2 unit.  p * s is rounded to fp16 for the second product; p, its sum and the minima's term stay in 32 bits.
 //
 // What bounds it: HBM, 5 D / 4 bytes per token and K/V head, and close behind it the instructions that take the codes
 // apart.  The work is the list of all tiles of 32 (64) tokens of all (sequence, K/V head, block of query rows), and every warp of
@@ -44,10 +44,12 @@ struct Shape {
 };
 constexpr int kItemCost = 2;         // tiles that an item takes as long as beside its own, see all_units
 constexpr int kTagCache4Load = 40;   // of a bounded wait, in the status word
-// A reference is set kHeadroom log2 units below its row's largest score and raised when a score is kRaise above it; the
-// scales' unit is raised when one is kRaiseScale of it.  So a product p * s is at most 2^13 * 4 in fp16, whose normal numbers
-// then reach weights of 2^-19 of the largest.
-constexpr float kHeadroom = 5.f, kRaise = 13.f;
+// A reference is set kHeadroom log2 units below its row's largest score and raised when a score is kRaise above it, one unit
+// above the largest before; the scales' unit is raised when one is kRaiseScale of it.  So a product p * s is at most 2^11 * 4
+// in fp16, whose normal numbers then reach weights of 2^-24 of the largest, and the largest weights, which are what rounding
+// shows in most, are close to powers of two (8192 and 60000 tokens: results off by 2.4e-4 and 2.5e-4; raised only eight
+// units above: 2.8e-4 and 3.5e-4).
+constexpr float kHeadroom = 10.f, kRaise = 11.f;
 constexpr float kRaiseScale = 4.f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
