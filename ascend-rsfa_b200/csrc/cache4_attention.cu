@@ -25,17 +25,13 @@ namespace {
 constexpr int kWarps = 4;            // per CTA
 constexpr int kThreads = 32 * kWarps;
 constexpr int kJoinThreads = 128, kJoinMost = 512;
-#ifndef C4_CTAS128
-#define C4_CTAS128 3
-#define C4_STAGES128 3
-#endif
 // Tokens per tile: what a tile costs apart from its tokens is spread over 5 KB (10 KB) of them.
 __host__ __device__ constexpr int tile_tokens(int D) { return D == 64 ? 64 : 32; }
 // CTAs per multiprocessor by the registers of their accumulators, and slots of a warp's ring by its shared memory.
 template <int D, int NT>
 struct Shape {
-  static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : C4_CTAS128;
-  static constexpr int kStages = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 4) : C4_STAGES128;
+  static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : 3;
+  static constexpr int kStages = D == 256 ? 2 : NT == 2 && D == 128 ? 4 : 3;
   static constexpr int kTile = tile_tokens(D);
   static constexpr int kPieces = kTile / 16;     // loads per tile: a page holds whole ones
   static constexpr int kPieceBytes = 16 * Record<D>::kBytes;
@@ -225,6 +221,8 @@ __device__ __forceinline__ Cursor cursor_at(const Cache4& c, const int* counts, 
       sequences += __popc(filled);
     }
   }
+  k.item = k.t = k.end = k.left = 0;
+  if (k.b < 0) return k;                // only if the lengths have changed meanwhile
   k.n = tokens_of(c, k.b);
   const int length = k.tiles + cost;
   k.item = static_cast<int>(quotient(from - first, length));
@@ -693,7 +691,8 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
 // as the warp is done with a slot, across the items of its share.
 template <int D, int NT, bool kBf16>
 __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attention_kernel(const Cache4 c, const Cache4Attention a, const Rows rows,
-                                                                                        const int row_blocks, const unsigned long long wait_limit_ns) {
+                                                                                        const int row_blocks, const bool keep, const unsigned long long wait_limit_ns,
+                                                                                        const int test_drop_load) {
   using R = Record<D>;
   using Sh = Shape<D, NT>;
   constexpr int kTile = Sh::kTile;
@@ -726,6 +725,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   uint32_t there = 0;                      // lanes that have a page
   uint32_t have = 0;                       // a bit per piece of every slot: asked for
   constexpr uint32_t kAll = (1u << Sh::kPieces) - 1u;
+  int drop = test_drop_load + 1;
   auto page_of = [&](int piece) {
     const int slot = piece * 16;
     return slot < load.n ? c.table[static_cast<int64_t>(load.b) * c.table_stride + (slot >> c.page_shift)] : -1;
@@ -746,6 +746,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
     const uint32_t asked = (there >> off) & kAll;
     have = (have & ~(kAll << (Sh::kPieces * stage))) | asked << (Sh::kPieces * stage);
     const uint32_t bar = my_bar + 8 * stage;
+    if (--drop == 0) {                     // test hook: neither the load nor the arrival that announces it
+      if (++load.t == load.end) next_item(load, c, a.counts, per_sequence, kItemCost);
+      return;
+    }
     if (lane == 0) mbar_arrive_expect_tx(bar, __popc(asked) * Sh::kPieceBytes);
     const int i = lane - off;
     if (static_cast<unsigned>(i) < Sh::kPieces && ((there >> lane) & 1))
@@ -763,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
   for (int i = 0; i < Sh::kStages && load.t < load.end; ++i) issue(i);
 
   const int score_rows = min(8 * NT, rows.count);     // of a tile; as many as an item has
-  float* const kept = c.weight != nullptr && row_blocks == 1 ? a.scores : nullptr;
+  float* const kept = keep ? a.scores : nullptr;
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -974,7 +978,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
   }
 }
 
-// The same with more rows than one block: the scores are computed again from K, against the rows' log-sum-exp.
+// The same without kept scores (see keeps_scores): they are computed again from K, against the rows' log-sum-exp.
 template <int D, int NT, bool kBf16>
 __global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks) {
   using R = Record<D>;
@@ -1027,6 +1031,25 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cac
   }
 }
 
+// Sixteen query rows at a time where there are more than eight: the cache is read half as often.  At D = 256 the
+// accumulators of sixteen rows leave no room for anything else.
+bool sixteen_rows(int D, int rows) { return D <= 128 && rows > 8; }
+
+// Bytes of the scores of the longest sequences that the table allows.
+size_t score_bytes(const Cache4& c, int rows) {
+  const size_t tiles = static_cast<size_t>(c.B) * c.H * (((static_cast<size_t>(c.max_pages) << c.page_shift) + tile_tokens(c.D) - 1) / tile_tokens(c.D));
+  return tiles * rows * tile_tokens(c.D) * sizeof(float);
+}
+// The scores are kept for the weights where a token's fit beside its record: one block of rows, and no more than half
+// of what the cache itself takes (a table may allow for far longer sequences than there are pages).  Four sequences of
+// 32768 tokens, 8 heads, kept against computed again, us: D = 128, 1 / 8 / 16 rows, 66 / 78 / 122 against 111 / 117 / 133;
+// D = 64, 8 / 16 rows, 63 / 91 against 84 / 91; D = 256, 8 rows, 114 against 157.
+bool keeps_scores(const Cache4& c, int Hq, int S) {
+  const int rows = Hq / c.H * S, block = sixteen_rows(c.D, rows) ? 16 : 8;
+  const size_t cache_bytes = (static_cast<size_t>(c.pages) << c.page_shift) * c.H * (c.D * 5 / 4);
+  return c.weight != nullptr && rows <= block && score_bytes(c, rows) <= cache_bytes / 2;
+}
+
 template <int D, int NT, bool kBf16>
 cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, cudaStream_t stream, long long* launches) {
   Rows rows;
@@ -1035,11 +1058,12 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   const int row_blocks = (rows.count + 8 * NT - 1) / (8 * NT);
   using Sh = Shape<D, NT>;
   const int grid = sm_count * Sh::kCtas;
-  const bool pdl = option_pdl() != 0;
+  const bool pdl = option_pdl() != 0, keep = keeps_scores(c, a.Hq, a.S);
   static std::atomic<unsigned long long> smem_done{0};   // per kernel instantiation, bit per device
   cudaError_t e = set_dynamic_smem_once(smem_done, reinterpret_cast<const void*>(cache4_attention_kernel<D, NT, kBf16>), Sh::kRingBytes);
   if (e != cudaSuccess) return e;
-  e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, kThreads, Sh::kRingBytes, stream, pdl, c, a, rows, row_blocks, option_wait_limit_ns());
+  e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, kThreads, Sh::kRingBytes, stream, pdl, c, a, rows, row_blocks, keep, option_wait_limit_ns(),
+                        option_test_drop_load());
   if (e != cudaSuccess) return e;
   *launches += 1;
   // Where items are cut into many pieces, every row gets a CTA of its own, with a warp for every eight pieces.
@@ -1062,7 +1086,7 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (c.weight != nullptr) {
-    if (row_blocks == 1)
+    if (keep)
       e = launch_persistent(cache4_weight_kernel<tile_tokens(D)>, 8 * sm_count, kThreads, 0, stream, pdl, c, a, rows);
     else
       e = launch_persistent(cache4_weight_again_kernel<D, NT, kBf16>, 4 * sm_count, kThreads, 0, stream, pdl, c, a, rows, row_blocks);
@@ -1070,10 +1094,6 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   }
   return e;
 }
-
-// Sixteen query rows at a time where there are more than eight: the cache is read half as often.  At D = 256 the
-// accumulators of sixteen rows leave no room for anything else.
-bool sixteen_rows(int D, int rows) { return D <= 128 && rows > 8; }
 
 template <int D>
 cudaError_t launch_dim(const Cache4& c, const Cache4Attention& a, int sm_count, cudaStream_t stream, long long* launches) {
@@ -1090,7 +1110,7 @@ template <int D, int NT>
 size_t pieces_bytes(int sm_count) {
   return static_cast<size_t>(sm_count) * Shape<D, NT>::kCtas * kWarps * 2 * piece_floats<D, NT>() * sizeof(float);
 }
-// The pieces, then the kept scores of the longest sequences that the table allows.
+// The pieces, then the kept scores.
 Cache4Workspace cache4_attention_workspace(const Cache4& c, int Hq, int S, int sm_count) {
   const int rows = Hq / c.H * S;
   const bool wide = sixteen_rows(c.D, rows);
@@ -1098,9 +1118,7 @@ Cache4Workspace cache4_attention_workspace(const Cache4& c, int Hq, int S, int s
   w.pieces = c.D == 64    ? (wide ? pieces_bytes<64, 2>(sm_count) : pieces_bytes<64, 1>(sm_count))
              : c.D == 128 ? (wide ? pieces_bytes<128, 2>(sm_count) : pieces_bytes<128, 1>(sm_count))
                           : pieces_bytes<256, 1>(sm_count);
-  const bool one_block = rows <= (wide ? 16 : 8);
-  const size_t tiles = static_cast<size_t>(c.B) * c.H * (((static_cast<size_t>(c.max_pages) << c.page_shift) + tile_tokens(c.D) - 1) / tile_tokens(c.D));
-  w.total = w.pieces + (c.weight != nullptr && one_block ? tiles * rows * tile_tokens(c.D) * sizeof(float) : 0);
+  w.total = w.pieces + (keeps_scores(c, Hq, S) ? score_bytes(c, rows) : 0);
   return w;
 }
 

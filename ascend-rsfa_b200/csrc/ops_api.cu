@@ -32,7 +32,7 @@ int take_cache(const rsfa_cache4* in, rsfa::Cache4* c) {
   int shift = 4;
   while (shift < 10 && (1 << shift) != in->page_size) ++shift;
   if ((1 << shift) != in->page_size) return RSFA_ERR_INVALID_ARGUMENT;      // 16 ... 1024
-  if (static_cast<long long>(in->max_pages) << shift > kMostInt) return RSFA_ERR_TOO_LARGE;
+  if (static_cast<long long>(in->max_pages) << shift > 1LL << 30) return RSFA_ERR_TOO_LARGE;
   const int64_t rows = static_cast<int64_t>(in->page_size);
   const int64_t bytes = rows * (in->head_dim * 5 / 4);
   if (!aligned(in->kv, 16) || (in->kv_stride[0] & 15) != 0 || (in->kv_stride[1] & 15) != 0) return RSFA_ERR_INVALID_ARGUMENT;

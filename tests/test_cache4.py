@@ -366,6 +366,92 @@ def test_attention_over_pages_beyond_32_bits(cuda_device):
     assert bool(torch.isfinite(got).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,H,S,D", [(4, 4, 1, 64), (16, 2, 1, 128), (16, 1, 1, 128), (3, 1, 2, 256), (8, 1, 5, 64)])
+def test_weights_with_a_table_far_wider_than_the_cache(cuda_device, Hq, H, S, D):
+    """The scores are not kept then but computed again."""
+    lengths = [100, S, 333]
+    kv, table, n = make(cuda_device, lengths, H, D, 32, torch.float16, seed=2)
+    wide = torch.full((3, 4096), -1, dtype=torch.int32, device=cuda_device)
+    wide[:, : table.shape[1]] = table
+    q = rows(cuda_device, (3, Hq, S, D), torch.float16, 1, 2.0)
+    before = torch.rand(kv.shape[:3], device=cuda_device)
+    weight = before.clone()
+    o, lse = kc.cache4_attention(q, kv, wide, n, 0.1, weight=weight, want_lse=True)
+    check_attention(o, q, kv, wide, n, 0.1, None, lse, weight, before)
+    fa.device_status()
+
+
+@pytest.mark.gpu
+def test_pages_and_heads_in_any_order_of_storage(cuda_device):
+    dtype, H, D, page = torch.bfloat16, 3, 64, 16
+    plain, table, n = make(cuda_device, [50, 17], H, D, page, dtype)
+    P = plain.shape[0]
+    kv = torch.empty((H, P + 2, page, 80), dtype=torch.uint8, device=cuda_device)[:, 1:P + 1].transpose(0, 1)      # heads outermost, a gap
+    weight = torch.empty((H, 2, P, page), device=cuda_device)[:, 1].transpose(0, 1)
+    position = torch.empty((P, H, 2 * page), dtype=torch.int32, device=cuda_device)[..., page:]
+    kv.copy_(plain), weight.copy_(torch.rand(P, H, page, device=cuda_device)), position.copy_(torch.arange(P * H * page, device=cuda_device).view(P, H, page))
+    q, k = rows(cuda_device, (2, 6, 1, D), dtype, 1), rows(cuda_device, (2, H, 1, D), dtype, 2)
+    dense = [t.contiguous() for t in (kv, weight, position)]
+    pos = torch.tensor([[9000], [9001]], dtype=torch.int32, device=cuda_device)
+    table = torch.stack((table, table), -1).flatten(1)[:, ::2].contiguous() if table.shape[1] > 1 else table
+    rows_of_table = torch.cat((table, table), 1)[:, : table.shape[1]]                                                # a row stride of its own
+    out = []
+    for kv_, w_, p_, t_ in ((kv, weight, position, rows_of_table), (*dense, table)):
+        kc.cache4_append(k, k, kv_, t_, n, weight=w_, position=p_, positions=pos)
+        out.append([kc.cache4_attention(q, kv_, t_, n, 0.1, weight=w_), *kc.cache4_read(kv_, t_, n, 50, dtype), kc.cache4_evict(kv_, w_, p_, t_, n, 20, 3),
+                    kv_.contiguous(), w_.contiguous(), p_.contiguous()])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    fa.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dropped", [0, 1, 5])
+def test_a_wait_that_runs_out_is_reported(cuda_device, dropped):
+    """The loads of every warp's first, second or sixth tile are left out: the kernel returns by itself and says so, and
+    the next call is right.  Nothing is in flight for those tiles.  (15000 tiles: at least eight per warp of 148
+    multiprocessors with twelve each.)"""
+    kv, table, n = make(cuda_device, [60000], 8, 128, 64, torch.float16)
+    q = rows(cuda_device, (1, 8, 1, 128), torch.float16, 1)
+    want = kc.cache4_attention(q, kv, table, n, 0.1)
+    fa.device_status()
+    limit = int(lib.rsfa_get_option(b"wait_limit_ms"))
+    try:
+        fa.set_option("wait_limit_ms", 1)
+        fa.set_option("test_drop_load", dropped)
+        kc.cache4_attention(q, kv, table, n, 0.1)
+        torch.cuda.synchronize()
+    finally:
+        fa.set_option("test_drop_load", -1)
+        fa.set_option("wait_limit_ms", limit)
+    with pytest.raises(RuntimeError, match="device status 0x10028"):
+        fa.device_status()
+    assert torch.equal(kc.cache4_attention(q, kv, table, n, 0.1), want)
+    fa.device_status()
+
+
+@pytest.mark.gpu
+def test_check_status_option_makes_the_next_call_fail(cuda_device):
+    kv, table, n = make(cuda_device, [20], 1, 64, 16, torch.float16)
+    q = rows(cuda_device, (1, 1, 1, 64), torch.float16, 1)
+    rope = ro.rotary_table(4, 64, device=cuda_device)
+    fa.device_status()
+    try:
+        fa.set_option("check_status", 1)
+        kc.cache4_attention(q, kv, table + 1000, n, 0.1)
+        torch.cuda.synchronize()
+        for call in (lambda: kc.cache4_attention(q, kv, table, n, 0.1), lambda: ro.rotary(q, None, rope), lambda: kc.cache4_read(kv, table, n, 4, torch.float16)):
+            with pytest.raises(RuntimeError, match="device status"):
+                call()
+        with pytest.raises(RuntimeError, match="0x20002"):
+            fa.device_status()
+        kc.cache4_attention(q, kv, table, n, 0.1)
+    finally:
+        fa.set_option("check_status", 0)
+    fa.device_status()
+
+
 # ------------------------------------------------------------------ eviction
 
 @pytest.mark.gpu
