@@ -9,28 +9,39 @@
 // word ARE the fp16 number u * 2^-24, one position further up u * 2^-20, and MMAs take subnormal operands as they are;
 // the powers of two come out in the scores' factor and in the accumulators' final one.
 //
-// Rows of scores are handed on by a flash recurrence whose reference is raised only when a score exceeds what it
-// was set for by a log2 unit.  p * s is rounded to fp16 for the second product; p, its sum and the minima's term stay in 32 bits.
+// The second product runs over codes less their middle, u - 8 (exact), and the middles m + 8 s of the groups are a third,
+// small one: what rounding p * s to fp16 leaves is then in proportion to a group's range.  p itself is 32 bits wide where
+// it is summed and added to the weights; for the middles it is rounded to the cache's type.
 //
-// What bounds it: HBM, 5 D / 4 bytes per token and K/V head, and close behind it the instructions that take the codes
-// apart.  The work is the list of all tiles of 32 (64) tokens of all (sequence, K/V head, block of query rows), and every warp of
+// Rows of scores are handed on by a flash recurrence whose reference is raised only when a score exceeds what it
+// was set for by a log2 unit.
+//
+// The work is the list of all tiles of 32 (64) tokens of all (sequence, K/V head, block of query rows), and every warp of
 // the device takes an equal, contiguous share of it, whatever the lengths are.  A share's first and last item may
 // continue in other warps: their sums go to a workspace and a second kernel joins them.
+//
+// What bounds it: not HBM, 5 D / 4 bytes per token and K/V head, but the issue slots right behind it: some 320
+// instructions per 16 tokens, K/V head and 8 rows, most of them to take the codes apart and to bring weights and scales
+// together.  (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist
+// unpacked in registers only.)  Times with 128 dims, against the time for the bytes alone: one sequence of 131072 tokens,
+// 8 heads, 51.6 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 86 us (53); 256 sequences of 200
+// tokens 39 us (11); one sequence of 16 tokens 10.6 us, two dependent kernels of about 5 each.
 #include "../../include/rsfa.h"
 #include "ops_common.cuh"
 
 namespace rsfa {
 namespace {
 
-constexpr int kWarps = 4;            // per CTA
-constexpr int kThreads = 32 * kWarps;
+constexpr int kWeightWarps = 4, kWeightThreads = 32 * kWeightWarps;
 constexpr int kJoinThreads = 128, kJoinMost = 512;
 // Tokens per tile: what a tile costs apart from its tokens is spread over 5 KB (10 KB) of them.
 __host__ __device__ constexpr int tile_tokens(int D) { return D == 64 ? 64 : 32; }
-// CTAs per multiprocessor by the registers of their accumulators, and slots of a warp's ring by its shared memory.
+// One CTA per multiprocessor: as many warps as the registers of their accumulators allow, and slots of a warp's ring by the
+// shared memory that is left.  (Three CTAs of four warps: the same loop, but three times the CTAs to start, 256 sequences of
+// 200 tokens in 48 us for 39.)
 template <int D, int NT>
 struct Shape {
-  static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : 3;
+  static constexpr int kWarps = D == 256 || (NT == 2 && D == 128) ? 8 : 12, kThreads = 32 * kWarps;
   static constexpr int kStages = D == 256 ? 2 : NT == 2 && D == 128 ? 4 : 3;
   static constexpr int kTile = tile_tokens(D);
   static constexpr int kPieces = kTile / 16;     // loads per tile: a page holds whole ones
@@ -133,7 +144,7 @@ __device__ __forceinline__ int tiles_of(const Cache4& c, const int* counts, int 
 }
 // What is divided among the warps: an item of n tiles is n + cost units, cost of them in front for what an item takes by
 // itself (its query rows, its results).  Short items would otherwise make the shares that have many of them the last
-// ones: 64 sequences of 1 to 8192 tokens 103 -> 86 us (94 with a cost of one tile, 85 and 86 with three and four).
+// ones: 64 sequences of 1 to 8192 tokens 103 -> 86 us when it was measured (94 with a cost of one tile, 85 and 86 with three and four).
 //
 // One warp: units of all sequences and of those before b, per K/V head and block of rows.
 __device__ __forceinline__ long long all_units(const Cache4& c, const int* counts, int cost, int b, long long* before) {
@@ -151,19 +162,23 @@ __device__ __forceinline__ long long all_units(const Cache4& c, const int* count
   *before = m;
   return n;
 }
-// Worker w of `workers`, no more than there are units, has the units from share_begin(w) to share_begin(w + 1).  Its number
-// goes over the CTAs first, so that a few units are spread over all multiprocessors.
-__device__ __forceinline__ long long worker_here() { return static_cast<long long>(threadIdx.x >> 5) * gridDim.x + blockIdx.x; }
-__device__ __forceinline__ long long workers_used(long long total, long long all) { return total < all ? total : all; }
 // a / b for a >= 0, b > 0: 32-bit division, a quarter of the instructions, where that is enough.
 __device__ __forceinline__ long long quotient(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
-__device__ __forceinline__ long long share_begin(long long total, long long worker, long long workers) { return quotient(total * worker, workers); }
-__device__ __forceinline__ long long worker_of(long long total, long long unit, long long workers) {
-  return quotient((unit + 1) * workers - 1, total);
-}
+// The units in equal, contiguous shares, one per worker (warp); a few units go to as many workers, one each.  A worker's
+// number goes over the CTAs first, so that those are spread over all multiprocessors.  (Shares by how much a scheduler prefers
+// its first warp to its second and third, 1.56 to 1.73 and 1.86 us per tile, made all of them end together, and later: the
+// multiprocessor is as fast with the last of them alone.)
+struct Shares {
+  long long total;       // units
+  int workers;           // that have any
+  __device__ __forceinline__ Shares(long long units, int all_workers) : total(units), workers(units < all_workers ? static_cast<int>(units) : all_workers) {}
+  __device__ __forceinline__ static int here() { return static_cast<int>(threadIdx.x >> 5) * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x); }
+  __device__ __forceinline__ long long begin(int worker) const { return quotient(total * worker, workers); }
+  __device__ __forceinline__ int of(long long unit) const { return static_cast<int>(quotient((unit + 1) * workers - 1, total)); }
+};
 
 // A place in the list: tiles t to end of item `item` of sequence b are the share's.
 struct Cursor {
@@ -690,29 +705,32 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
 // Every warp works for itself: a ring of tiles in shared memory, which its first lane fills with bulk copies as soon
 // as the warp is done with a slot, across the items of its share.
 template <int D, int NT, bool kBf16>
-__global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attention_kernel(const Cache4 c, const Cache4Attention a, const Rows rows,
+__global__ void __launch_bounds__((Shape<D, NT>::kThreads), 1) cache4_attention_kernel(const Cache4 c, const Cache4Attention a, const Rows rows,
                                                                                         const int row_blocks, const bool keep, const unsigned long long wait_limit_ns,
                                                                                         const int test_drop_load) {
   using R = Record<D>;
   using Sh = Shape<D, NT>;
   constexpr int kTile = Sh::kTile;
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ __align__(8) uint64_t full_bar[kWarps * Sh::kStages];
+  __shared__ __align__(8) uint64_t full_bar[Sh::kWarps * Sh::kStages];
   __shared__ int abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x < kWarps * Sh::kStages) mbar_init(smem_u32(&full_bar[threadIdx.x]), 1);
+  if (threadIdx.x < Sh::kWarps * Sh::kStages) mbar_init(smem_u32(&full_bar[threadIdx.x]), 1);
   if (threadIdx.x == 0) abort_word = 0;
   fence_barrier_init();
   fence_proxy_async();
   __syncthreads();
-  griddep_launch_dependents();
+  // The kernels behind this one read lengths and pages before it is done: they may not start before the ones in front
+  // of it are.
   griddep_wait();
+  griddep_launch_dependents();
   const int per_sequence = c.H * row_blocks;
   long long none;
   const long long total = all_units(c, a.counts, kItemCost, 0, &none) * per_sequence;
-  const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
-  if (worker >= workers) return;
-  Cursor use = cursor_at(c, a.counts, per_sequence, kItemCost, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  const Shares shares(total, gridDim.x * Sh::kWarps);
+  const int worker = shares.here();
+  if (worker >= shares.workers) return;
+  Cursor use = cursor_at(c, a.counts, per_sequence, kItemCost, shares.begin(worker), shares.begin(worker + 1));
   if (use.t >= use.end) return;            // nothing but an item's cost
   Cursor load = use;
   uint8_t* const my_ring = ring + warp * Sh::kStages * Sh::kSlotBytes;
@@ -763,11 +781,10 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
       open_window(window + 32, pages_next);
     }
   };
-#pragma unroll 1
-  for (int i = 0; i < Sh::kStages && load.t < load.end; ++i) issue(i);
 
   const int score_rows = min(8 * NT, rows.count);     // of a tile; as many as an item has
   float* const kept = keep ? a.scores : nullptr;
+  for (int i = 0; i < Sh::kStages && load.t < load.end; ++i) issue(i);
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -807,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
     }
     if (!ok) break;
     float* piece = nullptr;
-    if (t0 > 0 || t1 < tiles) piece = a.pieces + (worker * 2 + (t0 == 0)) * piece_floats<D, NT>();
+    if (t0 > 0 || t1 < tiles) piece = a.pieces + (worker * 2ll + (t0 == 0)) * piece_floats<D, NT>();
     store_sums<D, NT, kBf16>(x, a, rows, b, h, row0, piece);
     next_item(use, c, a.counts, per_sequence, kItemCost);
   }
@@ -825,16 +842,14 @@ __global__ void __launch_bounds__(kThreads, (Shape<D, NT>::kCtas)) cache4_attent
 // answers for items without tokens.  The pieces are taken in an order that does not depend on timing.
 template <int D, int NT, bool kBf16>
 __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks,
-                                                                const long long all_workers, const int rows_each) {
+                                                                const int all_workers, const int rows_each) {
   constexpr int kEach = D / 32;
   __shared__ float part[kJoinMost / 32][D];
   __shared__ float2 sums[kJoinMost / 32];
-  griddep_launch_dependents();
-  griddep_wait();
   const int item = blockIdx.x % (c.H * row_blocks), b = blockIdx.x / (c.H * row_blocks), h = item / row_blocks;
   const int from = blockIdx.y * rows_each, row0 = (item - h * row_blocks) * 8 * NT + from;
   const int count = min(min(rows_each, 8 * NT - from), rows.count - row0);   // rows of this CTA
-  if (count <= 0) return;
+  if (count <= 0) return;        // (the kernel behind this one waits for the whole grid all the same)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int tiles = tiles_of(c, a.counts, b);
   auto answer = [&](int row, int64_t* at_lse) {
@@ -843,6 +858,8 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
     return static_cast<uint16_t*>(a.o) + b * a.o_stride[0] + hq * a.o_stride[1] + t * a.o_stride[2];
   };
   if (tiles == 0) {
+    griddep_wait();
+    griddep_launch_dependents();
     for (int r = warp; r < count; r += warps) {
       int64_t at_lse;
       uint16_t* dst = answer(row0 + r, &at_lse);
@@ -854,9 +871,12 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
   const int per_sequence = c.H * row_blocks;
   long long before;
   const long long total = all_units(c, a.counts, kItemCost, b, &before) * per_sequence;
-  const long long workers = workers_used(total, all_workers);
+  const Shares shares(total, all_workers);
   const long long first = before * per_sequence + static_cast<long long>(item) * (tiles + kItemCost) + kItemCost;   // unit of its first tile
-  const long long w0 = worker_of(total, first, workers), w1 = worker_of(total, first + tiles - 1, workers);
+  // lengths were there before the first kernel started, its pieces are now
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long w0 = shares.of(first), w1 = shares.of(first + tiles - 1);
   if (w0 == w1) return;                       // in one piece: answered already
   const int pieces = static_cast<int>(w1 - w0) + 1;
   // the warps in teams, one per row, as far as they go
@@ -927,15 +947,16 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
 // one warp, so nothing is added twice at once and the order is fixed.  This one reads the scores that the attention
 // kernel has kept, 4 bytes per row and token: 32 tokens per warp at a time, one per lane.
 template <int kTile>
-__global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c, const Cache4Attention a, const Rows rows) {
+__global__ void __launch_bounds__(kWeightThreads) cache4_weight_kernel(const Cache4 c, const Cache4Attention a, const Rows rows) {
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31;
   long long none;
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
-  const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
-  if (worker >= workers) return;
-  Cursor k = cursor_at(c, a.counts, c.H, 0, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  const Shares shares(total, gridDim.x * kWeightWarps);
+  const int worker = shares.here();
+  if (worker >= shares.workers) return;
+  Cursor k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
   const int mask = (1 << c.page_shift) - 1;
   while (k.t < k.end) {
     // log-sum-exps of the item's rows, one per lane (there are no more than 16)
@@ -980,7 +1001,7 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_kernel(const Cache4 c,
 
 // The same without kept scores (see keeps_scores): they are computed again from K, against the rows' log-sum-exp.
 template <int D, int NT, bool kBf16>
-__global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks) {
+__global__ void __launch_bounds__(kWeightThreads) cache4_weight_again_kernel(const Cache4 c, const Cache4Attention a, const Rows rows, const int row_blocks) {
   using R = Record<D>;
   constexpr int kTile = tile_tokens(D);
   griddep_launch_dependents();
@@ -988,9 +1009,10 @@ __global__ void __launch_bounds__(kThreads) cache4_weight_again_kernel(const Cac
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   long long none;
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
-  const long long worker = worker_here(), workers = workers_used(total, static_cast<long long>(gridDim.x) * kWarps);
-  if (worker >= workers) return;
-  Cursor k = cursor_at(c, a.counts, c.H, 0, share_begin(total, worker, workers), share_begin(total, worker + 1, workers));
+  const Shares shares(total, gridDim.x * kWeightWarps);
+  const int worker = shares.here();
+  if (worker >= shares.workers) return;
+  Cursor k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
   const int mask = (1 << c.page_shift) - 1;
   while (k.t < k.end) {
     const int run = k.end - k.t;
@@ -1057,18 +1079,18 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   rows.count = rows.group * a.S;
   const int row_blocks = (rows.count + 8 * NT - 1) / (8 * NT);
   using Sh = Shape<D, NT>;
-  const int grid = sm_count * Sh::kCtas;
+  const int grid = sm_count;
   const bool pdl = option_pdl() != 0, keep = keeps_scores(c, a.Hq, a.S);
   static std::atomic<unsigned long long> smem_done{0};   // per kernel instantiation, bit per device
   cudaError_t e = set_dynamic_smem_once(smem_done, reinterpret_cast<const void*>(cache4_attention_kernel<D, NT, kBf16>), Sh::kRingBytes);
   if (e != cudaSuccess) return e;
-  e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, kThreads, Sh::kRingBytes, stream, pdl, c, a, rows, row_blocks, keep, option_wait_limit_ns(),
+  e = launch_persistent(cache4_attention_kernel<D, NT, kBf16>, grid, Sh::kThreads, Sh::kRingBytes, stream, pdl, c, a, rows, row_blocks, keep, option_wait_limit_ns(),
                         option_test_drop_load());
   if (e != cudaSuccess) return e;
   *launches += 1;
   // Where items are cut into many pieces, every row gets a CTA of its own, with a warp for every eight pieces.
   const int items = c.B * c.H * row_blocks;
-  const long long pieces = static_cast<long long>(grid) * kWarps / items;
+  const long long pieces = static_cast<long long>(grid) * Sh::kWarps / items;
   const bool many_pieces = pieces > 8;
   const int rows_each = many_pieces ? 1 : 8 * NT;
   int join_threads = kJoinThreads;
@@ -1082,14 +1104,14 @@ cudaError_t launch_one(const Cache4& c, const Cache4Attention& a, int sm_count, 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, cache4_join_kernel<D, NT, kBf16>, c, a, rows, row_blocks, static_cast<long long>(grid) * kWarps, rows_each);
+  e = cudaLaunchKernelEx(&cfg, cache4_join_kernel<D, NT, kBf16>, c, a, rows, row_blocks, grid * Sh::kWarps, rows_each);
   if (e != cudaSuccess) return e;
   *launches += 1;
   if (c.weight != nullptr) {
     if (keep)
-      e = launch_persistent(cache4_weight_kernel<tile_tokens(D)>, 8 * sm_count, kThreads, 0, stream, pdl, c, a, rows);
+      e = launch_persistent(cache4_weight_kernel<tile_tokens(D)>, 8 * sm_count, kWeightThreads, 0, stream, pdl, c, a, rows);
     else
-      e = launch_persistent(cache4_weight_again_kernel<D, NT, kBf16>, 4 * sm_count, kThreads, 0, stream, pdl, c, a, rows, row_blocks);
+      e = launch_persistent(cache4_weight_again_kernel<D, NT, kBf16>, 4 * sm_count, kWeightThreads, 0, stream, pdl, c, a, rows, row_blocks);
     if (e == cudaSuccess) *launches += 1;
   }
   return e;
@@ -1108,7 +1130,7 @@ cudaError_t launch_dim(const Cache4& c, const Cache4Attention& a, int sm_count, 
 
 template <int D, int NT>
 size_t pieces_bytes(int sm_count) {
-  return static_cast<size_t>(sm_count) * Shape<D, NT>::kCtas * kWarps * 2 * piece_floats<D, NT>() * sizeof(float);
+  return static_cast<size_t>(sm_count) * Shape<D, NT>::kWarps * 2 * piece_floats<D, NT>() * sizeof(float);
 }
 // The pieces, then the kept scores.
 Cache4Workspace cache4_attention_workspace(const Cache4& c, int Hq, int S, int sm_count) {
