@@ -945,11 +945,12 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
 
 // The weights: every token's softmax weights over all query rows of its K/V head, added to weight[].  A token belongs to
 // one warp, so nothing is added twice at once and the order is fixed.  This one reads the scores that the attention
-// kernel has kept, 4 bytes per row and token: 32 tokens per warp at a time, one per lane.
+// kernel has kept, 4 bytes per row and token: 128 tokens per warp at a time, four per lane.  What bounds it is how much of
+// that is on its way at once: 2 sequences of 131072 tokens, 8 heads of 8 rows, 18 us (67 MB of scores, mostly from L2, and
+// 17 of weights: 4.7 TB/s; 4 bytes per load and page numbers looked up when they are needed: 29 us).
 template <int kTile>
 __global__ void __launch_bounds__(kWeightThreads) cache4_weight_kernel(const Cache4 c, const Cache4Attention a, const Rows rows) {
   griddep_launch_dependents();
-  griddep_wait();
   const int lane = threadIdx.x & 31;
   long long none;
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
@@ -957,6 +958,7 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_kernel(const Cac
   const int worker = shares.here();
   if (worker >= shares.workers) return;
   Cursor k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
+  griddep_wait();          // lengths were there before the first kernel started
   const int mask = (1 << c.page_shift) - 1;
   while (k.t < k.end) {
     // log-sum-exps of the item's rows, one per lane (there are no more than 16)
@@ -966,34 +968,46 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_kernel(const Cac
       lse = a.lse[(static_cast<int64_t>(k.b) * a.Hq + hq) * a.S + t] * kLog2e;
       if (lse == -INFINITY) lse = 0.f;                         // a row that sees nothing: its scores are -inf
     }
-    const int run = k.end - k.t;
-    // 32 tokens are a group; the loads of four groups go out together
-    constexpr int kGroups = 4, kPerTile = kTile / 32;
-    for (int i = 0; i < run * kPerTile; i += kGroups) {
-      const float* scores[kGroups];
-      float* weight[kGroups];
-      float sum[kGroups], old[kGroups];
+    // 32 tokens are a group, four of them neighbouring tokens of a lane; four groups at a time, and the page numbers of the
+    // four behind them
+    constexpr int kPerTile = kTile / 32, kRows = 4;
+    const int groups = (k.end - k.t) * kPerTile, own = lane >> 3, quad = 4 * (lane & 7);
+    auto slot_of = [&](int i) { return k.t * kTile + 32 * (i + own) + quad; };
+    auto page_of = [&](int i) {
+      const int slot = slot_of(i);
+      return i + own < groups && slot < k.n ? c.table[k.b * c.table_stride + (slot >> c.page_shift)] : 0;
+    };
+    int next_page = page_of(0);
+    for (int i = 0; i < groups; i += 4) {
+      const int g = min(i + own, groups - 1), slot = slot_of(i), page = next_page;
+      const float* scores = a.scores + (k.at + k.t + g / kPerTile) * rows.count * kTile + g % kPerTile * 32 + quad;
+      int live = i + own < groups ? min(max(k.n - slot, 0), 4) : 0;
+      if (page < 0 || page >= c.pages) {
+        report_bad_index(c.status, kTagCachePage);
+        live = 0;
+      }
+      float* weight = c.weight + page * c.weight_stride[0] + k.item * c.weight_stride[1] + (slot & mask);
+      float old[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) {
-        const int g = min(i + j, run * kPerTile - 1), tile = g / kPerTile, part = g % kPerTile * 32;
-        scores[j] = a.scores + (k.at + k.t + tile) * rows.count * kTile + part + lane;
-        const int slot = (k.t + tile) * kTile + part + lane;
-        int64_t page;
-        const bool ours = i + j < run * kPerTile && slot < k.n && find_page(c, k.b, slot, &page);
-        weight[j] = ours ? c.weight + page * c.weight_stride[0] + k.item * c.weight_stride[1] + (slot & mask) : nullptr;
-        sum[j] = 0.f;
+      for (int j = 0; j < 4; ++j) old[j] = j < live ? weight[j] : 0.f;
+      if (i + 4 < groups) next_page = page_of(i + 4);
+      for (int r0 = 0; r0 < rows.count; r0 += kRows) {
+        float4 v[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          v[r] = r0 + r < rows.count ? *reinterpret_cast<const float4*>(scores + (r0 + r) * kTile) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const float of_row = __shfl_sync(0xffffffffu, lse, r0 + r);
+          sum[0] += ex2(v[r].x - of_row);
+          sum[1] += ex2(v[r].y - of_row);
+          sum[2] += ex2(v[r].z - of_row);
+          sum[3] += ex2(v[r].w - of_row);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) old[j] = weight[j] != nullptr ? *weight[j] : 0.f;
-#pragma unroll 4
-      for (int r = 0; r < rows.count; ++r) {
-        const float of_row = __shfl_sync(0xffffffffu, lse, r);
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) sum[j] += ex2(scores[j][r * kTile] - of_row);
-      }
-#pragma unroll
-      for (int j = 0; j < kGroups; ++j)
-        if (weight[j] != nullptr) *weight[j] = old[j] + sum[j];
+      for (int j = 0; j < 4; ++j)
+        if (j < live) weight[j] = old[j] + sum[j];
     }
     next_item(k, c, a.counts, c.H, 0);
   }
@@ -1005,7 +1019,6 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_again_kernel(con
   using R = Record<D>;
   constexpr int kTile = tile_tokens(D);
   griddep_launch_dependents();
-  griddep_wait();
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   long long none;
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
@@ -1013,6 +1026,7 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_again_kernel(con
   const int worker = shares.here();
   if (worker >= shares.workers) return;
   Cursor k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
+  griddep_wait();          // lengths were there before the first kernel started
   const int mask = (1 << c.page_shift) - 1;
   while (k.t < k.end) {
     const int run = k.end - k.t;
