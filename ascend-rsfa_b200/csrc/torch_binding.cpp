@@ -1,9 +1,10 @@
-// The ordinary calls of attention() and of the operators around it from PyTorch in native code.  attention(): check the tensors, allocate the result, find the
-// current stream, call rsfa_fwd.  The same steps in Python (flash_attention_forward.py, _forward) take 10 us of
-// the host's time per call, three times what the launch itself takes, which is what a call of a few heads or
-// of a short sequence costs its caller; here they take about 1.5 us.
+// The ordinary calls of attention() and of the operators around it (rotary.py, kv_cache.py) from PyTorch in native code:
+// check the tensors, allocate the results and the scratch, find the current stream, call the library.  attention():
+// the same steps in Python (flash_attention_forward.py, _forward) take 10 us of the host's time per call, three times what
+// the launch itself takes, which is what a call of a few heads or of a short sequence costs its caller; here they take
+// about 1.5 us.
 //
-// forward() answers only for the ordinary case and returns None for everything else - tensors to copy first,
+// A function here answers only for the ordinary case and returns None for everything else - tensors to copy first,
 // empty ones, another device than the current one, subclasses, dispatch or function modes, transforms,
 // tracing, argument types other than the plain ones, anything to refuse - and the Python code decides then.
 // So nothing is accepted, refused or seen by a mode differently than without this file.

@@ -135,9 +135,9 @@ RSFA_API int rsfa_fwd_noalloc(const void* q, const void* k, const void* v, void*
  * is made outside stream capture) and keep nothing from one call for the next; scratch is the
  * caller's, and a scratch buffer belongs to one call at a time.  What lies in device memory cannot
  * be checked when a call is made: a kernel that finds a position, page number or length out of range
- * touches nothing outside, goes on (the results of that sequence have no meaning) and leaves (2 << 16) | tag in the status word (rsfa_device_status): tag
- * 1 a position outside the rotary table, 2 a page outside the cache, 3 a length below zero or beyond the
- * sequence's pages.
+ * touches nothing outside, goes on (the results of that sequence have no meaning) and leaves
+ * (2 << 16) | tag in the status word (rsfa_device_status): tag 1 a position outside the rotary table, 2 a
+ * page outside the cache, 3 a length below zero or beyond the sequence's pages.
  */
 
 /* How the angles of rotary positions are scaled for contexts longer than those of training. */
@@ -178,8 +178,9 @@ RSFA_API int rsfa_rotary(const void* q, const void* k, void* q_out, void* k_out,
  * head_dim / 2 of K codes, as many of V codes, then for K and for V a (scale, minimum) pair of `dtype` per group of
  * 32 dims; a value is scale * code + minimum.  The order of the codes is the kernels' own (csrc/ops_common.cuh).
  * head_dim 64, 128 or 256; page_size a power of two, 16 ... 1024; kv 16-byte aligned, its strides (bytes: page, head)
- * multiples of 16, a head's rows of a page contiguous; max_pages * page_size no more than 2^30.  weight (fp32) and position (int32), one per record with element
- * strides (page, head), are NULL where a call does not use them.  Sequences may share pages that a call only reads.
+ * multiples of 16, a head's rows of a page contiguous; max_pages * page_size no more than 2^30.  weight (fp32) and
+ * position (int32), one per record with element strides (page, head), are NULL where a call does not use them.
+ * Sequences may share pages that a call only reads.
  */
 typedef struct rsfa_cache4 {
   void* kv;
@@ -214,7 +215,8 @@ RSFA_API int rsfa_cache4_read(const rsfa_cache4* cache, void* k, void* v, int N,
  * K/V head h serves the query heads h * q_heads / heads ... .  o like q, both of cache->dtype; a row that sees nothing
  * (a sequence of length zero, a row of padding) is zero, its lse -infinity.  lse: [B,q_heads,S] fp32, natural log, may
  * be NULL unless cache->weight is given: weight[slot] then grows by the softmax weights that the token gets from all
- * query rows of its K/V head (and no page belongs to two sequences).  Results do not depend on timing.  strides: 8 element strides, q[4], o[4].
+ * query rows of its K/V head (and no page belongs to two sequences).  Results do not depend on timing.
+ * strides: 8 element strides, q[4], o[4].
  * workspace: rsfa_cache4_attention_workspace bytes (or a negative error), 16-byte aligned, no content asked for; with
  * weight it holds the scores, up to half the size of the cache.
  */
@@ -271,8 +273,8 @@ RSFA_API int rsfa_sm_count(int device);
  * Synchronise `device` and return the status word its kernels share (this call allocates nothing
  * and reads only the scratch that rsfa_fwd or rsfa_fwd_noalloc has already set up on the device): RSFA_OK, or
  * RSFA_ERR_DEVICE_STATUS with the raw word in *raw (if not NULL): (1 << 16) | tag, where tag names
- * the wait that ran out, or (2 << 16) | tag, see above, for an index out of range.  Reading clears the word.  rsfa_fwd itself returns RSFA_OK for a call
- * whose kernel later gives up (the launch is asynchronous) and the output of that call is then
+ * the wait that ran out (40: a load of rsfa_cache4_attention), or (2 << 16) | tag, see above, for an
+ * index out of range.  Reading clears the word.  rsfa_fwd itself returns RSFA_OK for a call whose kernel later gives up (the launch is asynchronous) and the output of that call is then
  * incomplete: callers that care call this function at their synchronisation points, or set the
  * "check_status" option, under which every rsfa_fwd copies the word to the host behind its kernels
  * and the next rsfa_fwd on that device returns RSFA_ERR_DEVICE_STATUS without launching once a
@@ -296,7 +298,8 @@ RSFA_API long long rsfa_launch_count(void);
  * "check_status" (0 / 1, see rsfa_device_status), "test_drop_load" (-1 = off; n >= 0: every CTA of the
  * 128-key tcgen05 kernel leaves out its n-th K/V tile load and the barrier arrival that announces it, and
  * the kernel for a single key tile, of the loads that it starts with, those of the heads from n on (of B * H),
- * and every warp of rsfa_cache4_attention its n-th tile of the cache, so that a bounded wait runs out - for tests of the wait-expired path; the output of such a call is incomplete).
+ * and every warp of rsfa_cache4_attention its n-th tile of the cache, so that a bounded wait runs out - for
+ * tests of the wait-expired path; the output of such a call is incomplete).
  * rsfa_get_option also answers "workspace_devices": the number of devices on which rsfa_fwd has
  * created its workspace (0 in a process that has only used rsfa_fwd_noalloc).
  * Unknown names -> RSFA_ERR_INVALID_ARGUMENT.
