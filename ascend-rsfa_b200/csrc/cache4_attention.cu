@@ -133,6 +133,10 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// The kernels behind the attention kernel read lengths and counts ahead of their wait for it.  What wrote these is complete, the
+// attention kernel has waited for it; the fence is there so that this multiprocessor's L1 has no older copy of them.
+__device__ __forceinline__ void fence_ahead() { __threadfence(); }
+
 // ------------------------------------------------------------------ the list of tiles
 // Items are (sequence, K/V head, block of query rows) in this order, an item's tiles follow one another.
 __device__ __forceinline__ int visible_tokens(const Cache4& c, const int* counts, int b) {
@@ -287,7 +291,7 @@ __device__ __forceinline__ void load_query(Query<D, NT>& f, const Cache4& c, con
       const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + hq * a.q_stride[1] + i * a.q_stride[2] + 8 * q4;
 #pragma unroll
       for (int w = 0; w < G; ++w) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + 32 * w));
+        const uint4 v = *reinterpret_cast<const uint4*>(src + 32 * w);
         const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -846,6 +850,7 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
   constexpr int kEach = D / 32;
   __shared__ float part[kJoinMost / 32][D];
   __shared__ float2 sums[kJoinMost / 32];
+  fence_ahead();
   const int item = blockIdx.x % (c.H * row_blocks), b = blockIdx.x / (c.H * row_blocks), h = item / row_blocks;
   const int from = blockIdx.y * rows_each, row0 = (item - h * row_blocks) * 8 * NT + from;
   const int count = min(min(rows_each, 8 * NT - from), rows.count - row0);   // rows of this CTA
@@ -951,6 +956,7 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
 template <int kTile>
 __global__ void __launch_bounds__(kWeightThreads) cache4_weight_kernel(const Cache4 c, const Cache4Attention a, const Rows rows) {
   griddep_launch_dependents();
+  fence_ahead();
   const int lane = threadIdx.x & 31;
   long long none;
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
@@ -1019,6 +1025,7 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_again_kernel(con
   using R = Record<D>;
   constexpr int kTile = tile_tokens(D);
   griddep_launch_dependents();
+  fence_ahead();
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   long long none;
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;

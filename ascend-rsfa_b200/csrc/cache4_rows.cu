@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
     for (int i = 0; i < kAppendAtOnce; ++i) {
       const bool any = t0 + i * k.step + k.sub < to;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) next[i][j] = any ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < 2; ++j) next[i][j] = any ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0, 0, 0, 0);
       src += step_bytes;
     }
   };

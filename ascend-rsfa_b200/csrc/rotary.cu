@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, 
         if (h + i < h1) {
           const uint16_t* src;
           address(h + i, &src, &dst[i]);
-          a[i] = __ldg(reinterpret_cast<const uint4*>(src));
-          if (!kInterleaved && turns) c[i] = __ldg(reinterpret_cast<const uint4*>(src + half));
+          a[i] = *reinterpret_cast<const uint4*>(src);
+          if (!kInterleaved && turns) c[i] = *reinterpret_cast<const uint4*>(src + half);
         }
       }
 #pragma unroll
