@@ -10,6 +10,7 @@
 namespace {
 
 constexpr long long kMostInt = 2147483647LL;
+constexpr double kMostTiles = 1099511627776.0;   // 2^40, over a thousand warps of a B200 and more
 
 bool valid_dtype(int dtype) { return dtype == RSFA_DTYPE_F16 || dtype == RSFA_DTYPE_BF16; }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -218,6 +219,9 @@ int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, floa
   if (!valid_tensor(q, strides, c.B, q_heads, S, c.D) || !valid_tensor(o, strides + 4, c.B, q_heads, S, c.D)) return RSFA_ERR_INVALID_ARGUMENT;
   if (!aligned(lse, 4) || !aligned(counts, 4) || (c.weight != nullptr && lse == nullptr)) return RSFA_ERR_INVALID_ARGUMENT;
   if (static_cast<double>(c.B) * q_heads * S > static_cast<double>(kMostInt)) return RSFA_ERR_TOO_LARGE;
+  // a warp's share of all tiles (of 32 tokens or more, for 8 query rows or more) is counted in 32 bits
+  const double tiles = std::ceil(static_cast<double>(c.max_pages) * (1 << c.page_shift) / 32.0) + 2.0;
+  if (c.B * std::ceil(static_cast<double>(q_heads / c.H) * S / 8.0) * c.H * tiles > kMostTiles) return RSFA_ERR_TOO_LARGE;
   rsfa::CallScratch d;
   rc = rsfa::begin_call(&d);
   if (rc != RSFA_OK) return rc;

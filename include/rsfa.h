@@ -217,6 +217,7 @@ RSFA_API int rsfa_cache4_read(const rsfa_cache4* cache, void* k, void* v, int N,
  * be NULL unless cache->weight is given: weight[slot] then grows by the softmax weights that the token gets from all
  * query rows of its K/V head (and no page belongs to two sequences).  Results do not depend on timing.
  * strides: 8 element strides, q[4], o[4].
+ * At most 2^40 tiles of 32 tokens for 8 query rows, counted by max_pages, else RSFA_ERR_TOO_LARGE.
  * workspace: rsfa_cache4_attention_workspace bytes (or a negative error), 16-byte aligned, no content asked for; with
  * weight it holds the scores, up to half the size of the cache.
  */

@@ -128,6 +128,13 @@ def test_c_refusals_need_no_device():
     assert lib.rsfa_cache4_attention_workspace(c_cache(head_dim=48), 2, 1) == bad and lib.rsfa_cache4_attention_workspace(c, 3, 1) == bad
 
 
+def test_more_tiles_than_are_counted_are_refused():
+    # 2^20 sequences of up to 2^30 slots that share their pages: 2^25 tiles of each of 2 heads
+    p, st = ctypes.c_void_p(4096), (ctypes.c_int64 * 8)(*([512, 256, 64, 1] * 2))
+    c = c_cache(batch=1 << 20, max_pages=1 << 26, table_stride=0, weight=None)
+    assert lib.rsfa_cache4_attention(c, p, p, p, 2, 4, st, None, 0.5, p, 1 << 62, None) == _capi.RSFA_ERR_TOO_LARGE
+
+
 def test_oracle_record_round_trip():
     for dtype in DTYPES:
         for D in (64, 128, 256):
