@@ -25,7 +25,6 @@ from .rotary import _call, _ordinary, _readable, _rows
 
 _lib = _capi.load()
 _HEAD_DIMS = (64, 128, 256)
-_workspace_bytes = {}
 
 
 def _strides(*tensors):
@@ -141,6 +140,17 @@ def cache4_read(kv, table, lengths, n, dtype, starts=None):
     return k, v
 
 
+class _without_gradient(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, kv, table, lengths, sm_scale, counts, weight):
+        return cache4_attention(q.detach(), kv, table, lengths, sm_scale, counts=counts, weight=weight, want_lse=True)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError("cache4_attention() has no gradient")
+
+
 def cache4_attention(q, kv, table, lengths, sm_scale, counts=None, weight=None, want_lse=False):
     """Attention of the sequences' last tokens over the cache: o like q [B, Hq, S, D], or (o, lse).
 
@@ -148,8 +158,11 @@ def cache4_attention(q, kv, table, lengths, sm_scale, counts=None, weight=None, 
     has been appended before.  Hq is a multiple of the cache's heads: head h serves query heads h * Hq / heads ... .
     Rows that see nothing - a sequence of length 0, padding behind counts[b] - are zero with an lse of -inf.
     weight: grows, per token and K/V head, by the softmax weights that all query rows of that head give the token.
-    lse: [B, Hq, S] fp32, m + log(l).  There is no gradient.
+    lse: [B, Hq, S] fp32, m + log(l).  There is no gradient: a backward pass that reaches the call raises.
     """
+    if torch.is_grad_enabled() and q.requires_grad:
+        o, lse = _without_gradient.apply(q, kv, table, lengths, sm_scale, counts, weight)
+        return (o, lse) if want_lse else o
     done = _ordinary("cache4_attention", q, kv, table, lengths, sm_scale, counts, weight, want_lse)
     if done is not None:
         return done if want_lse else done[0]
@@ -167,16 +180,10 @@ def cache4_attention(q, kv, table, lengths, sm_scale, counts=None, weight=None, 
     qd = _readable(q)
     o = _rows(qd)
     lse = torch.empty((B, Hq, S), dtype=torch.float32, device=q.device) if want_lse or weight is not None else None
-    key = (D, Hq // c.heads * S, kv.device.index, 0 if weight is None else B * c.heads * c.page_size * c.max_pages)
-    nbytes = _workspace_bytes.get(key)
-    if nbytes is None:
-        with torch.cuda.device(kv.device):
-            nbytes = _lib.rsfa_cache4_attention_workspace(ctypes.byref(c), Hq, S)
-        if nbytes < 0:
-            _capi.check(nbytes, "rsfa_cache4_attention_workspace")
-        if len(_workspace_bytes) > 256:
-            _workspace_bytes.clear()
-        _workspace_bytes[key] = nbytes
+    with torch.cuda.device(kv.device):
+        nbytes = _lib.rsfa_cache4_attention_workspace(ctypes.byref(c), Hq, S)
+    if nbytes < 0:
+        _capi.check(nbytes, "rsfa_cache4_attention_workspace")
     # the call's own scratch, from the pool of the current stream or of the graph that is being captured
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     _call(kv.device, "rsfa_cache4_attention", _lib.rsfa_cache4_attention, ctypes.byref(c), qd.data_ptr(), o.data_ptr(),

@@ -676,3 +676,31 @@ def test_native_and_python_routes_agree(cuda_device, monkeypatch):
     assert native.cache4_append(k, k, kv, table, n, None, None, None, pos) is None and native.cache4_append(q, q, kv, table, n, None, None, None, None) is None
     assert native.cache4_read(kv, table, n, 0, True, None) is None and native.cache4_read(kv, table.long(), n, 4, True, None) is None
     assert native.cache4_evict(kv, None, None, table, n, 4, 2) is None
+
+
+@pytest.mark.gpu
+def test_a_backward_pass_through_the_attention_raises(cuda_device):
+    kv, table, lengths = make(cuda_device, [40], 1, 64, 16, torch.float16)
+    q = rows(cuda_device, (1, 2, 1, 64), torch.float16, 7)
+    want = kc.cache4_attention(q, kv, table, lengths, 0.125, want_lse=True)
+    got = kc.cache4_attention(q.requires_grad_(), kv, table, lengths, 0.125, want_lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and torch.equal(kc.cache4_attention(q, kv, table, lengths, 0.125), want[0])
+    with pytest.raises(NotImplementedError):
+        got[0].sum().backward()
+    with torch.no_grad():
+        assert not kc.cache4_attention(q, kv, table, lengths, 0.125).requires_grad
+
+
+@pytest.mark.gpu
+def test_scratch_is_sized_for_every_call(cuda_device):
+    """The same number of slots as one sequence of two pages and as two of one page, which are different numbers of tiles; a
+    table that is not contiguous, so both calls take the Python route."""
+    for lengths in ([30], [16, 9]):
+        kv, table, n = make(cuda_device, lengths, 1, 128, 16, torch.float16)
+        wide = torch.zeros(table.shape[0], table.shape[1] + 1, dtype=torch.int32, device=cuda_device)
+        wide[:, :-1] = table
+        q = rows(cuda_device, (len(lengths), 1, 1, 128), torch.float16, 8)
+        weight, before = (torch.zeros(kv.shape[:3], device=cuda_device) for _ in range(2))
+        counts = torch.ones(2 * len(lengths), dtype=torch.int32, device=cuda_device)[::2]
+        got, lse = kc.cache4_attention(q, kv, wide[:, :-1], n, 128 ** -0.5, counts=counts, weight=weight, want_lse=True)
+        check_attention(got, q, kv, table, lengths, 128 ** -0.5, lse=lse, weight=weight, weight_before=before)
