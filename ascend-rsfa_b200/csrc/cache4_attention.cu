@@ -854,7 +854,10 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
   const int item = blockIdx.x % (c.H * row_blocks), b = blockIdx.x / (c.H * row_blocks), h = item / row_blocks;
   const int from = blockIdx.y * rows_each, row0 = (item - h * row_blocks) * 8 * NT + from;
   const int count = min(min(rows_each, 8 * NT - from), rows.count - row0);   // rows of this CTA
-  if (count <= 0) return;        // (the kernel behind this one waits for the whole grid all the same)
+  if (count <= 0) {
+    griddep_wait();              // no CTA ends before the kernel in front does
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int tiles = tiles_of(c, a.counts, b);
   auto answer = [&](int row, int64_t* at_lse) {
@@ -962,9 +965,11 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_kernel(const Cac
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
   const Shares shares(total, gridDim.x * kWeightWarps);
   const int worker = shares.here();
-  if (worker >= shares.workers) return;
-  Cursor k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
+  const bool used = worker < shares.workers;
+  Cursor k;
+  if (used) k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
   griddep_wait();          // lengths were there before the first kernel started
+  if (!used) return;       // behind the wait: this grid's end has to be behind that of the ones in front
   const int mask = (1 << c.page_shift) - 1;
   while (k.t < k.end) {
     // log-sum-exps of the item's rows, one per lane (there are no more than 16)
@@ -1031,9 +1036,11 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_again_kernel(con
   const long long total = all_units(c, a.counts, 0, 0, &none) * c.H;
   const Shares shares(total, gridDim.x * kWeightWarps);
   const int worker = shares.here();
-  if (worker >= shares.workers) return;
-  Cursor k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
+  const bool used = worker < shares.workers;
+  Cursor k;
+  if (used) k = cursor_at(c, a.counts, c.H, 0, shares.begin(worker), shares.begin(worker + 1));
   griddep_wait();          // lengths were there before the first kernel started
+  if (!used) return;       // behind the wait: this grid's end has to be behind that of the ones in front
   const int mask = (1 << c.page_shift) - 1;
   while (k.t < k.end) {
     const int run = k.end - k.t;

@@ -704,3 +704,18 @@ def test_scratch_is_sized_for_every_call(cuda_device):
         counts = torch.ones(2 * len(lengths), dtype=torch.int32, device=cuda_device)[::2]
         got, lse = kc.cache4_attention(q, kv, wide[:, :-1], n, 128 ** -0.5, counts=counts, weight=weight, want_lse=True)
         check_attention(got, q, kv, table, lengths, 128 ** -0.5, lse=lse, weight=weight, weight_before=before)
+
+
+@pytest.mark.gpu
+def test_what_follows_a_batch_without_tokens_sees_its_zeros(cuda_device):
+    """No kernel of the call has work but the one that writes zeros, and the next operator waits for that one, too."""
+    kv, table, lengths = make(cuda_device, [0] * 64, 2, 128, 16, torch.float16)
+    q = rows(cuda_device, (64, 16, 1, 128), torch.float16, 5)
+    weight = torch.zeros(kv.shape[:3], device=cuda_device)
+    cos_sin, last = ro.rotary_table(4, 128, device=cuda_device), torch.tensor([3], dtype=torch.int32, device=cuda_device)
+    for _ in range(20):
+        stale = torch.full_like(q, math.nan)
+        del stale                                                  # the next allocation of this size
+        o, lse = kc.cache4_attention(q, kv, table, lengths, 0.1, weight=weight, want_lse=True)
+        turned, _ = ro.rotary(o, None, cos_sin, last)
+        assert bool((turned == 0).all()) and bool((o == 0).all()) and bool((lse == -math.inf).all()) and bool((weight == 0).all())
