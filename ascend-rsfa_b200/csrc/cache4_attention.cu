@@ -38,11 +38,13 @@ constexpr int kJoinThreads = 128, kJoinMost = 512;
 __host__ __device__ constexpr int tile_tokens(int D) { return D == 64 ? 64 : 32; }
 // One CTA per multiprocessor: as many warps as the registers of their accumulators allow, and slots of a warp's ring by the
 // shared memory that is left.  (Three CTAs of four warps: the same loop, but three times the CTAs to start, 256 sequences of
-// 200 tokens in 48 us for 39.)
+// 200 tokens in 48 us for 39.  Sixteen rows of 64 dims by 8 warps without spills, 16 sequences of 16384 tokens, 64 heads over
+// 4, in 45.3 us; by 12 with them in 49.2.  Eight rows by 16 warps with two slots: 32 sequences of 16384 tokens 85.7 us for
+// 89.3, 16 of up to 2048 tokens 24.1 for 21.5, left at 12.)
 template <int D, int NT>
 struct Shape {
-  static constexpr int kWarps = D == 256 || (NT == 2 && D == 128) ? 8 : 12, kThreads = 32 * kWarps;
-  static constexpr int kStages = D == 256 ? 2 : NT == 2 && D == 128 ? 4 : 3;
+  static constexpr int kWarps = D == 256 || NT == 2 ? 8 : 12, kThreads = 32 * kWarps;
+  static constexpr int kStages = D == 256 ? 2 : NT == 2 ? 4 : 3;
   static constexpr int kTile = tile_tokens(D);
   static constexpr int kPieces = kTile / 16;     // loads per tile: a page holds whole ones
   static constexpr int kPieceBytes = 16 * Record<D>::kBytes;
