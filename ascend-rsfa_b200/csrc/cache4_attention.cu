@@ -25,7 +25,7 @@
 // together.  (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist
 // unpacked in registers only.)  Times with 128 dims, against the time for the bytes alone: one sequence of 131072 tokens,
 // 8 heads, 51.6 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 86 us (53); 256 sequences of 200
-// tokens 39 us (11); one sequence of 16 tokens 10.6 us, two dependent kernels of about 5 each.
+// tokens 39 us (11); one of 500 tokens 9.5 us, two dependent kernels.
 #include "../../include/rsfa.h"
 #include "ops_common.cuh"
 
@@ -883,12 +883,11 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
   const long long total = all_units(c, a.counts, kItemCost, b, &before) * per_sequence;
   const Shares shares(total, all_workers);
   const long long first = before * per_sequence + static_cast<long long>(item) * (tiles + kItemCost) + kItemCost;   // unit of its first tile
+  const int w0 = shares.of(first), pieces = shares.of(first + tiles - 1) - w0 + 1;
   // lengths were there before the first kernel started, its pieces are now
   griddep_wait();
   griddep_launch_dependents();
-  const long long w0 = shares.of(first), w1 = shares.of(first + tiles - 1);
-  if (w0 == w1) return;                       // in one piece: answered already
-  const int pieces = static_cast<int>(w1 - w0) + 1;
+  if (pieces == 1) return;                    // answered already
   // the warps in teams, one per row, as far as they go
   const int teams = min(count, warps), members = warps / teams, team = warp % teams, member = warp / teams;
   for (int r0 = 0; r0 < count; r0 += teams) {
@@ -896,7 +895,7 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
     const bool busy = r < count && member < members;
     if (busy) {
       auto piece_of = [&](int i) {            // the first one is its worker's last item, the others their workers' first
-        return a.pieces + ((w0 + i) * 2 + (i == 0)) * piece_floats<D, NT>() + (from + r) * (D + 2);
+        return a.pieces + ((w0 + i) * 2ll + (i == 0)) * piece_floats<D, NT>() + (from + r) * (D + 2);
       };
       float ref = kNoScore, l = 0.f, sum[kEach];
 #pragma unroll
@@ -905,6 +904,9 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
       for (int i0 = member; i0 < pieces; i0 += 32 * members) {
         const int mine = i0 + lane * members;
         const float2 ml = mine < pieces ? *reinterpret_cast<const float2*>(piece_of(mine) + D) : make_float2(kNoScore, 0.f);
+        float next[kEach];                    // of the first piece, asked for at once: where there are few it is the only one
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) next[j] = piece_of(i0)[lane + 32 * j];
         float top = ml.x;
 #pragma unroll
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -915,8 +917,11 @@ __global__ void __launch_bounds__(kJoinMost) cache4_join_kernel(const Cache4 c, 
 #pragma unroll
         for (int j = 0; j < kEach; ++j) sum[j] *= before;
         const int here = min(32, (pieces - i0 + members - 1) / members);
+        const float share0 = __shfl_sync(0xffffffffu, by, 0);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) sum[j] = fmaf(share0, next[j], sum[j]);
 #pragma unroll 8
-        for (int k = 0; k < here; ++k) {
+        for (int k = 1; k < here; ++k) {
           const float* p = piece_of(i0 + k * members);
           const float share = __shfl_sync(0xffffffffu, by, k);
 #pragma unroll
