@@ -20,9 +20,8 @@
 // the device takes an equal, contiguous share of it, whatever the lengths are.  A share's first and last item may
 // continue in other warps: their sums go to a workspace and a second kernel joins them.
 //
-// What bounds it: not HBM, 5 D / 4 bytes per token and K/V head, but the issue slots right behind it: some 320
-// instructions per 16 tokens, K/V head and 8 rows, most of them to take the codes apart and to bring weights and scales
-// together.  (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist
+// What bounds it: not HBM, 5 D / 4 bytes per token and K/V head, but some 320 instructions per 16 tokens, K/V head and 8
+// rows, at the rate at which three warps per scheduler, all that registers allow, keep it busy: 56 % of the issue slots.  (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist
 // unpacked in registers only.)  Times with 128 dims, against the time for the bytes alone: one sequence of 131072 tokens,
 // 8 heads, 51.0 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 86 us (53); 256 sequences of 200
 // tokens 39 us (11); one of 500 tokens 9.5 us, two dependent kernels.
