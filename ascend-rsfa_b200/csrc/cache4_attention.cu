@@ -21,8 +21,9 @@
 // continue in other warps: their sums go to a workspace and a second kernel joins them.
 //
 // What bounds it: not HBM, 5 D / 4 bytes per token and K/V head, but some 320 instructions per 16 tokens, K/V head and 8
-// rows, at the rate at which three warps per scheduler, all that registers allow, keep it busy: 56 % of the issue slots.  (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist
-// unpacked in registers only.)  Times with 128 dims, against the time for the bytes alone: one sequence of 131072 tokens,
+// rows, at the rate at which three warps per scheduler, all that registers allow, keep it busy: 56 % of the issue slots.
+// (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist unpacked in
+// registers only.)  Times with 128 dims, against the time for the bytes alone: one sequence of 131072 tokens,
 // 8 heads, 51.0 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 86 us (53); 256 sequences of 200
 // tokens 39 us (11); one of 500 tokens 9.5 us, two dependent kernels.
 #include "../../include/rsfa.h"
@@ -104,17 +105,6 @@ __device__ __forceinline__ float scale_of(uint32_t pair, uint16_t by) {
     asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nfma.rn.f32.bf16 %0, l, %2, %3;\n}\n" : "=f"(r) : "r"(pair), "h"(by), "f"(0.f));
   else
     asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %1;\nfma.rn.f32.f16 %0, l, %2, %3;\n}\n" : "=f"(r) : "r"(pair), "h"(by), "f"(0.f));
-  return r;
-}
-// 8 s + m of two neighbouring tokens' pairs (low half scale, high half minimum).
-template <bool kBf16>
-__device__ __forceinline__ uint32_t middles(uint32_t first, uint32_t second) {
-  const uint32_t s = __byte_perm(first, second, 0x5410), m = __byte_perm(first, second, 0x7632);
-  uint32_t r;
-  if constexpr (kBf16)
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(s), "r"(0x41004100u), "r"(m));
-  else
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(s), "r"(0x48004800u), "r"(m));
   return r;
 }
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -422,13 +412,13 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
 // rounding of P then shows times u - 8 instead of u, and neither it nor an MMA's own (which cuts its sums off, at 2^-24 of what
 // its operands' exponents allow) comes up against a sum that is mostly the codes' middle.  With u * 2^-24 as the operand
 // here, too, results were off by 4.5e-4 over 60000 tokens, with u - 8 by 2.8e-4 (fp16, whose own rounding is 2.1e-4).
-// The last sum (`mids`) comes out of an MMA of its own, whose row w is group w, with p and m + 8 s rounded to the
-// cache's type like the weights and values of any 16-bit attention.
+// The last sum (`mids`) comes out of an MMA of its own, whose rows w and w + 8 are the minima and the scales of group w as they
+// are stored; p is rounded to the cache's type for it, the same for both, like the weights of any 16-bit attention.
 template <int D, int NT>
 struct Sums {
   static constexpr int G = D / 32;
   float o[2 * G][NT][4];       // tile 2 w + t: dims 32 w + 4 g + 2 t and + 1, times 2^-9 over `unit`
-  float mids[NT][4];           // sum p (m + 8 s) of group g % G, rows 2 c, 2 c + 1 (twice)
+  float mids[NT][4];           // sum p m of group g % G, rows 2 c, 2 c + 1, then sum p s
   float l[NT][2], ref[NT][2];
   float unit;                  // power of two that s is divided by
   uint32_t per_unit;           // 1 / unit, a 16-bit number of the cache's type
@@ -518,10 +508,12 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
       ph[w] = z.x, ph[w + 1] = z.y, ph[w + 2] = z.z, ph[w + 3] = z.w;
     }
   }
-  const uint32_t mid_lo = middles<kBf16>(mid[0], mid[1]), mid_hi = middles<kBf16>(mid[2], mid[3]);
+  // rows of minima, then rows of scales
+  const uint32_t m_lo = __byte_perm(mid[0], mid[1], 0x7632), s_lo = __byte_perm(mid[0], mid[1], 0x5410);
+  const uint32_t m_hi = __byte_perm(mid[2], mid[3], 0x7632), s_hi = __byte_perm(mid[2], mid[3], 0x5410);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
-    mma_own<kBf16>(x.mids[nt], mid_lo, mid_lo, mid_hi, mid_hi, transpose_8x8(from_f32x2<kBf16>(p[nt][0], p[nt][1])),
+    mma_own<kBf16>(x.mids[nt], m_lo, s_lo, m_hi, s_hi, transpose_8x8(from_f32x2<kBf16>(p[nt][0], p[nt][1])),
                    transpose_8x8(from_f32x2<kBf16>(p[nt][2], p[nt][3])));
 #pragma unroll
   for (int w = 0; w < G; ++w) {
@@ -571,6 +563,7 @@ __device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2],
       x.ref[nt][i] = ref;
       x.l[nt][i] *= by;
       x.mids[nt][i] *= by;
+      x.mids[nt][i + 2] *= by;
 #pragma unroll
       for (int j = 0; j < 2 * (D / 32); ++j) {
         x.o[j][nt][i] *= by_both;
@@ -678,7 +671,7 @@ __device__ __forceinline__ void store_sums(Sums<D, NT>& x, const Cache4Attention
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
 #pragma unroll
-      for (int w = 0; w < G; ++w) m[w] = __shfl_sync(0xffffffffu, x.mids[nt][i], 4 * w + q4);
+      for (int w = 0; w < G; ++w) m[w] = __shfl_sync(0xffffffffu, fmaf(8.f, x.mids[nt][i + 2], x.mids[nt][i]), 4 * w + q4);
       const int r = 8 * nt + 2 * q4 + i, row = row0 + r;
       if (row < rows.count) {
         if (piece != nullptr) {

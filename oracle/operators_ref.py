@@ -97,16 +97,16 @@ def records(k, v):
 
 
 def values(rec, dtype):
-    """Records [n, 5 D / 4] -> (K values, V values, V values without their minima) in 64 bits."""
+    """Records [n, 5 D / 4] -> (K values, V values, V values less those of code 8) in 64 bits."""
     n, D = rec.shape[0], rec.shape[1] * 4 // 5
     G, out, at = D // 32, [], D
     for places in code_places(D):
         u = torch.stack([(rec[:, byte] >> bit) & 15 for byte, bit in places], -1).double()
         pairs = rec[:, at:at + 4 * G].contiguous().view(dtype).double().reshape(n, G, 2)
         at += 4 * G
-        part = u * pairs[..., 0].repeat_interleave(32, -1)
-        out.append(part + pairs[..., 1].repeat_interleave(32, -1))
-    return out[0], out[1], part
+        scale = pairs[..., 0].repeat_interleave(32, -1)
+        out.append(u * scale + pairs[..., 1].repeat_interleave(32, -1))
+    return out[0], out[1], (u - 8) * scale
 
 
 def rows_of(kv, table, b, h, n):
@@ -120,18 +120,22 @@ def rows_of(kv, table, b, h, n):
 
 def attention(q, kv, table, lengths, sm_scale, counts=None):
     """(o, lse, weights {(b, h): [n]}, bound) in 64 bits; bound: per output, the sums its error is made of
-    (sum p s u, sum p |v|, largest sum |q| |k| of a visible token)."""
+    (sum p s |u - 8|, sum p |m + 8 s|, sum p (|m| + 8 s), sum p |v|, largest sum |q| |k| of a visible token)."""
     B, Hq, S, D = q.shape
     H, dev = kv.shape[1], q.device
     o = torch.zeros((B, Hq, S, D), dtype=torch.float64, device=dev)
     lse = torch.full((B, Hq, S), -math.inf, dtype=torch.float64, device=dev)
-    parts, sizes, terms = torch.zeros_like(o), torch.zeros_like(o), torch.zeros_like(lse)
+    parts, middles, both, sizes = (torch.zeros_like(o) for _ in range(4))
+    terms = torch.zeros_like(lse)
     weights = {}
     for b in range(B):
         n = int(lengths[b])
         count = S if counts is None else min(int(counts[b]), S)
         for h in range(H):
-            k, v, part = values(rows_of(kv, table, b, h, n), q.dtype)
+            rec = rows_of(kv, table, b, h, n)
+            k, v, part = values(rec, q.dtype)
+            eight = rec[:, -(D // 8):].contiguous().view(q.dtype)[:, ::2].double().repeat_interleave(32, -1) * 8     # 8 s of V
+            apart = (v - part - eight).abs() + eight
             total = torch.zeros(n, dtype=torch.float64, device=dev)
             for hq in range(h * (Hq // H), (h + 1) * (Hq // H)):
                 for i in range(count):
@@ -142,12 +146,12 @@ def attention(q, kv, table, lengths, sm_scale, counts=None):
                     s = k[:see] @ x * sm_scale
                     lse[b, hq, i] = torch.logsumexp(s, 0)
                     p = torch.exp(s - lse[b, hq, i])
-                    o[b, hq, i], parts[b, hq, i] = p @ v[:see], p @ part[:see]
-                    sizes[b, hq, i] = p @ v[:see].abs()
+                    o[b, hq, i], parts[b, hq, i], middles[b, hq, i] = p @ v[:see], p @ part[:see].abs(), p @ (v - part)[:see].abs()
+                    sizes[b, hq, i], both[b, hq, i] = p @ v[:see].abs(), p @ apart[:see]
                     terms[b, hq, i] = (k[:see].abs() @ x.abs()).max() * abs(sm_scale)
                     total[:see] += p
             weights[b, h] = total
-    return o, lse, weights, (parts, sizes, terms)
+    return o, lse, weights, (parts, middles, both, sizes, terms)
 
 
 def evict(weight, position, budget, recent):

@@ -38,13 +38,17 @@ def make(dev, lengths, H, D, page, dtype, seed=0, room=None, std=1.0):
 
 
 def check_attention(got, q, kv, table, lengths, scale, counts=None, lse=None, weight=None, weight_before=None):
-    """The operator's own roundings: p * s to fp16 (2^-11 of the part that the codes carry; below fp16's normal
-    numbers an absolute 2^-25 of the largest scale times 2^-6 per token, 15 codes: counted as 2^-24 of the sizes), the
-    result to 16 bits, and 32-bit sums.  A score is a sum of D products of at most `terms` in total, rounded a few
-    times in 32 bits, and an exponential with a relative error of 2^-22: weights are off by 2^-19 (1 + terms) at most."""
-    o, want_lse, weights, (parts, sizes, terms) = ref.attention(q, kv, table, lengths, scale, counts)
+    """The operator's own roundings.  A result is sum p s (u - 8) + sum p (m + 8 s): p * s is rounded to fp16, half a step of
+    2^-11, and p to the cache's type, half a step of that, so the two sums are off by 2^-11 sum p s |u - 8| and by half a
+    step of sum p |m + 8 s|; the result is rounded to 16 bits.  The 32-bit sums sum P (u - 8), sum p m and sum p s are cut off
+    at 2^-24 of what they come to, some 2^8 times: 2^-16 of sum p s |u - 8| and sum p (|m| + 8 s), which the difference of the
+    last two can be far below.  (That covers P below fp16's normal numbers, an absolute 2^-25 where the largest is 2^10.)
+    A score is a sum of D products of at most `terms` in total, rounded a few times in 32 bits, and an exponential with a
+    relative error of 2^-22: weights are off by 2^-19 (1 + terms) at most."""
+    o, want_lse, weights, (parts, middles, both, sizes, terms) = ref.attention(q, kv, table, lengths, scale, counts)
     off = 2.0 ** -19 * (1 + terms)
-    bound = HALF_STEP[q.dtype] * o.abs() + 2.0 ** -11 * parts + (2 * off + 2.0 ** -16)[..., None] * sizes + TINY[q.dtype]
+    bound = (HALF_STEP[q.dtype] * (o.abs() + middles) + 2.0 ** -11 * parts + 2 * off[..., None] * sizes + 2.0 ** -16 * (parts + both)
+             + TINY[q.dtype])
     err = (got.double() - o).abs()
     assert bool((err <= bound).all()), (float(err.max()), float((err - bound).max()))
     if lse is not None:
@@ -60,7 +64,9 @@ def check_attention(got, q, kv, table, lengths, scale, counts=None, lse=None, we
             for h in range(H):
                 want[table[b].long()[slot // P], h, slot % P] += weights[b, h]
         rel = 2.0 * float(off.max()) + 2.0 ** -20
-        assert bool(((weight.double() - want).abs() <= rel * (want - weight_before.double()) + 2.0 ** -23 * want.abs() + 1e-30).all())
+        # the sum of up to eight rows, then half a step of 2^-24 for every block of rows that is added, and one for `want`
+        blocks = -(-q.shape[1] // H * q.shape[2] // 8) + 1
+        assert bool(((weight.double() - want).abs() <= rel * (want - weight_before.double()) + 2.0 ** -24 * blocks * want.abs() + 1e-30).all())
 
 
 # ------------------------------------------------------------------ without a GPU
@@ -719,3 +725,19 @@ def test_what_follows_a_batch_without_tokens_sees_its_zeros(cuda_device):
         o, lse = kc.cache4_attention(q, kv, table, lengths, 0.1, weight=weight, want_lse=True)
         turned, _ = ro.rotary(o, None, cos_sin, last)
         assert bool((turned == 0).all()) and bool((o == 0).all()) and bool((lse == -math.inf).all()) and bool((weight == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,D,Hq,H,S,page,scale,std", [([46, 107, 76, 1, 275, 0, 0], 256, 80, 5, 9, 64, 1.0, 1.0),
+                                                             ([5, 5, 0, 1, 2, 3, 4], 256, 4, 2, 1, 64, 0.0625, 3.0),
+                                                             ([39, 1, 0, 40, 25], 128, 9, 3, 4, 128, 1.0, 3.0),
+                                                             ([191, 0, 147, 1, 23], 64, 12, 3, 5, 32, -0.125, 1.0)])
+def test_attention_of_few_tokens_and_many_rows(cuda_device, dtype, lengths, D, Hq, H, S, page, scale, std):
+    """Rows that one token has nearly to itself, whose dims are then sums that cancel, and more rows than two blocks."""
+    kv, table, n = make(cuda_device, lengths, H, D, page, dtype, seed=17, std=std)
+    q = rows(cuda_device, (len(lengths), Hq, S, D), dtype, 18)
+    weight = torch.rand(kv.shape[:3], device=cuda_device)
+    before = weight.clone()
+    got, lse = kc.cache4_attention(q, kv, table, n, scale, weight=weight, want_lse=True)
+    check_attention(got, q, kv, table, lengths, scale, lse=lse, weight=weight, weight_before=before)
