@@ -24,7 +24,7 @@
 // rows, at the rate at which three warps per scheduler, all that registers allow, keep it busy: 56 % of the issue slots.
 // (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist unpacked in
 // registers only.)  Times with 128 dims, against the time for the bytes alone: one sequence of 131072 tokens,
-// 8 heads, 51.0 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 86 us (53); 256 sequences of 200
+// 8 heads, 51.0 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 85 us (53); 256 sequences of 200
 // tokens 39 us (11); one of 500 tokens 9.5 us, two dependent kernels.
 #include "../../include/rsfa.h"
 #include "ops_common.cuh"
