@@ -541,8 +541,7 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
 // tokens).
 template <int D, int NT, bool kBf16>
 __device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2], uint32_t widest) {
-  float scale = to_f32<kBf16>(static_cast<uint16_t>(widest));
-  scale = scale < INFINITY ? scale : 0.f;                         // NaN is left to the products
+  float scale = to_f32<kBf16>(static_cast<uint16_t>(widest));      // finite
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, d));
   // the power of two below it, where it is above what the unit is for
@@ -570,6 +569,21 @@ __device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2],
         x.o[j][nt][i + 2] *= by_both;
       }
     }
+}
+
+// What the widest finite scale of a lane's share of a tile is (see one_tile), where one that is not finite hides it.
+template <int D, bool kBf16>
+__device__ __noinline__ uint32_t widest_finite(const uint8_t* rec) {
+  using R = Record<D>;
+  constexpr int G = D / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  uint32_t widest = 0;
+  for (int token = g; token < tile_tokens(D); token += 8)
+    for (int w = 0; w < (G + 3) / 4; ++w) {
+      const uint32_t scale = *reinterpret_cast<const uint16_t*>(rec + token * R::kBytes + R::kVPairs + 4 * ((q4 + 4 * w) % G));
+      if (scale < (kBf16 ? 0x7f80u : 0x7c00u)) widest = max(widest, scale);
+    }
+  return widest;
 }
 
 // One tile at `rec`, whose first slot is `slot`.  scores: where the tile's scores are kept, null: nowhere.
@@ -603,7 +617,7 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
       top[nt][i] = most * f.factor[nt][i];
       higher |= top[nt][i] > x.ref[nt][i] + kRaise;
     }
-  // a scale much above all before: each lane looks at its share of the tile's
+  // a scale much above all before: each lane looks at its share of the tile's (as integers, which their bits order like)
   uint32_t widest = 0;
 #pragma unroll
   for (int i = 0; i < 2 * kBlocks; ++i)
@@ -612,7 +626,8 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
       widest = max(widest, *reinterpret_cast<const uint16_t*>(rec + (g + 8 * i) * R::kBytes + R::kVPairs + 4 * ((q4 + 4 * w) % G)) + 0u);
   bool odd = false;
   if (__any_sync(0xffffffffu, higher || widest > x.unit_limit)) {
-    odd = __any_sync(0xffffffffu, widest > (kBf16 ? 0x7f80u : 0x7c00u));
+    odd = __any_sync(0xffffffffu, widest >= (kBf16 ? 0x7f80u : 0x7c00u));
+    if (odd) widest = widest_finite<D, kBf16>(rec);
     raise<D, NT, kBf16>(x, top, widest);
   }
   if (scores != nullptr) {

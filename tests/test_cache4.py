@@ -741,3 +741,38 @@ def test_attention_of_few_tokens_and_many_rows(cuda_device, dtype, lengths, D, H
     before = weight.clone()
     got, lse = kc.cache4_attention(q, kv, table, n, scale, weight=weight, want_lse=True)
     check_attention(got, q, kv, table, lengths, scale, lse=lse, weight=weight, weight_before=before)
+
+
+# ------------------------------------------------------------------ rows that see what others do not
+
+def attention_bound(q, kv, table, lengths, scale, counts=None):
+    """The result in 64 bits and the bound of check_attention, for results that are NaN in places."""
+    o, _, _, (parts, middles, both, sizes, terms) = ref.attention(q, kv, table, lengths, scale, counts)
+    off = 2.0 ** -19 * (1 + terms)
+    return o, (HALF_STEP[q.dtype] * (o.abs() + middles) + 2.0 ** -11 * parts + 2 * off[..., None] * sizes + 2.0 ** -16 * (parts + both)
+               + TINY[q.dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [32, 256])
+@pytest.mark.parametrize("D,Hq", [(64, 1), (64, 8), (128, 4), (128, 16), (256, 2)])
+def test_a_row_of_v_with_an_infinity_beside_one_of_wide_scales(cuda_device, dtype, bad, D, Hq):
+    """The last of two query tokens sees slot 8, whose V holds an infinity in its first `bad` dims; both rest on slot 0, whose
+    V is a hundred times as wide as the others'.  The first has finite results, the second NaN in the groups of these dims only."""
+    n = 9
+    kv, weight, position = kc.cache4_empty(2, 1, 16, D, device=cuda_device)
+    table, lengths = torch.tensor([[1]], dtype=torch.int32, device=cuda_device), torch.tensor([n], dtype=torch.int32, device=cuda_device)
+    k, v, q = (rows(cuda_device, s, dtype, i) for i, s in enumerate(((1, 1, n, D), (1, 1, n, D), (1, Hq, 2, D))))
+    k[:, :, 0, 0], q[..., 0] = 8, 8
+    v[:, :, 0] *= 100
+    v[:, :, 8, : bad : 32] = math.inf
+    kc.cache4_append(k, v, kv, table, lengths)
+    got = kc.cache4_attention(q, kv, table, lengths, 0.5)
+    check_attention(got[:, :, :1], q[:, :, :1], kv, table, [n - 1], 0.5)
+    o, bound = attention_bound(q, kv, table, lengths, 0.5)
+    nan = torch.zeros_like(o, dtype=torch.bool)
+    nan[:, :, 1, :bad] = True
+    assert torch.equal(o.isnan(), nan) and torch.equal(got.isnan(), nan)
+    assert bool(((got.double() - o).abs() <= bound)[~nan].all())
+    fa.device_status()
