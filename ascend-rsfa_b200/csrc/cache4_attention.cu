@@ -11,7 +11,7 @@
 //
 // The second product runs over codes less their middle, u - 8 (exact), and the middles m + 8 s of the groups are a third,
 // small one: what rounding p * s to fp16 leaves is then in proportion to a group's range.  p itself is 32 bits wide where
-// it is summed and added to the weights; for the middles it is rounded to the cache's type.
+// it is summed and added to the weights; the middles take it as two numbers of the cache's type.
 //
 // Rows of scores are handed on by a flash recurrence whose reference is raised only when a score exceeds what it
 // was set for by a log2 unit.
@@ -56,8 +56,8 @@ constexpr int kTagCache4Load = 40;   // of a bounded wait, in the status word
 // A reference is set kHeadroom log2 units below its row's largest score and raised when a score is kRaise above it, one unit
 // above the largest before; the scales' unit is raised when one is kRaiseScale of it.  So a product p * s is at most 2^11 * 4
 // in fp16, whose normal numbers then reach weights of 2^-24 of the largest, and the largest weights, which are what rounding
-// shows in most, are close to powers of two (8192 and 60000 tokens: results off by 2.4e-4 and 2.5e-4; raised only eight
-// units above: 2.8e-4 and 3.5e-4).
+// shows in most, are close to powers of two (fp16, whose own rounding is 2.1e-4: 4 sequences of up to 8192 tokens, 64 of 1 to 8192 and
+// one of 60000, results off by 2.4e-4, 2.6e-4 and 2.5e-4; raised only eight units above, the first and the last: 2.8e-4 and 3.5e-4).
 constexpr float kHeadroom = 10.f, kRaise = 11.f;
 constexpr float kRaiseScale = 4.f;
 
@@ -412,8 +412,10 @@ __device__ __forceinline__ void block_scores(float (&s)[NT][4], const uint8_t* r
 // rounding of P then shows times u - 8 instead of u, and neither it nor an MMA's own (which cuts its sums off, at 2^-24 of what
 // its operands' exponents allow) comes up against a sum that is mostly the codes' middle.  With u * 2^-24 as the operand
 // here, too, results were off by 4.5e-4 over 60000 tokens, with u - 8 by 2.8e-4 (fp16, whose own rounding is 2.1e-4).
-// The last sum (`mids`) comes out of an MMA of its own, whose rows w and w + 8 are the minima and the scales of group w as they
-// are stored; p is rounded to the cache's type for it, the same for both, like the weights of any 16-bit attention.
+// The last sum (`mids`) comes out of MMAs of its own, whose rows w and w + 8 are the minima and the scales of group w as they
+// are stored.  They take p as its 16-bit rounding and what that leaves, 16 bits of it or more: the sum that the result is divided
+// by has all 32, and V rows that have much in common would not come back as that (with the first part alone bf16 results
+// were off by 1.71e-3 for 1.67e-3, 1.67e-3 of it their own rounding; 64 sequences of 1 to 8192 tokens 85.7 us for 86.9).
 template <int D, int NT>
 struct Sums {
   static constexpr int G = D / 32;
@@ -512,9 +514,13 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
   const uint32_t m_lo = __byte_perm(mid[0], mid[1], 0x7632), s_lo = __byte_perm(mid[0], mid[1], 0x5410);
   const uint32_t m_hi = __byte_perm(mid[2], mid[3], 0x7632), s_hi = __byte_perm(mid[2], mid[3], 0x5410);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-    mma_own<kBf16>(x.mids[nt], m_lo, s_lo, m_hi, s_hi, transpose_8x8(from_f32x2<kBf16>(p[nt][0], p[nt][1])),
-                   transpose_8x8(from_f32x2<kBf16>(p[nt][2], p[nt][3])));
+  for (int nt = 0; nt < NT; ++nt) {
+    const uint32_t p_lo = from_f32x2<kBf16>(p[nt][0], p[nt][1]), p_hi = from_f32x2<kBf16>(p[nt][2], p[nt][3]);
+    const float2 t_lo = to_f32x2<kBf16>(p_lo), t_hi = to_f32x2<kBf16>(p_hi);
+    mma_own<kBf16>(x.mids[nt], m_lo, s_lo, m_hi, s_hi, transpose_8x8(p_lo), transpose_8x8(p_hi));
+    mma_own<kBf16>(x.mids[nt], m_lo, s_lo, m_hi, s_hi, transpose_8x8(from_f32x2<kBf16>(p[nt][0] - t_lo.x, p[nt][1] - t_lo.y)),
+                   transpose_8x8(from_f32x2<kBf16>(p[nt][2] - t_hi.x, p[nt][3] - t_hi.y)));
+  }
 #pragma unroll
   for (int w = 0; w < G; ++w) {
     // the half words of group w: low half token 2 c (2 c + 8), high half the token behind it

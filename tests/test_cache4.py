@@ -776,3 +776,25 @@ def test_a_row_of_v_with_an_infinity_beside_one_of_wide_scales(cuda_device, dtyp
     assert torch.equal(o.isnan(), nan) and torch.equal(got.isnan(), nan)
     assert bool(((got.double() - o).abs() <= bound)[~nan].all())
     fa.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,Hq,H,S", [(64, 4, 4, 1), (64, 24, 2, 1), (128, 8, 2, 1), (128, 16, 2, 2), (256, 4, 2, 3)])
+def test_values_with_a_common_offset(cuda_device, dtype, D, Hq, H, S):
+    """V rows that are nearly the same come back as what they have in common: the weights of the groups' middles and the sum that
+    they are divided by are the same to 2^-16, so that the result's own rounding, half a step at its size, is what is left."""
+    lengths = [3, 4, 5, 9, 40, 700]
+    B, n = len(lengths), max(lengths)
+    kv, table, ls = make(cuda_device, lengths, H, D, 16, dtype, seed=3)
+    k = rows(cuda_device, (B, H, n, D), dtype, 1)
+    offset = (1 + torch.rand((B, H, 1, D // 32, 1), generator=torch.Generator(device=cuda_device).manual_seed(2), device=cuda_device)).expand(-1, -1, n, -1, 32).flatten(3)
+    v = (offset + 2.0 ** -6 * rows(cuda_device, (B, H, n, D), torch.float32, 3)).to(dtype)
+    kc.cache4_append(k, v, kv, table, ls, counts=ls)
+    q = rows(cuda_device, (B, Hq, S, D), dtype, 4)
+    got = kc.cache4_attention(q, kv, table, ls, 0.1)
+    o, _, _, (parts, middles, both, sizes, terms) = ref.attention(q, kv, table, ls, 0.1)
+    rest = 2.0 ** -11 * parts + 2.0 ** -16 * (parts + middles + both) + 2.0 ** -18 * (1 + terms)[..., None] * sizes
+    half = 2.0 ** torch.floor(torch.log2(o.abs() + rest)) * HALF_STEP[dtype]
+    err = (got.double() - o).abs()
+    assert bool((err <= half + rest).all()), (float((err - half - rest).max()), int((err > half + rest).sum()), err.numel())
