@@ -1,7 +1,7 @@
 """Rotary positions for q and k, in front of attention() or of the 4-bit cache (kv_cache.py).
 
     table = rotary_table(length, dim)                      # once, or again when the context outgrows it
-    q, k = rotary(q, k, table, positions)                  # differentiable
+    q, k = rotary(q, k, table, positions)                  # differentiable, in both modes
 
 on the same [B, H, S, D] fp16 / bf16 CUDA tensors as attention(); the reference applies no positions, its
 callers do.  The work is done by hand-written kernels in librsfa_b200.so (csrc/rotary.cu): without the
@@ -11,6 +11,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _capi
 from .flash_attention_forward import _DTYPES, _current_stream, _dense, _rsfa_torch
@@ -118,12 +119,27 @@ def _turn(q, k, table, positions, interleaved, inverse):
     return qo, ko
 
 
+def _tangent(t):
+    return None if t is None else unpack_dual(t).tangent
+
+
+def _turn_recorded(q, k, table, positions, interleaved, inverse):
+    """_turn(), seen by autograd where a gradient is recorded or a tangent carried."""
+    if k is not None and (_tangent(q) is None) != (_tangent(k) is None):
+        # a node's outputs have tangents together or not at all
+        return tuple(_turn_recorded(t, None, table, positions, interleaved, inverse)[0] for t in (q, k))
+    if _tangent(q) is None and not (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        return _turn(q, k, table, positions, interleaved, inverse)
+    return _rotary.apply(q, k, table, positions, interleaved, inverse)
+
+
 class _rotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, table, positions, interleaved, inverse):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(table, positions)
+        ctx.save_for_forward(table, positions)
         ctx.how = (interleaved, inverse)
         return _turn(q, k, table, positions, interleaved, inverse)
 
@@ -132,13 +148,17 @@ class _rotary(torch.autograd.Function):
         # the transposed rotation of the gradients; it can be differentiated again
         table, positions = ctx.saved_tensors
         interleaved, inverse = ctx.how
-        turn = _rotary.apply if torch.is_grad_enabled() else _turn
         if dq is None:
             if dk is not None:
-                dk = turn(dk, None, table, positions, interleaved, not inverse)[0]
+                dk = _turn_recorded(dk, None, table, positions, interleaved, not inverse)[0]
         else:
-            dq, dk = turn(dq, dk, table, positions, interleaved, not inverse)
+            dq, dk = _turn_recorded(dq, dk, table, positions, interleaved, not inverse)
         return dq, dk, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        # tangents turn like what they belong to
+        return _turn_recorded(tq, tk, *ctx.saved_tensors, *ctx.how)
 
 
 def rotary(q, k, table, positions=None, interleaved=False):
@@ -176,6 +196,4 @@ def rotary(q, k, table, positions=None, interleaved=False):
             raise ValueError("positions must be int32 or int64 on the device of q")
         if positions.shape not in ((q.shape[2],), (1, q.shape[2]), (q.shape[0], q.shape[2])):
             raise ValueError("positions must be [S], [1, S] or [B, S]")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _rotary.apply(q, k, table, positions, bool(interleaved), False)
-    return _turn(q, k, table, positions, bool(interleaved), False)
+    return _turn_recorded(q, k, table, positions, bool(interleaved), False)

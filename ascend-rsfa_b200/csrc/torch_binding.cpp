@@ -170,10 +170,13 @@ const at::Tensor* plain_cuda(PyObject* obj, at::ScalarType type, int64_t dims, i
     return nullptr;
   return &t;
 }
+// The tangent that a tensor has in forward-mode differentiation; undefined: none.
+at::Tensor tangent_of(const at::Tensor& t) { return t.defined() && t.unsafeGetTensorImpl()->autograd_meta() != nullptr ? t._fw_grad(0) : at::Tensor(); }
 // The same for [B, H, S, D] rows that the library reads as they are (plain_tensor) and that are not empty.
 const at::Tensor* plain_rows(PyObject* obj, int device) {
   if (!plain_tensor(obj)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(obj);
+  if (tangent_of(t).defined()) return nullptr;
   if (t.device().index() != device || t.numel() == 0 || t.size(0) > INT32_MAX || t.size(1) > INT32_MAX || t.size(2) > INT32_MAX) return nullptr;
   return &t;
 }
@@ -272,18 +275,34 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
     const bool q_first = of_q.defined();                       // the library wants the first of its two tensors
     const at::Tensor first = q_first ? of_q : of_k, second = q_first ? of_k : at::Tensor();
     at::Tensor a, b;
-    if (c10::GradMode::is_enabled() && (first.requires_grad() || (second.defined() && second.requires_grad()))) {
-      const auto again = RotaryFunction::apply(first, given(second), saved[0], given(saved[1]), interleaved, inverse);
-      a = again[0];
-      if (second.defined()) b = again[1];
-    } else {
-      const int rc = turn(first, second, saved[0], saved[1], interleaved, inverse, &a, &b);
-      TORCH_CHECK(rc == 0, "rsfa_rotary failed with code ", rc);
+    const at::Tensor of_first = readable(tangent_of(first)), of_second = readable(tangent_of(second));
+    turn_again(primal(first), primal(second), saved, interleaved, inverse, &a, &b);
+    if (of_first.defined() || of_second.defined()) {           // a gradient's tangent turns like the gradient
+      at::Tensor ta, tb;
+      if (of_first.defined())
+        turn_again(of_first, of_second, saved, interleaved, inverse, &ta, &tb);
+      else
+        turn_again(of_second, of_first, saved, interleaved, inverse, &tb, &ta);
+      if (ta.defined()) a._set_fw_grad(ta, 0, false);
+      if (tb.defined()) b._set_fw_grad(tb, 0, false);
     }
     out[q_first ? 0 : 1] = a;
     if (q_first) out[1] = b;
     return out;
   }
+  // Recorded in its turn, where that is asked for.
+  static void turn_again(const at::Tensor& first, const at::Tensor& second, const torch::autograd::variable_list& saved, bool interleaved, bool inverse,
+                         at::Tensor* a, at::Tensor* b) {
+    if (c10::GradMode::is_enabled() && (first.requires_grad() || (second.defined() && second.requires_grad()))) {
+      const auto again = RotaryFunction::apply(first, given(second), saved[0], given(saved[1]), interleaved, inverse);
+      *a = again[0];
+      if (second.defined()) *b = again[1];
+      return;
+    }
+    const int rc = turn(first, second, saved[0], saved[1], interleaved, inverse, a, b);
+    TORCH_CHECK(rc == 0, "rsfa_rotary failed with code ", rc);
+  }
+  static at::Tensor primal(const at::Tensor& t) { return tangent_of(t).defined() ? t._fw_primal(0) : t; }
   static std::optional<at::Tensor> given(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
   // Rows as the library reads them, copied once if need be.
   static at::Tensor readable(const at::Tensor& t) {

@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad as fwAD
 
 from ascend_rsfa import _capi
 from ascend_rsfa import flash_attention_forward as fa
@@ -228,3 +229,47 @@ def test_captured_forward_and_backward(cuda_device):
         y.data.zero_(), gq.zero_()
         graph.replay()
         assert torch.equal(gq, want) and torch.equal(y, eager)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("route", ["native", "python"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_forward_mode(cuda_device, monkeypatch, route, interleaved):
+    """A tangent is turned like what it belongs to, with and without gradients recorded, and through the backward pass."""
+    if route == "python":
+        monkeypatch.setattr(ro, "_native", None)
+    B, Hq, Hk, S, D, R = 2, 3, 1, 9, 64, 32
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    rand = lambda *s: torch.randn(s, generator=g, device=cuda_device).bfloat16()  # noqa: E731
+    table, pos = ro.rotary_table(40, R, device=cuda_device), torch.randint(0, 40, (B, S), generator=g, device=cuda_device)
+    q, tq, k, tk = rand(B, Hq, S, D), rand(B, Hq, S, D), rand(B, Hk, S, D), rand(B, Hk, S, D)
+    turned = lambda x, inverse=False: ref.rotary(x, table, pos, interleaved, inverse)  # noqa: E731
+    plain = ro.rotary(q, k, table, pos, interleaved)
+    for grad in (False, True):
+        for qs, ks in ((True, True), (True, False), (False, True)):
+            with fwAD.dual_level(), torch.set_grad_enabled(grad):
+                x, y = q.clone().requires_grad_(grad), k.clone().requires_grad_(grad)
+                out = ro.rotary(fwAD.make_dual(x, tq) if qs else x, fwAD.make_dual(y, tk) if ks else y, table, pos, interleaved)
+                for o, p, t, used in zip(out, plain, (tq, tk), (qs, ks)):
+                    primal, tangent = fwAD.unpack_dual(o)
+                    assert torch.equal(primal, p) and (not grad or o.requires_grad)
+                    if used:
+                        close(tangent, t, table, turned(t), torch.bfloat16, pos, interleaved)
+                    else:
+                        assert tangent is None or bool((tangent == 0).all())
+                if qs:
+                    one = fwAD.unpack_dual(ro.rotary(fwAD.make_dual(x, tq), None, table, pos, interleaved)[0]).tangent
+                    close(one, tq, table, turned(tq), torch.bfloat16, pos, interleaved)
+    # forward over reverse: the gradient's tangent is the tangent of what comes in, turned back
+    dq, dk, ddq, ddk = rand(B, Hq, S, D), rand(B, Hk, S, D), rand(B, Hq, S, D), rand(B, Hk, S, D)
+    x, y = q.clone().requires_grad_(), k.clone().requires_grad_()
+    for both in (True, False):
+        with fwAD.dual_level():
+            out = ro.rotary(x, y if both else None, table, pos, interleaved)
+            seeds = (fwAD.make_dual(dq, ddq), fwAD.make_dual(dk, ddk))
+            got = torch.autograd.grad(out if both else out[0], (x, y) if both else x, seeds if both else seeds[0])
+            for o, d, dd in zip(got, (dq, dk), (ddq, ddk)):
+                primal, tangent = fwAD.unpack_dual(o)
+                close(primal, d, table, turned(d, True), torch.bfloat16, pos, interleaved, True)
+                close(tangent, dd, table, turned(dd, True), torch.bfloat16, pos, interleaved, True)
+    fa.device_status()
