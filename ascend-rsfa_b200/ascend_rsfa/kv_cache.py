@@ -21,7 +21,7 @@ import torch
 
 from . import _capi
 from .flash_attention_forward import _DTYPES
-from .rotary import _call, _ordinary, _readable, _rows
+from .rotary import _call, _ordinary, _readable, _rows, _tangent
 
 _lib = _capi.load()
 _HEAD_DIMS = (64, 128, 256)
@@ -140,6 +140,11 @@ def cache4_read(kv, table, lengths, n, dtype, starts=None):
     return k, v
 
 
+def _refuse_tangent(q):
+    if _tangent(q) is not None:
+        raise NotImplementedError("cache4_attention() has no derivative in forward mode")
+
+
 class _without_gradient(torch.autograd.Function):
 
     @staticmethod
@@ -158,14 +163,17 @@ def cache4_attention(q, kv, table, lengths, sm_scale, counts=None, weight=None, 
     has been appended before.  Hq is a multiple of the cache's heads: head h serves query heads h * Hq / heads ... .
     Rows that see nothing - a sequence of length 0, padding behind counts[b] - are zero with an lse of -inf.
     weight: grows, per token and K/V head, by the softmax weights that all query rows of that head give the token.
-    lse: [B, Hq, S] fp32, m + log(l).  There is no gradient: a backward pass that reaches the call raises.
+    lse: [B, Hq, S] fp32, m + log(l).  There is no gradient: a backward pass that reaches the call raises,
+    and so does a call with a tangent.
     """
     if torch.is_grad_enabled() and q.requires_grad:
+        _refuse_tangent(q)
         o, lse = _without_gradient.apply(q, kv, table, lengths, sm_scale, counts, weight)
         return (o, lse) if want_lse else o
     done = _ordinary("cache4_attention", q, kv, table, lengths, sm_scale, counts, weight, want_lse)
     if done is not None:
         return done if want_lse else done[0]
+    _refuse_tangent(q)                   # the native form does not answer for a tensor that has one
     if q.dtype not in _DTYPES:
         raise ValueError("q must be float16 or bfloat16")
     c, lengths = _cache(kv, table, lengths, q.dtype, weight)

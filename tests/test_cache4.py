@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from ascend_rsfa import _capi
 from ascend_rsfa import flash_attention_forward as fa
@@ -798,3 +799,18 @@ def test_values_with_a_common_offset(cuda_device, dtype, D, Hq, H, S):
     half = 2.0 ** torch.floor(torch.log2(o.abs() + rest)) * HALF_STEP[dtype]
     err = (got.double() - o).abs()
     assert bool((err <= half + rest).all()), (float((err - half - rest).max()), int((err > half + rest).sum()), err.numel())
+
+
+@pytest.mark.gpu
+def test_a_tangent_through_the_attention_raises(cuda_device):
+    """As one through attention() does: nothing would be said of its derivative otherwise."""
+    kv, table, lengths = make(cuda_device, [40], 1, 64, 16, torch.float16)
+    q = rows(cuda_device, (1, 2, 1, 64), torch.float16, 7)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(NotImplementedError):
+            kc.cache4_attention(dual, kv, table, lengths, 0.125)
+        with pytest.raises(NotImplementedError), torch.no_grad():
+            kc.cache4_attention(dual, kv, table, lengths, 0.125)
+        with pytest.raises(NotImplementedError):
+            kc.cache4_attention(forward_ad.make_dual(q.clone().requires_grad_(), torch.ones_like(q)), kv, table, lengths, 0.125)
