@@ -94,7 +94,7 @@ def cache4_append(k, v, kv, table, lengths, counts=None, weight=None, position=N
     """Quantises K and V rows [B, heads, S, D] into the last slots of their sequences.
 
     lengths are the sequences' lengths with the new rows: row j goes to slot lengths[b] - counts[b] + j.
-    counts (int32 [B], default S): rows of sequence b that count, the first ones of a padded batch.  Slots below zero
+    counts (int32 [B], default S): rows of sequence b that count, the first ones of a padded batch.  Slots below zero or behind the pages
     are left out, so a sequence that is not in use has length 0.
     weight is set to 0 for the new tokens, position to positions [B, S] (int32), the number by which
     cache4_evict() knows the newest ones.

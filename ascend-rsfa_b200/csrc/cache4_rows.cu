@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
   const Chunk k = chunk_of<D / kAppendDims>(c, rows.S);
   // rows behind the count are padding; a slot below zero is no token (a sequence that is not in use)
   const int count = rows.counts != nullptr ? min(max(rows.counts[k.b], 0), rows.S) : rows.S;
-  const int to = min(k.tokens, count - k.first);
+  int to = min(k.tokens, count - k.first);
   if (to <= 0) return;
   // The first rows are asked for before the sequence's length and pages are.
   const int64_t* st = k.kv ? rows.v_stride : rows.k_stride;
@@ -161,7 +161,9 @@ __global__ void __launch_bounds__(kThreads) cache4_append_kernel(const Cache4 c,
     }
   };
   load(0);
-  const int slot0 = tokens_of(c, k.b) - count + k.first;       // of the CTA's first token
+  const int slot0 = length_of(c, k.b) - count + k.first;       // of the CTA's first token
+  // of a length beyond the pages the rows behind them are left out, not put in the place of others
+  to = static_cast<int>(min(static_cast<long long>(to), static_cast<long long>(room_of(c)) - slot0));
   const int from = max(0, -slot0);
   if (from >= to) return;
   __shared__ ChunkPages at;

@@ -77,16 +77,16 @@ __device__ __forceinline__ bool find_page(const Cache4& c, int b, int slot, int6
   *page = id;
   return true;
 }
-// Tokens of sequence b, no more than its pages hold.
-__device__ __forceinline__ int tokens_of(const Cache4& c, int b) {
+// Slots of a sequence's pages, 2^30 at most.
+__device__ __forceinline__ int room_of(const Cache4& c) { return c.max_pages << c.page_shift; }
+// What the length of sequence b says, none if it is negative.  The status word is set if it is that or more than the pages hold.
+__device__ __forceinline__ int length_of(const Cache4& c, int b) {
   const int n = c.lengths[b];
-  const int64_t room = static_cast<int64_t>(c.max_pages) << c.page_shift;
-  if (n < 0 || n > room) {
-    report_bad_index(c.status, kTagCacheLength);
-    return n < 0 ? 0 : static_cast<int>(room);
-  }
-  return n;
+  if (n < 0 || n > room_of(c)) report_bad_index(c.status, kTagCacheLength);
+  return max(n, 0);
 }
+// Tokens of sequence b, no more than its pages hold.
+__device__ __forceinline__ int tokens_of(const Cache4& c, int b) { return min(length_of(c, b), room_of(c)); }
 
 }  // namespace
 }  // namespace rsfa

@@ -197,7 +197,7 @@ typedef struct rsfa_cache4 {
 
 /*
  * K and V rows [B,heads,S,D] into the last slots of each sequence: row j < counts[b] (NULL: S) goes to slot
- * lengths[b] - counts[b] + j, so lengths is what they are WITH the new rows; slots below zero are left out.  Per group the
+ * lengths[b] - counts[b] + j, so lengths is what they are WITH the new rows; slots below zero or behind the pages are left out.  Per group the
  * minimum, the scale 16-bit((max - min) / 15) and the nearest codes; a group that holds an infinity or NaN reads back
  * as NaN.  weight is set to 0 and position to positions[b][j] (element strides; given if position is).
  * strides: 8 element strides, k[4], v[4], as rsfa_fwd asks for them.

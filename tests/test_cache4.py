@@ -814,3 +814,31 @@ def test_a_tangent_through_the_attention_raises(cuda_device):
             kc.cache4_attention(dual, kv, table, lengths, 0.125)
         with pytest.raises(NotImplementedError):
             kc.cache4_attention(forward_ad.make_dual(q.clone().requires_grad_(), torch.ones_like(q)), kv, table, lengths, 0.125)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length,counts", [(49, None), (50, [3, 3]), (51, None), (52, None), (2 ** 31 - 1, None), (48 + 2, [1, 1]), (-1, None)])
+def test_append_beyond_the_pages_keeps_what_they_hold(cuda_device, length, counts):
+    """Rows whose slots would be behind the last page are left out, and the rows in front of them keep what they are."""
+    dtype, H, D, page, S, room = torch.bfloat16, 2, 64, 16, 3, 48
+    kv, table, lengths = make(cuda_device, [room, 20], H, D, page, dtype)
+    weight, position = torch.rand(kv.shape[:3], device=cuda_device), torch.zeros(kv.shape[:3], dtype=torch.int32, device=cuda_device)
+    lengths[0] = length
+    k, v = rows(cuda_device, (2, H, S, D), dtype, 1), rows(cuda_device, (2, H, S, D), dtype, 2)
+    positions = torch.full((2, S), 9, dtype=torch.int32, device=cuda_device)
+    want = [t.clone() for t in (kv, weight, position)]
+    for b, n in enumerate((length, 20)):
+        c = S if counts is None else counts[b]
+        for j in range(c):
+            slot = n - c + j
+            if 0 <= slot < room:
+                at = (int(table[b, slot // page]), slice(None), slot % page)
+                want[0][at] = ref.records(k[b, :, j], v[b, :, j])
+                want[1][at], want[2][at] = 0.0, 9
+    fa.device_status()
+    c = None if counts is None else torch.tensor(counts, dtype=torch.int32, device=cuda_device)
+    kc.cache4_append(k, v, kv, table, lengths, counts=c, weight=weight, position=position, positions=positions)
+    with pytest.raises(RuntimeError, match="device status 0x20003"):
+        fa.device_status()
+    for got, exp in zip((kv, weight, position), want):
+        assert torch.equal(got, exp)
