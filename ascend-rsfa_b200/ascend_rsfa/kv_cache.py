@@ -94,8 +94,8 @@ def cache4_append(k, v, kv, table, lengths, counts=None, weight=None, position=N
     """Quantises K and V rows [B, heads, S, D] into the last slots of their sequences.
 
     lengths are the sequences' lengths with the new rows: row j goes to slot lengths[b] - counts[b] + j.
-    counts (int32 [B], default S): rows of sequence b that count, the first ones of a padded batch.  Slots below zero or behind the pages
-    are left out, so a sequence that is not in use has length 0.
+    counts (int32 [B], default S): rows of sequence b that count, the first ones of a padded batch.  Slots below zero
+    or behind the pages are left out, so a sequence that is not in use has length 0.
     weight is set to 0 for the new tokens, position to positions [B, S] (int32), the number by which
     cache4_evict() knows the newest ones.
     """
@@ -220,7 +220,8 @@ def cache4_evict(kv, weight, position, table, lengths, budget, recent=0):
     out = torch.empty_like(lengths)
     if c.batch == 0:
         return out
-    nbytes = _lib.rsfa_cache4_evict_workspace(c.batch, c.heads, budget)
+    # as many records can move as there are slots within the budget, or beyond it
+    nbytes = _lib.rsfa_cache4_evict_workspace(c.batch, c.heads, min(budget, max(c.max_pages * c.page_size - budget, 0)))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
     _call(kv.device, "rsfa_cache4_evict", _lib.rsfa_cache4_evict, ctypes.byref(c), budget, recent, out.data_ptr(), ws.data_ptr(), nbytes)
     return out

@@ -27,7 +27,7 @@ constexpr int kSelectBytes = kKeysInShared * 8 + kPagesInShared * 4;
 constexpr int kMoveThreads = 256;
 constexpr uint32_t kProtected = 0xffffffffu;
 
-__device__ __forceinline__ int64_t moves_at(const Cache4Evict& e, int bh) { return static_cast<int64_t>(bh) * (2ll * e.budget + 2); }
+__device__ __forceinline__ int64_t moves_at(const Cache4Evict& e, int bh) { return static_cast<int64_t>(bh) * (2ll * e.most_moves + 2); }
 
 // Exclusive prefix sum over the block and the block's total.
 template <int kWarps>
@@ -257,8 +257,13 @@ __global__ void __launch_bounds__(kMoveThreads) cache4_move_kernel(const Cache4 
 
 }  // namespace
 
-size_t cache4_evict_workspace(int B, int H, int budget) {
-  return static_cast<size_t>(B) * H * (2ull * budget + 2) * sizeof(int);
+// A record moves from a slot beyond the budget to one within it: no more of them than there are of either.
+int cache4_most_moves(const Cache4& c, int budget) {
+  const int room = c.max_pages << c.page_shift;
+  return room <= budget ? 0 : room - budget < budget ? room - budget : budget;
+}
+size_t cache4_evict_workspace(int B, int H, int most_moves) {
+  return static_cast<size_t>(B) * H * (2ull * most_moves + 2) * sizeof(int);
 }
 
 cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& ev, int sm_count, cudaStream_t stream, long long* launches) {
@@ -281,7 +286,7 @@ cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& ev, int sm_c
   const int pieces = c.D * 5 / 4 / 16 + 1;
   // enough CTAs for a large cut, and no more than its moves could keep busy
   long long each = (8ll * sm_count + heads - 1) / heads;
-  const long long most = (static_cast<long long>(ev.budget) * pieces + kMoveThreads - 1) / kMoveThreads;
+  const long long most = (static_cast<long long>(ev.most_moves) * pieces + kMoveThreads - 1) / kMoveThreads;
   if (each > most) each = most;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(heads), static_cast<unsigned>(each < 1 ? 1 : each));

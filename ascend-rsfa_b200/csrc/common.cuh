@@ -99,6 +99,7 @@ struct Cache4Attention {
 
 struct Cache4Evict {
   int budget, recent;
+  int most_moves;          // of a head; what `moves` has room for
   int* new_lengths;
   int* moves;              // workspace
 };
@@ -163,7 +164,8 @@ struct Cache4Workspace {
 };
 Cache4Workspace cache4_attention_workspace(const Cache4& c, int Hq, int S, int sm_count);
 cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& e, int sm_count, cudaStream_t stream, long long* launches);
-size_t cache4_evict_workspace(int B, int H, int budget);
+int cache4_most_moves(const Cache4& c, int budget);
+size_t cache4_evict_workspace(int B, int H, int most_moves);
 // Adds to the process-wide kernel-launch counter behind rsfa_launch_count().
 void count_launches(long long n);
 // Current values of the "wait_limit_ms" (in ns), "pdl" and "test_drop_load" options.

@@ -248,9 +248,9 @@ int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, floa
   return rsfa::end_call(d, static_cast<cudaStream_t>(stream), e, launches);
 }
 
-long long rsfa_cache4_evict_workspace(int batch, int heads, int budget) {
-  if (batch < 1 || heads < 1 || budget < 1) return RSFA_ERR_INVALID_ARGUMENT;
-  return static_cast<long long>(rsfa::cache4_evict_workspace(batch, heads, budget));
+long long rsfa_cache4_evict_workspace(int batch, int heads, int most_moves) {
+  if (batch < 1 || heads < 1 || most_moves < 0) return RSFA_ERR_INVALID_ARGUMENT;
+  return static_cast<long long>(rsfa::cache4_evict_workspace(batch, heads, most_moves));
 }
 
 int rsfa_cache4_evict(const rsfa_cache4* cache, int budget, int recent, int* new_lengths, void* workspace, long long workspace_bytes,
@@ -261,8 +261,9 @@ int rsfa_cache4_evict(const rsfa_cache4* cache, int budget, int recent, int* new
   if (c.weight == nullptr || c.position == nullptr || new_lengths == nullptr || new_lengths == c.lengths) return RSFA_ERR_INVALID_ARGUMENT;
   if (budget < 1 || recent < 0 || recent > budget || !aligned(new_lengths, 4)) return RSFA_ERR_INVALID_ARGUMENT;
   if (static_cast<double>(c.B) * c.H > static_cast<double>(kMostInt)) return RSFA_ERR_TOO_LARGE;
+  const int most_moves = rsfa::cache4_most_moves(c, budget);
   if (workspace == nullptr || !aligned(workspace, 16) ||
-      workspace_bytes < static_cast<long long>(rsfa::cache4_evict_workspace(c.B, c.H, budget)))
+      workspace_bytes < static_cast<long long>(rsfa::cache4_evict_workspace(c.B, c.H, most_moves)))
     return RSFA_ERR_INVALID_ARGUMENT;
   rsfa::CallScratch d;
   rc = rsfa::begin_call(&d);
@@ -271,6 +272,7 @@ int rsfa_cache4_evict(const rsfa_cache4* cache, int budget, int recent, int* new
   rsfa::Cache4Evict e;
   e.budget = budget;
   e.recent = recent;
+  e.most_moves = most_moves;
   e.new_lengths = new_lengths;
   e.moves = static_cast<int*>(workspace);
   long long launches = 0;

@@ -10,6 +10,7 @@
 // So nothing is accepted, refused or seen by a mode differently than without this file.
 #include <Python.h>
 
+#include <algorithm>
 #include <cstring>
 #include <optional>
 
@@ -522,7 +523,9 @@ PyObject* cache4_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
   rsfa_cache4 c;
   if (!plain_cache(args[0], args[3], args[4], args[1], args[2], RSFA_DTYPE_F16, device, &c)) Py_RETURN_NONE;
   const at::Tensor& lengths = THPVariable_Unpack(args[4]);
-  const long long bytes = g_ops.evict_workspace(c.batch, c.heads, budget);
+  // as many records can move as there are slots within the budget, or beyond it
+  const int64_t beyond = std::max<int64_t>(static_cast<int64_t>(c.max_pages) * c.page_size - budget, 0);
+  const long long bytes = g_ops.evict_workspace(c.batch, c.heads, static_cast<int>(std::min<int64_t>(budget, beyond)));
   if (bytes < 0) Py_RETURN_NONE;
   at::Tensor out = at::empty({c.batch}, lengths.options());
   at::Tensor scratch = at::empty({bytes}, lengths.options().dtype(at::kByte));

@@ -197,9 +197,9 @@ typedef struct rsfa_cache4 {
 
 /*
  * K and V rows [B,heads,S,D] into the last slots of each sequence: row j < counts[b] (NULL: S) goes to slot
- * lengths[b] - counts[b] + j, so lengths is what they are WITH the new rows; slots below zero or behind the pages are left out.  Per group the
- * minimum, the scale 16-bit((max - min) / 15) and the nearest codes; a group that holds an infinity or NaN reads back
- * as NaN.  weight is set to 0 and position to positions[b][j] (element strides; given if position is).
+ * lengths[b] - counts[b] + j, so lengths is what they are WITH the new rows; slots below zero or behind the
+ * pages are left out.  Per group the minimum, the scale 16-bit((max - min) / 15) and the nearest codes; a group
+ * that holds an infinity or NaN reads back as NaN.  weight is set to 0 and position to positions[b][j] (element strides; given if position is).
  * strides: 8 element strides, k[4], v[4], as rsfa_fwd asks for them.
  */
 RSFA_API int rsfa_cache4_append(const rsfa_cache4* cache, const void* k, const void* v, int S, const int64_t* strides,
@@ -232,9 +232,10 @@ RSFA_API int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void
  * weight that is negative or NaN counts as none.  Kept records beyond slot `budget` move, with weight and position, into
  * the slots below that are given up, both in rising order; nothing else is written.  new_lengths[b] =
  * min(lengths[b], budget), which is not lengths itself: other layers' caches may still need that.  0 <= recent <= budget.
- * No page may belong to two sequences.  workspace as above.
+ * No page may belong to two sequences.  workspace as above, for
+ * most_moves = min(budget, max_pages * page_size - budget), 0 where that is negative: no more records of a head can move.
  */
-RSFA_API long long rsfa_cache4_evict_workspace(int batch, int heads, int budget);
+RSFA_API long long rsfa_cache4_evict_workspace(int batch, int heads, int most_moves);
 RSFA_API int rsfa_cache4_evict(const rsfa_cache4* cache, int budget, int recent, int* new_lengths, void* workspace,
                                long long workspace_bytes, void* stream);
 

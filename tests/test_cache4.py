@@ -842,3 +842,33 @@ def test_append_beyond_the_pages_keeps_what_they_hold(cuda_device, length, count
         fa.device_status()
     for got, exp in zip((kv, weight, position), want):
         assert torch.equal(got, exp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("route", ["native", "python"])
+@pytest.mark.parametrize("budget", [2 ** 31 - 1, 1024, 1 << 12, (1 << 12) - 1])
+def test_scratch_of_an_eviction_goes_by_what_can_move(cuda_device, monkeypatch, route, budget):
+    """A budget at or above what the table has room for moves nothing, one a slot below it one record per head at most."""
+    if route == "python":
+        monkeypatch.setattr(ro, "_native", None)
+    B, H, D, page, n = 2, 4, 64, 64, 1 << 12
+    kv, weight, position = kc.cache4_empty(B * n // page, H, page, D, device=cuda_device)
+    table = torch.arange(B * n // page, dtype=torch.int32, device=cuda_device).view(B, -1)
+    lengths = torch.tensor([n, 100], dtype=torch.int32, device=cuda_device)
+    kv.random_(0, 256)
+    weight.random_(1, 1000)
+    position.copy_(torch.arange(B * n, dtype=torch.int32, device=cuda_device).view(-1, 1, page).expand_as(position))
+    want = kv.clone()
+    slot = torch.arange(n, device=cuda_device)
+    for h in range(H):
+        moves, _ = ref.evict(weight[:n // page, h].flatten(), slot, budget, 5)
+        for to, source in moves:
+            want[to // page, h, to % page] = kv[source // page, h, source % page]
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    new = kc.cache4_evict(kv, weight, position, table, lengths, budget, 5)
+    most = min(budget, max(n - budget, 0))
+    assert torch.cuda.max_memory_allocated() - before <= B * H * 8 * (most + 2) + 2048
+    assert new.tolist() == [min(n, budget), 100] and torch.equal(kv, want)
+    fa.device_status()
