@@ -21,7 +21,7 @@ _native = _rsfa_torch   # the ordinary calls in native code (csrc/torch_binding.
 if _native is not None:
     _native.bind_ops(*(ctypes.cast(getattr(_lib, "rsfa_" + n), ctypes.c_void_p).value for n in (
         "rotary", "cache4_append", "cache4_read", "cache4_attention_workspace", "cache4_attention",
-        "cache4_evict_workspace", "cache4_evict")))
+        "cache4_evict_workspace", "cache4_evict", "strerror")))
 _TURNS = {"yarn": (1.0, 32.0), "bands": (1.0, 4.0)}   # usual (low, high) numbers of turns over the original length
 
 

@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cstring>
 #include <optional>
+#include <string>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
@@ -149,7 +150,17 @@ struct Ops {
   decltype(&rsfa_cache4_attention) attention = nullptr;
   decltype(&rsfa_cache4_evict_workspace) evict_workspace = nullptr;
   decltype(&rsfa_cache4_evict) evict = nullptr;
+  decltype(&rsfa_strerror) strerror = nullptr;
 } g_ops;
+
+// Raises what _capi.check() raises for a code of the library, where there is no Python caller to hand it to.
+void check_code(int rc, const char* what) {
+  if (rc == RSFA_OK) return;
+  const std::string message = std::string(what) + " failed: " + g_ops.strerror(rc) + " (code " + std::to_string(rc) + ")";
+  TORCH_CHECK_VALUE(rc != RSFA_ERR_INVALID_ARGUMENT && rc != RSFA_ERR_TOO_LARGE, message);
+  TORCH_CHECK_NOT_IMPLEMENTED(rc != RSFA_ERR_UNSUPPORTED, message);
+  TORCH_CHECK(false, message);
+}
 
 // The current device, if the tensor lives on it; -1: it does not (there may be no device at all).
 int device_of(PyObject* obj) {
@@ -258,8 +269,7 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
                                                 const at::Tensor& table, const std::optional<at::Tensor>& pos_or, bool interleaved, bool inverse) {
     const at::Tensor k = k_or.value_or(at::Tensor()), pos = pos_or.value_or(at::Tensor());
     at::Tensor qo, ko;
-    const int rc = turn(q, k, table, pos, interleaved, inverse, &qo, &ko);
-    TORCH_CHECK(rc == 0, "rsfa_rotary failed with code ", rc);
+    check_code(turn(q, k, table, pos, interleaved, inverse, &qo, &ko), "rsfa_rotary");
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({table, pos});
     ctx->saved_data["interleaved"] = interleaved;
@@ -300,8 +310,7 @@ struct RotaryFunction : public torch::autograd::Function<RotaryFunction> {
       if (second.defined()) *b = again[1];
       return;
     }
-    const int rc = turn(first, second, saved[0], saved[1], interleaved, inverse, a, b);
-    TORCH_CHECK(rc == 0, "rsfa_rotary failed with code ", rc);
+    check_code(turn(first, second, saved[0], saved[1], interleaved, inverse, a, b), "rsfa_rotary");
   }
   static at::Tensor primal(const at::Tensor& t) { return tangent_of(t).defined() ? t._fw_primal(0) : t; }
   static std::optional<at::Tensor> given(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
@@ -541,12 +550,12 @@ PyObject* cache4_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // bind_ops(addresses of the functions of Ops, in its order)
 PyObject* bind_ops(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "bind_ops takes seven addresses");
+  if (n != 8) {
+    PyErr_SetString(PyExc_TypeError, "bind_ops takes eight addresses");
     return nullptr;
   }
-  void* p[7];
-  for (int i = 0; i < 7; ++i) {
+  void* p[8];
+  for (int i = 0; i < 8; ++i) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (p[i] == nullptr && PyErr_Occurred()) return nullptr;
   }
@@ -557,6 +566,7 @@ PyObject* bind_ops(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_ops.attention = reinterpret_cast<decltype(g_ops.attention)>(p[4]);
   g_ops.evict_workspace = reinterpret_cast<decltype(g_ops.evict_workspace)>(p[5]);
   g_ops.evict = reinterpret_cast<decltype(g_ops.evict)>(p[6]);
+  g_ops.strerror = reinterpret_cast<decltype(g_ops.strerror)>(p[7]);
   Py_RETURN_NONE;
 }
 

@@ -273,3 +273,32 @@ def test_forward_mode(cuda_device, monkeypatch, route, interleaved):
                 close(primal, d, table, turned(d, True), torch.bfloat16, pos, interleaved, True)
                 close(tangent, dd, table, turned(dd, True), torch.bfloat16, pos, interleaved, True)
     fa.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("route", ["native", "python"])
+def test_refusals_of_the_library_with_a_gradient_recorded(cuda_device, monkeypatch, route):
+    """The same errors with and without a gradient, and by either route."""
+    if route == "python":
+        monkeypatch.setattr(ro, "_native", None)
+    q = torch.zeros(1, 65536, 1, 16, dtype=torch.float16, device=cuda_device)
+    table = ro.rotary_table(4, 16, device=cuda_device)
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="rsfa_rotary failed: problem too large"):
+            ro.rotary(x, None, table)
+    q = torch.zeros(1, 2, 1, 16, dtype=torch.float16, device=cuda_device, requires_grad=True)
+    good = ro.rotary(q, None, table)[0]
+    fa.device_status()
+    try:
+        fa.set_option("check_status", 1)
+        ro.rotary(q.detach(), None, table, torch.tensor([9], device=cuda_device))
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="rsfa_rotary failed: a kernel reported"):
+            ro.rotary(q, None, table)
+        with pytest.raises(RuntimeError, match="rsfa_rotary failed: a kernel reported"):
+            good.sum().backward()
+        with pytest.raises(RuntimeError, match="0x20001"):
+            fa.device_status()
+    finally:
+        fa.set_option("check_status", 0)
+    fa.device_status()
