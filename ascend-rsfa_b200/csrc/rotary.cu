@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, 
   if (!known && chunk == 0 && blockIdx.y == 0) report_bad_index(p.status, kTagRotaryPosition);
   const float2* table = reinterpret_cast<const float2*>(p.table) + (known ? pos : 0) * (p.R >> 1);
   const float sign = p.inverse ? -1.f : 1.f;
-  const float lost = known ? 0.f : __int_as_float(0x7fffffff);   // a row without a position comes out as NaN
+  const float lost = known ? 0.f : __int_as_float(0x7fffffff);   // a row without a position comes out as NaN,
+  const uint32_t lost16 = known ? 0u : 0x7fff7fffu;               // in either type, where it is copied as well
 
   constexpr int kPairs = kWide ? (kInterleaved ? 4 : 8) : 1;
   float2 cs[8];
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, 
               *reinterpret_cast<uint4*>(dst[i] + half) = c[i];
             }
           }
+          if (!turns) a[i].x |= lost16, a[i].y |= lost16, a[i].z |= lost16, a[i].w |= lost16;
           *reinterpret_cast<uint4*>(dst[i]) = a[i];
         }
       }
@@ -130,6 +132,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p, 
         const float x = to_f32<kBf16>(a), y = to_f32<kBf16>(c);
         a = from_f32<kBf16>(x * cs[0].x - y * cs[0].y);
         c = from_f32<kBf16>(y * cs[0].x + x * cs[0].y);
+      } else {
+        a |= lost16;
+        c |= lost16;
       }
       dst[0] = a;
       dst[other] = c;

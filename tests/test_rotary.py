@@ -302,3 +302,21 @@ def test_refusals_of_the_library_with_a_gradient_recorded(cuda_device, monkeypat
     finally:
         fa.set_option("check_status", 0)
     fa.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,R", [(64, 32), (128, 16), (64, 6), (32, 20), (256, 2), (16, 16)])
+def test_the_whole_row_of_a_position_outside_the_table_is_nan(cuda_device, dtype, interleaved, D, R):
+    table = ro.rotary_table(16, R, device=cuda_device)
+    q, k = (torch.randn(2, h, 5, D, device=cuda_device).to(dtype) for h in (3, 18))
+    pos = torch.tensor([[0, 16, 15, -1, 3], [2 ** 31 - 1, 1, 2, 3, -2 ** 31]], device=cuda_device, dtype=torch.int32)
+    fa.device_status()
+    lost = ((pos < 0) | (pos >= 16))[:, None, :, None]
+    for x, y in zip((q, k), ro.rotary(q, k, table, pos, interleaved)):
+        assert torch.equal(y.isnan(), lost.expand_as(y))
+        assert torch.equal(torch.where(lost, 0, y)[..., R:], torch.where(lost, 0, x)[..., R:])
+    with pytest.raises(RuntimeError, match="device status 0x20001"):
+        fa.device_status()
+    fa.device_status()
