@@ -1036,6 +1036,18 @@ __global__ void __launch_bounds__(kWeightThreads) cache4_weight_kernel(const Cac
           sum[3] += ex2(v[r].w - of_row);
         }
       }
+      if (__any_sync(0xffffffffu, lse != lse)) {               // a row is NaN: the tokens that it does not see are not
+        sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+#pragma unroll 1
+        for (int r = 0; r < rows.count; ++r) {
+          const float of_row = __shfl_sync(0xffffffffu, lse, r);
+          const float4 x = *reinterpret_cast<const float4*>(scores + r * kTile);
+          if (x.x != -INFINITY) sum[0] += ex2(x.x - of_row);
+          if (x.y != -INFINITY) sum[1] += ex2(x.y - of_row);
+          if (x.z != -INFINITY) sum[2] += ex2(x.z - of_row);
+          if (x.w != -INFINITY) sum[3] += ex2(x.w - of_row);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (j < live) weight[j] = old[j] + sum[j];

@@ -872,3 +872,25 @@ def test_scratch_of_an_eviction_goes_by_what_can_move(cuda_device, monkeypatch, 
     assert torch.cuda.max_memory_allocated() - before <= B * H * 8 * (most + 2) + 2048
     assert new.tolist() == [min(n, budget), 100] and torch.equal(kv, want)
     fa.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D,Hq,H", [(64, 4, 4), (128, 8, 2)])
+def test_weights_of_tokens_that_a_nan_row_does_not_see(cuda_device, wide, D, Hq, H):
+    """The first of two query tokens is NaN: the tokens that it sees get NaN, the last one the second token's weight alone.  With
+    scores that are kept and, for a table far wider than the cache, ones that are computed again."""
+    n, page = 37, 16
+    kv, table, lengths = make(cuda_device, [n], H, D, page, torch.float16)
+    if wide:
+        table = torch.cat((table, torch.full((1, 4096), -1, dtype=torch.int32, device=cuda_device)), 1)
+    q = rows(cuda_device, (1, Hq, 2, D), torch.float16, 1)
+    weight, want = (torch.zeros(kv.shape[:3], device=cuda_device) for _ in range(2))
+    kc.cache4_attention(q, kv, table, lengths, 0.1, weight=want)
+    last = (int(table[0, (n - 1) // page]), slice(None), (n - 1) % page)
+    want, weight = want[last].clone(), torch.zeros_like(weight)
+    q[:, :, 0, 3] = math.nan
+    kc.cache4_attention(q, kv, table, lengths, 0.1, weight=weight)
+    slot = torch.arange(n - 1, device=cuda_device)
+    assert bool(weight[table[0].long()[slot // page], :, slot % page].isnan().all())
+    assert torch.equal(weight[last], want) and bool((want > 0).all())
