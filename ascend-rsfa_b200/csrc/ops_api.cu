@@ -81,6 +81,20 @@ int take_rows(const rsfa::Cache4& c, void* k, void* v, int S, const int64_t* str
   return RSFA_OK;
 }
 
+// Query rows of all heads are counted in 32 bits, and so is a warp's share of all tiles (of 32 tokens or more, for 8 query rows
+// or more).
+bool countable(const rsfa::Cache4& c, int q_heads, int S) {
+  const double tiles = std::ceil(static_cast<double>(c.max_pages) * (1 << c.page_shift) / 32.0) + 2.0;
+  return static_cast<double>(c.B) * q_heads * S <= static_cast<double>(kMostInt) &&
+         c.B * std::ceil(static_cast<double>(q_heads / c.H) * S / 8.0) * c.H * tiles <= kMostTiles;
+}
+
+// Heads of all sequences are counted in 32 bits, the bytes of their moves in 64.
+bool movable(int batch, int heads, int most_moves) {
+  const double all = static_cast<double>(batch) * heads;
+  return all <= static_cast<double>(kMostInt) && all * (2.0 * most_moves + 2.0) * sizeof(int) < 9.0e18;
+}
+
 }  // namespace
 
 extern "C" {
@@ -200,6 +214,7 @@ long long rsfa_cache4_attention_workspace(const rsfa_cache4* cache, int q_heads,
   const int rc = take_cache(cache, &c);
   if (rc != RSFA_OK) return rc;
   if (q_heads < c.H || q_heads % c.H != 0 || S < 1) return RSFA_ERR_INVALID_ARGUMENT;
+  if (!countable(c, q_heads, S)) return RSFA_ERR_TOO_LARGE;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) {
     cudaGetLastError();
@@ -218,10 +233,7 @@ int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, floa
   if (q_heads < c.H || q_heads % c.H != 0 || S < 1 || strides == nullptr || !(sm_scale == sm_scale)) return RSFA_ERR_INVALID_ARGUMENT;
   if (!valid_tensor(q, strides, c.B, q_heads, S, c.D) || !valid_tensor(o, strides + 4, c.B, q_heads, S, c.D)) return RSFA_ERR_INVALID_ARGUMENT;
   if (!aligned(lse, 4) || !aligned(counts, 4) || (c.weight != nullptr && lse == nullptr)) return RSFA_ERR_INVALID_ARGUMENT;
-  if (static_cast<double>(c.B) * q_heads * S > static_cast<double>(kMostInt)) return RSFA_ERR_TOO_LARGE;
-  // a warp's share of all tiles (of 32 tokens or more, for 8 query rows or more) is counted in 32 bits
-  const double tiles = std::ceil(static_cast<double>(c.max_pages) * (1 << c.page_shift) / 32.0) + 2.0;
-  if (c.B * std::ceil(static_cast<double>(q_heads / c.H) * S / 8.0) * c.H * tiles > kMostTiles) return RSFA_ERR_TOO_LARGE;
+  if (!countable(c, q_heads, S)) return RSFA_ERR_TOO_LARGE;
   rsfa::CallScratch d;
   rc = rsfa::begin_call(&d);
   if (rc != RSFA_OK) return rc;
@@ -250,6 +262,7 @@ int rsfa_cache4_attention(const rsfa_cache4* cache, const void* q, void* o, floa
 
 long long rsfa_cache4_evict_workspace(int batch, int heads, int most_moves) {
   if (batch < 1 || heads < 1 || most_moves < 0) return RSFA_ERR_INVALID_ARGUMENT;
+  if (!movable(batch, heads, most_moves)) return RSFA_ERR_TOO_LARGE;
   return static_cast<long long>(rsfa::cache4_evict_workspace(batch, heads, most_moves));
 }
 
@@ -260,8 +273,8 @@ int rsfa_cache4_evict(const rsfa_cache4* cache, int budget, int recent, int* new
   if (rc != RSFA_OK) return rc;
   if (c.weight == nullptr || c.position == nullptr || new_lengths == nullptr || new_lengths == c.lengths) return RSFA_ERR_INVALID_ARGUMENT;
   if (budget < 1 || recent < 0 || recent > budget || !aligned(new_lengths, 4)) return RSFA_ERR_INVALID_ARGUMENT;
-  if (static_cast<double>(c.B) * c.H > static_cast<double>(kMostInt)) return RSFA_ERR_TOO_LARGE;
   const int most_moves = rsfa::cache4_most_moves(c, budget);
+  if (!movable(c.B, c.H, most_moves)) return RSFA_ERR_TOO_LARGE;
   if (workspace == nullptr || !aligned(workspace, 16) ||
       workspace_bytes < static_cast<long long>(rsfa::cache4_evict_workspace(c.B, c.H, most_moves)))
     return RSFA_ERR_INVALID_ARGUMENT;

@@ -894,3 +894,14 @@ def test_weights_of_tokens_that_a_nan_row_does_not_see(cuda_device, wide, D, Hq,
     slot = torch.arange(n - 1, device=cuda_device)
     assert bool(weight[table[0].long()[slot // page], :, slot % page].isnan().all())
     assert torch.equal(weight[last], want) and bool((want > 0).all())
+
+
+def test_the_workspace_query_refuses_what_the_call_refuses():
+    too_large = _capi.RSFA_ERR_TOO_LARGE
+    assert lib.rsfa_cache4_attention_workspace(c_cache(), 64, 1 << 30) == too_large
+    assert lib.rsfa_cache4_attention_workspace(c_cache(batch=1 << 20, max_pages=1 << 26, table_stride=0), 2, 4) == too_large
+    p = ctypes.c_void_p(4096)
+    assert lib.rsfa_cache4_evict_workspace(1 << 16, 1 << 15, 8) == too_large
+    assert lib.rsfa_cache4_evict_workspace(1 << 16, (1 << 15) - 1, (1 << 31) - 1) == too_large
+    c = c_cache(batch=1 << 16, heads=(1 << 15) - 1, max_pages=1 << 26, table_stride=0, kv_stride=(1 << 40, 1280), weight_stride=(1 << 20, 16), position_stride=(1 << 20, 16))
+    assert lib.rsfa_cache4_evict(c, 1 << 29, 2, ctypes.c_void_p(8192), p, 1 << 62, None) == too_large
