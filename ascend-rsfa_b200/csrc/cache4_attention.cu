@@ -60,6 +60,7 @@ constexpr int kTagCache4Load = 40;   // of a bounded wait, in the status word
 // one of 60000, results off by 2.4e-4, 2.6e-4 and 2.5e-4; raised only eight units above, the first and the last: 2.8e-4 and 3.5e-4).
 constexpr float kHeadroom = 10.f, kRaise = 11.f;
 constexpr float kRaiseScale = 4.f;
+constexpr float kFar = 256.f;        // see raise()
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -423,7 +424,7 @@ struct Sums {
   float mids[NT][4];           // sum p m of group g % G, rows 2 c, 2 c + 1, then sum p s
   float l[NT][2], ref[NT][2];
   float unit;                  // power of two that s is divided by
-  uint32_t per_unit;           // 1 / unit, a 16-bit number of the cache's type
+  uint32_t per_unit;           // 1 / unit, a 16-bit number of the cache's type; bf16: above it the unit that others are held against (raise)
   uint32_t unit_limit;         // 16-bit pattern of the scale from which on it is raised
 };
 // 1 / unit has to be a number of the cache's type: 2^-15 and 2^-100.  Scales below that are fp16's subnormal ones.
@@ -542,41 +543,6 @@ __device__ __forceinline__ void block_output(Sums<D, NT>& x, const float (&p)[NT
   }
 }
 
-// Raises the references of the rows to the largest score of a tile, and the unit to its widest scale.  Both in one
-// place: with a branch each the sums were copied from register to register in every tile (16 of 344 instructions per 16
-// tokens).
-template <int D, int NT, bool kBf16>
-__device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2], uint32_t widest) {
-  float scale = to_f32<kBf16>(static_cast<uint16_t>(widest));      // finite
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, d));
-  // the power of two below it, where it is above what the unit is for
-  const float unit = scale > x.unit * kRaiseScale ? __uint_as_float(__float_as_uint(scale) & 0x7f800000u) : x.unit;
-  const float by_unit = x.unit / unit;
-  x.unit = unit;
-  x.per_unit = from_f32<kBf16>(1.f / unit);
-  x.unit_limit = from_f32<kBf16>(unit * kRaiseScale);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float m = top[nt][i];
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      const float ref = m > x.ref[nt][i] + kRaise ? m - kHeadroom : x.ref[nt][i];
-      const float by = ex2(x.ref[nt][i] - ref), by_both = by * by_unit;
-      x.ref[nt][i] = ref;
-      x.l[nt][i] *= by;
-      x.mids[nt][i] *= by;
-      x.mids[nt][i + 2] *= by;
-#pragma unroll
-      for (int j = 0; j < 2 * (D / 32); ++j) {
-        x.o[j][nt][i] *= by_both;
-        x.o[j][nt][i + 2] *= by_both;
-      }
-    }
-}
-
 // What the widest finite scale of a lane's share of a tile is (see one_tile), where one that is not finite hides it.
 template <int D, bool kBf16>
 __device__ __noinline__ uint32_t widest_finite(const uint8_t* rec) {
@@ -590,6 +556,123 @@ __device__ __noinline__ uint32_t widest_finite(const uint8_t* rec) {
       if (scale < (kBf16 ? 0x7f80u : 0x7c00u)) widest = max(widest, scale);
     }
   return widest;
+}
+
+// The narrowest scale of a tile that is one (a group without a range has none); infinity: there is none.
+template <int D, bool kBf16>
+__device__ __noinline__ float narrowest(const uint8_t* rec) {
+  using R = Record<D>;
+  constexpr int G = D / 32;
+  constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
+  uint32_t least = kInf;               // as integers, less one: zero comes last
+  for (int token = threadIdx.x & 31; token < tile_tokens(D); token += 32)
+#pragma unroll
+    for (int w = 0; w < G; w += 2) {
+      const uint2 pairs = *reinterpret_cast<const uint2*>(rec + token * R::kBytes + R::kVPairs + 4 * w);
+      least = min(least, min((pairs.x & 0xffffu) - 1u, (pairs.y & 0xffffu) - 1u));
+    }
+  least = __reduce_min_sync(0xffffffffu, least);
+  return least >= kInf - 1u ? INFINITY : to_f32<kBf16>(static_cast<uint16_t>(least + 1u));
+}
+// log2 of the largest p * s of 16 tokens per query row, from log2 p of tokens (g, g + 8), against what `most` holds.
+template <int D, int NT, bool kBf16>
+__device__ __noinline__ void largest_products(const uint8_t* rec, const float* p, float* most) {
+  using R = Record<D>;
+  constexpr int G = D / 32;
+  const int g = (threadIdx.x & 31) >> 2;
+  for (int i = 0; i < 2; ++i) {
+    float widest = 0.f;
+    for (int w = 0; w < G; ++w) {
+      const float scale = to_f32<kBf16>(*reinterpret_cast<const uint16_t*>(rec + (g + 8 * i) * R::kBytes + R::kVPairs + 4 * w));
+      if (scale < INFINITY) widest = fmaxf(widest, scale);
+    }
+    for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < 2; ++j) most[2 * nt + j] = fmaxf(most[2 * nt + j], p[4 * nt + 2 * i + j] + __log2f(widest));
+  }
+}
+
+// Raises the references of the rows to the largest score of a tile, and the unit to its widest scale.  Both in one
+// place: with a branch each the sums were copied from register to register in every tile (16 of 344 instructions per 16
+// tokens).
+//
+// The unit is all rows', and a row whose own scales are far below it has its products rounded away: fp16's range from
+// 2^13 down to 2^-24 is enough for scales that are fp16 numbers themselves, those of bf16 can be 2^40 apart, in a token that the
+// row does not see.  So in bf16 a scale more than kFar above the narrowest of the first tile raises the unit only to where each
+// row's largest product of the tile is still 2^0; a row with larger products than fp16 holds gets a higher reference instead.
+template <int D, int NT, bool kBf16>
+__device__ __forceinline__ void raise(Sums<D, NT>& x, const float (&top)[NT][2], uint32_t widest, const float (&s)[tile_tokens(D) / 16][NT][4],
+                                      const Query<D, NT>& f, const uint8_t* rec) {
+  auto power_below = [](float v) { return __uint_as_float(__float_as_uint(v) & 0x7f800000u); };
+  const float scale = to_f32<kBf16>(static_cast<uint16_t>(__reduce_max_sync(0xffffffffu, widest)));   // finite
+  // the power of two below it, where it is above what the unit is for
+  float unit = scale > x.unit * kRaiseScale ? power_below(scale) : x.unit;
+  float ref[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float m = top[nt][i];
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      ref[nt][i] = m > x.ref[nt][i] + kRaise ? m - kHeadroom : x.ref[nt][i];
+    }
+  if constexpr (kBf16) {
+    if (unit > x.unit) {
+      float base = __uint_as_float(x.per_unit & 0xffff0000u);
+      if (base == 0.f) base = power_below(narrowest<D, kBf16>(rec));
+      if (unit > base * kFar) {
+        float most[2 * NT], least = INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) most[i] = -INFINITY;
+        for (int k = 0; k < tile_tokens(D) / 16; ++k) {
+          float p[4 * NT];
+#pragma unroll
+          for (int j = 0; j < 4 * NT; ++j) {
+            float score = s[0][j / 4][j % 4];
+#pragma unroll
+            for (int t = 1; t < tile_tokens(D) / 16; ++t)
+              if (t == k) score = s[t][j / 4][j % 4];
+            p[j] = fmaf(score, f.factor[j / 4][j & 1], -ref[j / 4][j & 1]);
+          }
+          largest_products<D, NT, kBf16>(rec + 16 * k * Record<D>::kBytes, p, most);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+          for (int d = 4; d < 32; d <<= 1) most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], d));
+          if (most[i] > -INFINITY) least = fminf(least, most[i]);  // a row that sees something
+        }
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 1));
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 2));
+        const int exponent = static_cast<int>(floorf(fminf(fmaxf(least, -100.f), 125.f)));
+        // no less than what makes scale / unit a 32-bit number
+        unit = fmaxf(fmaxf(x.unit, unit * 7.5231638452626401e-37f), fminf(unit, fmaxf(base, __uint_as_float(static_cast<uint32_t>(127 + exponent) << 23))));
+        const float log2_unit = static_cast<float>(static_cast<int>(__float_as_uint(unit) >> 23) - 127);
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) ref[i / 2][i % 2] += fmaxf(ceilf(most[i] - log2_unit - 13.f), 0.f);
+        base = unit;
+      }
+      x.per_unit = __float_as_uint(base);
+    }
+  }
+  const float by_unit = x.unit / unit;
+  x.unit = unit;
+  x.per_unit = (kBf16 ? x.per_unit & 0xffff0000u : 0u) | from_f32<kBf16>(1.f / unit);
+  x.unit_limit = from_f32<kBf16>(unit * kRaiseScale);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float by = ex2(x.ref[nt][i] - ref[nt][i]), by_both = by * by_unit;
+      x.ref[nt][i] = ref[nt][i];
+      x.l[nt][i] *= by;
+      x.mids[nt][i] *= by;
+      x.mids[nt][i + 2] *= by;
+#pragma unroll
+      for (int j = 0; j < 2 * (D / 32); ++j) {
+        x.o[j][nt][i] *= by_both;
+        x.o[j][nt][i + 2] *= by_both;
+      }
+    }
 }
 
 // One tile at `rec`, whose first slot is `slot`.  scores: where the tile's scores are kept, null: nowhere.
@@ -634,7 +717,7 @@ __device__ __forceinline__ bool one_tile(Sums<D, NT>& x, const Query<D, NT>& f, 
   if (__any_sync(0xffffffffu, higher || widest > x.unit_limit)) {
     odd = __any_sync(0xffffffffu, widest >= (kBf16 ? 0x7f80u : 0x7c00u));
     if (odd) widest = widest_finite<D, kBf16>(rec);
-    raise<D, NT, kBf16>(x, top, widest);
+    raise<D, NT, kBf16>(x, top, widest, s, f, rec);
   }
   if (scores != nullptr) {
 #pragma unroll

@@ -905,3 +905,38 @@ def test_the_workspace_query_refuses_what_the_call_refuses():
     assert lib.rsfa_cache4_evict_workspace(1 << 16, (1 << 15) - 1, (1 << 31) - 1) == too_large
     c = c_cache(batch=1 << 16, heads=(1 << 15) - 1, max_pages=1 << 26, table_stride=0, kv_stride=(1 << 40, 1280), weight_stride=(1 << 20, 16), position_stride=(1 << 20, 16))
     assert lib.rsfa_cache4_evict(c, 1 << 29, 2, ctypes.c_void_p(8192), p, 1 << 62, None) == too_large
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 2.0 ** 12), (torch.bfloat16, 2.0 ** 40), (torch.bfloat16, 2.0 ** 100), (torch.bfloat16, 2.0 ** -60)])
+@pytest.mark.parametrize("at", [0, 0.6, 1])
+@pytest.mark.parametrize("D,Hq,n", [(64, 2, 9), (64, 8, 300), (128, 3, 9), (128, 8, 300), (128, 16, 20000), (256, 2, 9), (256, 2, 150)])
+def test_a_row_of_v_of_another_size(cuda_device, dtype, size, at, D, Hq, n):
+    """One slot's V is `size` times as large as the others.  The second of two query tokens gives it no weight in its even heads (a
+    score far below the others) and rests on it in the odd ones; the first weighs it like any other, or does not see it where it
+    is the last.  Each result is as good as if there were no other rows."""
+    pages, slot = n // 16 + 1, int(at * (n - 1))
+    kv, weight, position = kc.cache4_empty(pages, 1, 16, D, device=cuda_device)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda_device)[None]
+    lengths = torch.tensor([n], dtype=torch.int32, device=cuda_device)
+    k, v, q = (rows(cuda_device, s, dtype, i) for i, s in enumerate(((1, 1, n, D), (1, 1, n, D), (1, Hq, 2, D))))
+    k[:, :, slot, 0] = 100
+    q[..., 0] = 0
+    q[:, ::2, 1, 0], q[:, 1::2, 1, 0] = -20, 20
+    v[:, :, slot] *= size
+    kc.cache4_append(k, v, kv, table, lengths)
+    got, lse = kc.cache4_attention(q, kv, table, lengths, 1.0, want_lse=True)
+    o, bound = attention_bound(q, kv, table, lengths, 1.0)
+    widest = ref.records(k.reshape(n, D), v.reshape(n, D))[:, -(D // 8):].contiguous().view(dtype)[:, ::2].max()
+    if size < 1:
+        # A product p * s that is no more than half of fp16's smallest step, 2^-25, is lost, times |u - 8| <= 8, where the weights
+        # add up to 2^10 at least, in units of the widest scale at most: a row of small values is as good as these allow.
+        bound = bound + n * 2.0 ** -32 * float(widest)
+    assert bool(((got.double() - o).abs() <= bound).all())
+    # A code is an fp16 number below 2^-14, a query's largest element one of 2^10 to 2^11, and an MMA cuts 16 products and their
+    # sum so far off at 2^-24 of what these exponents allow, 2^-3: a score is off by 17 * 2^-27 for codes that count 2^-24 and
+    # queries that count 2^-10 of their largest, once for the codes at the bottom and 1/16 of it for the others, per group.
+    _, want, _, (_, _, _, _, terms) = ref.attention(q, kv, table, lengths, 1.0)
+    scales = ref.records(k.reshape(n, D), v.reshape(n, D))[:, D:D + D // 8].contiguous().view(dtype)[:, ::2].double()
+    cut = 18.1 * 2.0 ** -13 * q.double().abs().amax(-1) * scales.sum(-1).max()
+    assert bool(((lse.double() - want).abs() <= 2.0 ** -19 * (1 + terms) + cut + 2.0 ** -22 * want.abs() + 2.0 ** -20).all())
