@@ -940,3 +940,91 @@ def test_a_row_of_v_of_another_size(cuda_device, dtype, size, at, D, Hq, n):
     scales = ref.records(k.reshape(n, D), v.reshape(n, D))[:, D:D + D // 8].contiguous().view(dtype)[:, ::2].double()
     cut = 18.1 * 2.0 ** -13 * q.double().abs().amax(-1) * scales.sum(-1).max()
     assert bool(((lse.double() - want).abs() <= 2.0 ** -19 * (1 + terms) + cut + 2.0 ** -22 * want.abs() + 2.0 ** -20).all())
+
+
+# ------------------------------------------------------------------ shares of many tiles
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype,D,Hq,S,lengths", [
+    (torch.float16, 64, 16, 1, [41000, 31000, 0, 77]), (torch.bfloat16, 128, 32, 2, [31000, 77, 41000]), (torch.bfloat16, 64, 160, 1, [30000, 18000]),
+    (torch.float16, 128, 96, 2, [5, 30000, 0, 18000]), (torch.float16, 256, 32, 1, [30000, 18000, 2]),
+])
+def test_shares_longer_than_a_window_of_pages(cuda_device, wide, dtype, D, Hq, S, lengths):
+    """Sixteen heads in pages of 16 slots: a warp's share (of 148 multiprocessors with twelve of them each, eight at D = 256 or with
+    more than eight rows) is 40 pages and more, so that the window of 32 page numbers moves on, every slot of the ring is used again and
+    again, and the weights take several rounds.  Three of the heads are compared."""
+    H, page, heads = 16, 16, [0, 5, 15]
+    assert H * sum(lengths) / 16 / (148 * (8 if D == 256 or Hq // H * S > 8 else 12)) > 40
+    kv, table, n = make(cuda_device, lengths, H, D, page, dtype, seed=5)
+    if wide:
+        table = torch.cat((table, torch.full((len(lengths), 4 * table.shape[1]), -1, dtype=torch.int32, device=cuda_device)), 1)
+    q = rows(cuda_device, (len(lengths), Hq, S, D), dtype, 6, 2.0)
+    before = torch.rand(kv.shape[:3], device=cuda_device)
+    weight = before.clone()
+    o, lse = kc.cache4_attention(q, kv, table, n, 0.1, weight=weight, want_lse=True)
+    assert torch.equal(kc.cache4_attention(q, kv, table, n, 0.1), o)
+    some = [x.unflatten(1, (H, Hq // H))[:, heads].flatten(1, 2) for x in (o, q, lse)]
+    check_attention(some[0], some[1], kv[:, heads], table, n, 0.1, None, some[2], weight[:, heads], before[:, heads])
+    fa.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype,D,Hq,H,S", [(torch.float16, 64, 4, 2, 1), (torch.bfloat16, 128, 8, 2, 1), (torch.float16, 128, 24, 2, 1), (torch.bfloat16, 256, 2, 2, 2)])
+def test_shares_of_several_heads_and_sequences(cuda_device, wide, dtype, D, Hq, H, S):
+    """2000 ragged sequences: a warp's share goes from the last head of one to the heads of the next ones, past some without
+    tokens, and the second head of a short one has the pages of the first.  Every fortieth sequence is compared."""
+    B, page, n = 2000, 16, 260
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    lengths = torch.tensor([0, 1, 2, 5, 16, 33, 100, 260], dtype=torch.int32, device=cuda_device)[torch.randint(0, 8, (B,), generator=g, device=cuda_device)]
+    each = -(-n // page)
+    kv = torch.full((B * each + 3, H, page, 5 * D // 4), 255, dtype=torch.uint8, device=cuda_device)
+    table = torch.randperm(B * each + 3, generator=g, device=cuda_device)[: B * each].to(torch.int32).view(B, each)
+    k, v = (rows(cuda_device, (B, H, n, D), dtype, s) for s in (2, 3))
+    kc.cache4_append(k, v, kv, table, lengths, counts=lengths)
+    if wide:
+        table = torch.cat((table, torch.full((B, 4 * each), -1, dtype=torch.int32, device=cuda_device)), 1)
+    q = rows(cuda_device, (B, Hq, S, D), dtype, 6, 2.0)
+    before = torch.rand(kv.shape[:3], device=cuda_device)
+    weight = before.clone()
+    o, lse = kc.cache4_attention(q, kv, table, lengths, 0.1, weight=weight, want_lse=True)
+    assert torch.equal(kc.cache4_attention(q, kv, table, lengths, 0.1), o)
+    some = torch.arange(0, B, 40, device=cuda_device)
+    theirs = table[some, :each].long().flatten()
+    only = before.clone()
+    only[theirs] = weight[theirs]
+    check_attention(o[some], q[some], kv, table[some], lengths[some], 0.1, None, lse[some], only, before)
+    empty = lengths == 0
+    assert bool((o[empty] == 0).all()) and bool((lse[empty] == -math.inf).all()) and bool(torch.isfinite(o).all())
+    # every row of a softmax adds one to a head's tokens
+    seen = torch.minimum(lengths, torch.full_like(lengths, S)).sum()
+    assert abs(float((weight.double() - before.double()).sum()) - float(seen) * Hq) <= 2.0 ** -19 * 64 * float(seen) * Hq
+    fa.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length,budget,recent", [(33000, 500, 100), (50001, 4000, 0), (65536, 1, 1)])
+def test_evict_of_more_pages_than_are_kept_at_hand(cuda_device, length, budget, recent):
+    """Sequences of more than 2048 pages, which select looks up again in the table, and of more keys than shared memory holds."""
+    H, D, page = 2, 64, 16
+    pages = -(-length // page)
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    table = torch.randperm(2 * pages, generator=g, device=cuda_device)[:pages].to(torch.int32)[None]
+    kv = torch.randint(0, 256, (2 * pages, H, page, 5 * D // 4), generator=g, device=cuda_device, dtype=torch.uint8)
+    weight = torch.rand(kv.shape[:3], generator=g, device=cuda_device)
+    position = torch.randint(0, 10 ** 6, kv.shape[:3], generator=g, device=cuda_device, dtype=torch.int32)
+    want = [t.clone() for t in (kv, weight, position)]
+    slot = torch.arange(length, device=cuda_device)
+    pg, off = table[0].long()[slot // page], slot % page
+    for h in range(H):
+        moves, _ = ref.evict(weight[pg, h, off], position[pg, h, off], budget, recent)
+        if moves:
+            to, frm = torch.tensor(moves, device=cuda_device).T
+            for x, y in zip(want, (kv, weight, position)):
+                x[pg[to], h, off[to]] = y[pg[frm], h, off[frm]]
+    new = kc.cache4_evict(kv, weight, position, table, torch.tensor([length], dtype=torch.int32, device=cuda_device), budget, recent)
+    assert new.tolist() == [budget]
+    for got, exp in zip((kv, weight, position), want):
+        assert torch.equal(got, exp)
+    fa.device_status()
