@@ -20,12 +20,16 @@
 // the device takes an equal, contiguous share of it, whatever the lengths are.  A share's first and last item may
 // continue in other warps: their sums go to a workspace and a second kernel joins them.
 //
-// What bounds it: not HBM, 5 D / 4 bytes per token and K/V head, but some 320 instructions per 16 tokens, K/V head and 8
-// rows, at the rate at which three warps per scheduler, all that registers allow, keep it busy: 56 % of the issue slots.
+// What bounds it: not HBM, 5 D / 4 bytes per token and K/V head, but some 355 instructions per 16 tokens, K/V head and 8
+// rows (528 for 16), at the rate at which three warps per scheduler (two), all that registers allow, keep it busy: 57 % of the
+// issue slots (49 %).
 // (Tensor cores of the newer kind want 128-row operands in shared memory; here 8 rows meet codes that exist unpacked in
 // registers only.)  Times with 128 dims, against the time for the bytes alone: one sequence of 131072 tokens,
-// 8 heads, 51.0 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 85 us (53); 256 sequences of 200
-// tokens 39 us (11); one of 500 tokens 9.5 us, two dependent kernels.
+// 8 heads, 51.2 us (25.6; 3.3 TB/s); 64 sequences of 1 to 8192 tokens, 32 heads over 8, 87 us (53); 256 sequences of 200
+// tokens 40.6 us (11); one of 500 tokens 9.5 us, two dependent kernels.
+//
+// More than 16 rows are blocks of 16 (8 at D = 256) that each read and unpack the cache again: made for decoding and a few tokens to
+// verify.  512 new tokens over 8192 held, 32 heads over 8 of 128 dims, take 491 us (144 TFLOP/s, 9 % of the dense rate), 2048 2.2 ms.
 #include "../../include/rsfa.h"
 #include "ops_common.cuh"
 
@@ -37,10 +41,10 @@ constexpr int kJoinThreads = 128, kJoinMost = 512;
 // Tokens per tile: what a tile costs apart from its tokens is spread over 5 KB (10 KB) of them.
 __host__ __device__ constexpr int tile_tokens(int D) { return D == 64 ? 64 : 32; }
 // One CTA per multiprocessor: as many warps as the registers of their accumulators allow, and slots of a warp's ring by the
-// shared memory that is left.  (Three CTAs of four warps: the same loop, but three times the CTAs to start, 256 sequences of
-// 200 tokens in 48 us for 39.  Sixteen rows of 64 dims by 8 warps without spills, 16 sequences of 16384 tokens, 64 heads over
-// 4, in 45.3 us; by 12 with them in 49.2.  Eight rows by 16 warps with two slots: 32 sequences of 16384 tokens 85.7 us for
-// 89.3, 16 of up to 2048 tokens 24.1 for 21.5, left at 12.)
+// shared memory that is left.  (When they were measured: three CTAs of four warps, the same loop, but three times the CTAs to
+// start, 256 sequences of 200 tokens in 48 us for 39.  Sixteen rows of 64 dims by 8 warps without spills, 16 sequences of 16384
+// tokens, 64 heads over 4, in 45.3 us; by 12 with them in 49.2.  Eight rows by 16 warps with two slots: 32 sequences of 16384
+// tokens 85.7 us for 89.3, 16 of up to 2048 tokens 24.1 for 21.5, left at 12.)
 template <int D, int NT>
 struct Shape {
   static constexpr int kWarps = D == 256 || NT == 2 ? 8 : 12, kThreads = 32 * kWarps;
@@ -1206,9 +1210,11 @@ size_t score_bytes(const Cache4& c, int rows) {
   return tiles * rows * tile_tokens(c.D) * sizeof(float);
 }
 // The scores are kept for the weights where a token's fit beside its record: one block of rows, and no more than half
-// of what the cache itself takes (a table may allow for far longer sequences than there are pages).  Four sequences of
-// 32768 tokens, 8 heads, kept against computed again, us: D = 128, 1 / 8 / 16 rows, 66 / 78 / 122 against 111 / 117 / 133;
-// D = 64, 8 / 16 rows, 63 / 91 against 84 / 91; D = 256, 8 rows, 114 against 157.
+// of what the cache itself takes.  They are placed by slot, so what counts is how long the table lets sequences be, which may be far
+// more than there are pages: 2 sequences of 131072 tokens, 64 heads over 8, bf16, with a table that fits and one four times as
+// wide, 109 and 181 us (D = 128), 76 and 130 (D = 64).  Four sequences of 32768 tokens, 8 heads, fp16, kept against computed
+// again, us: D = 128, 8 / 16 rows, 65 / 99 against 102 / 127; D = 64, 8 rows, 47 against 73 (16 are always computed again, 87);
+// D = 256, 8 rows, 98 against 146.
 bool keeps_scores(const Cache4& c, int Hq, int S) {
   const int rows = Hq / c.H * S, block = sixteen_rows(c.D, rows) ? 16 : 8;
   const size_t cache_bytes = (static_cast<size_t>(c.pages) << c.page_shift) * c.H * (c.D * 5 / 4);

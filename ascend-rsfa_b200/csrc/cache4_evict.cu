@@ -10,7 +10,7 @@
 // lists the moves by prefix sums over the slots.  move: the listed records, spread over the whole device.
 // What bounds it: the latency of the passes over n keys of one CTA and, where heads are fewer than multiprocessors, that one
 // CTA's shared memory; the traffic, 8 bytes per token and 2 * 5 D / 4 per move, is small next to a step's attention.
-// 256 heads of 2049 slots: select 13.0 us, one move each 3.7 us.  32 heads of 16384 slots cut to a quarter: select 18.5 us,
+// 256 heads of 2049 slots: select 12.9 us, one move each 3.9 us.  32 heads of 16384 slots cut to a quarter: select 18.6 us,
 // move 4.5 us.
 #include "../../include/rsfa.h"
 #include "ops_common.cuh"
@@ -272,7 +272,8 @@ cudaError_t launch_cache4_evict(const Cache4& c, const Cache4Evict& ev, int sm_c
   const int heads = c.B * c.H;
   cudaError_t e;
   // Short sequences with 256 threads, of which every multiprocessor holds several CTAs: 256 heads of 2049 slots
-  // 15.5 -> 13.0 us.
+  // 15.5 -> 13.0 us of select alone.  (By what the table allows, as the lengths are on the device; with the move behind it, which
+  // starts while select ends, a call takes 17.7 us with a table that fits and 17.0 with one of 131072 slots.)
   if (room <= 4096) {
     e = launch_persistent(cache4_select_kernel<256>, heads, 256, smem, stream, option_pdl() != 0, c, ev);
   } else {

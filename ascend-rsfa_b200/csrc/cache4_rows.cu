@@ -7,8 +7,9 @@
 // What bounds it: HBM for prompts, the launch for single tokens.  A thread that reads has eight dims, one 16-byte access of
 // the dense row; one that appends has 16, so that a group is two lanes, its range one shuffle and its scale computed by
 // no more than these two (eight: 77 us for 59).  With 8 heads of 128 dims, bf16: 4 sequences of 12288 new tokens are
-// appended in 59 us (4.5 TB/s; the instructions of ranges and codes bound it, HBM's time is 40), 8 sequences of up to 4096
-// tokens, padded, read in 29 us (5.4 TB/s), one token of each of 64 sequences appended or read in 2.7 us.
+// appended in 59 us (4.5 TB/s; the instructions of ranges and codes bound it, 76 % of the issue slots; HBM's time is 40), 8
+// sequences of up to 4096 tokens, padded, read in 29 us (5.4 TB/s, 77 % of the ALUs), one token of each of 64 sequences appended or
+// read in 2.7 us.
 #include "../../include/rsfa.h"
 #include "ops_common.cuh"
 
