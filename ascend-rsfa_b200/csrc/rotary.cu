@@ -10,8 +10,9 @@
 // the data they turn, are read once for all of these heads.  16 sequences of 4096 positions, 16 + 16 heads of 128 dims,
 // bf16: 163.2 us, 6.6 TB/s, what a plain copy of these bytes takes; 8 of 1000, 32 + 8 heads, 64 of 128 dims turned: 28.0 us
 // interleaved and 30.0 in halves (5.8 and 5.5 TB/s).  Where the dims that turn are no multiple of 16 (8 interleaved), a thread has
-// one pair in accesses of two bytes: 8, 20, 24 or 30 of the 128 dims in halves 70 us, 20 or 30 interleaved 63.  The table of 131072 positions by 64 frequencies, 67 MB, takes 13.3 us (5.1 TB/s): its
-// sines and cosines, one pair per 8 bytes, are about as long as their stores.
+// one pair in accesses of two bytes: 8, 20, 24 or 30 of the 128 dims in halves 70 us, 20 or 30 interleaved 63.  The table of
+// 131072 positions by 64 frequencies, 67 MB, takes 13.3 us (5.1 TB/s): its sines and cosines, one pair per 8 bytes, are about as
+// long as their stores.
 #include "../../include/rsfa.h"
 #include "ops_common.cuh"
 
